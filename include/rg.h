@@ -299,6 +299,73 @@ rg_status rg_groundtruth_mem(const float *base, uint32_t nb, uint32_t bstride, c
 rg_status rg_groundtruth(const char *base_fbin, const char *query_fbin, const char *gt_out, int metric, uint32_t K,
                          const int *devices, int ndev);
 
+/* ------------------------------------------------- softmax over a base (training)
+ * A table of embeddings seen as the classes of a classifier: the logits of query i are z_ij = scale * <q_i, b_j> over ALL rows j of
+ * the base (cosine: normalise the rows first, rg_normalize_rows).  Softmax cross entropy against one row per query -- the ids that
+ * rg_gt_* or a labelled set give --, and its gradient, without ever storing the nq x nb logits.  No counterpart in the reference: it is
+ * what trains the tables the reference indexes.
+ *
+ *   lse_i  = log sum_j exp(z_ij)                    own_i = z_{i, target_i}      loss_i = lse_i - own_i
+ *   rest_i = log sum_{j != target_i} exp(z_ij)      mean_i = sum_{j != target_i} exp(z_ij - rest_i) b_j
+ *   p_ij   = exp(z_ij - lse_i)                      w = dL/dloss
+ *   dq_i   = w_i scale (exp(rest_i - lse_i) mean_i - (1 - exp(-loss_i)) b_target)
+ *   db_j   = scale sum_i w_i (p_ij - [target_i = j]) q_i
+ * (the target is kept out of the sums: where a query is answered well, loss and gradient are made of what the others leave, and
+ * lse_i - own_i or mean minus target would lose it)
+ *
+ * Rows are `dtype` (RG_DTYPE_*; base, queries and their gradients alike), row strides in elements (any stride >= dim, any alignment of
+ * the element; rows of 16-byte aligned strides and bases load fastest), dim 1 .. 1024, sums in fp32.  fp32 rows are multiplied as pairs
+ * of 16-bit halves (22 bits of every element, relative to the largest of its row).  Targets are global ids (row + id_base);
+ * 0xffffffff = the query has no row: loss 0, no gradient.  A target no shard holds: own = -inf, loss = +inf.
+ *
+ * Shard form, like rg_gt_shard_dev: a rank holds rows [id_base, id_base + nb).  rg_softmax_shard_dev gives rest and own over the shard
+ * (-inf where the shard has no such row, mean 0 where it has none at all), rg_softmax_merge_dev joins nlists of them ([list][nq]) into
+ * the lse and the loss over the whole base, rg_softmax_grad_dev gives the shard's part of dq (the sum over the shards is dq) and the
+ * shard's rows of db.  Where one shard is the whole base its d_lse and d_loss are what the gradient takes, and no merge is needed.
+ *
+ * d_lse, d_loss, d_mean (fp32 [nq][dim]; kept for dq, at the precision dq is written in) may be NULL in rg_softmax_shard_dev, d_dq or
+ * d_db in rg_softmax_grad_dev.  d_work: scratch of rg_softmax_workspace() bytes (256-byte aligned, contents undefined before and after;
+ * calls that may run at the same time -- other streams, captured graphs -- need scratch of their own).  All calls enqueue on `stream` and
+ * return without synchronising; they can be captured.  Results do not depend on timing: the same call gives the same bits. */
+enum { RG_DTYPE_F32 = 0, RG_DTYPE_F16 = 1, RG_DTYPE_BF16 = 2 };
+enum { RG_SOFTMAX_STATS = 0, RG_SOFTMAX_MEAN = 1, RG_SOFTMAX_GRAD = 2 }; /* rg_softmax_shard_dev without / with d_mean, rg_softmax_grad_dev */
+/* nb: of the gradient, the rows d_db asks for (0 without d_db) */
+rg_status rg_softmax_workspace(int what, uint32_t nb, uint32_t nq, uint32_t dim, int dtype, uint64_t *bytes);
+rg_status rg_softmax_shard_dev(const void *d_base, uint32_t nb, uint64_t bstride, const void *d_queries, uint32_t nq, uint64_t qstride,
+                               uint32_t dim, int dtype, float scale, const uint32_t *d_targets, uint32_t id_base, float *d_rest,
+                               float *d_own, float *d_lse, float *d_loss, float *d_mean, void *d_work, uint64_t work_bytes, int device,
+                               void *stream);
+rg_status rg_softmax_merge_dev(const float *d_rest_in, const float *d_own_in, uint32_t nlists, uint32_t nq, const uint32_t *d_targets,
+                               float *d_lse, float *d_loss, int device, void *stream);
+/* d_lse, d_loss: over the whole base; d_rest, d_mean: what rg_softmax_shard_dev gave for this shard (only read for d_dq);
+ * d_weights [nq]: dL/dloss.  d_dq [nq][dqstride], d_db [nb][dbstride], dtype; only dim elements of a row are written. */
+rg_status rg_softmax_grad_dev(const void *d_base, uint32_t nb, uint64_t bstride, const void *d_queries, uint32_t nq, uint64_t qstride,
+                              uint32_t dim, int dtype, float scale, const uint32_t *d_targets, uint32_t id_base, const float *d_lse,
+                              const float *d_loss, const float *d_rest, const float *d_mean, const float *d_weights, void *d_dq,
+                              uint64_t dqstride, void *d_db, uint64_t dbstride, void *d_work, uint64_t work_bytes, int device,
+                              void *stream);
+
+/* ------------------------------------------------------------ a base in 4 bits
+ * A base in an eighth of its fp32 bytes, scored exhaustively: 4-bit codes, one fp16 scale (and, optionally, one fp16 minimum) per group of
+ * 32, 64 or 128 consecutive elements of a row.  No counterpart in the reference; stands beside rg_score_batch.
+ *   codes   [nb][cstride] bytes, element k of a row in byte k / 2, even elements in the low half; cstride % 4 == 0, >= ceil(dim / 8) * 4
+ *   scales  [nb][sstride] fp16, group k / group; mins alike (NULL: none)
+ *   value   scale * (code - 8) without minima, scale * code + min with them
+ * rg_q4_pack_dev: scale = fp16(max|x| * (1/7)) resp. min = fp16(min x), scale = fp16((max x - min x) * (1/15)), the products in fp32; code =
+ * the nearest level (ties to the even code), padding codes 0.  Rows must be finite; values whose scale leaves fp16's range (6e-8 .. 65504)
+ * are scaled by the caller first.
+ * rg_q4_unpack_dev: the fp32 values of the rows `d_ids` lists (NULL: rows 0 .. n-1) -- for an exact re-score or further training.
+ * rg_q4_score_dev: out[i][j] = <q_i, value of row j>, fp32 sums, dim 1 .. 4096; queries fp32 / fp16 / bf16.
+ * Enqueued on `stream`, no scratch, capturable. */
+rg_status rg_q4_pack_dev(const void *d_rows, uint32_t nb, uint64_t stride, uint32_t dim, int dtype, uint32_t group, uint8_t *d_codes,
+                         uint64_t cstride, uint16_t *d_scales, uint16_t *d_mins, uint64_t sstride, int device, void *stream);
+rg_status rg_q4_unpack_dev(const uint8_t *d_codes, uint64_t cstride, const uint16_t *d_scales, const uint16_t *d_mins, uint64_t sstride,
+                           uint32_t nb, uint32_t dim, uint32_t group, const uint32_t *d_ids, uint32_t n, float *d_out, uint64_t ostride,
+                           int device, void *stream);
+rg_status rg_q4_score_dev(const uint8_t *d_codes, uint64_t cstride, const uint16_t *d_scales, const uint16_t *d_mins, uint64_t sstride,
+                          uint32_t nb, uint32_t dim, uint32_t group, const void *d_queries, uint32_t nq, uint64_t qstride, int dtype,
+                          float *d_out, uint64_t ostride, int device, void *stream);
+
 /* --------------------------------------------------------- graph construction
  * Replaces: IndexBipartite::BuildRoarGraph(n_sq, nullptr, n_bp, base, params{M_sq, M_pjbp, L_pjpq, num_threads})
  * after LoadLearnBaseKNN (tests/test_build_roargraph.cpp:117-136; src/index_bipartite.cpp:143-233, 1043-1277).

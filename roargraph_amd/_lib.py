@@ -24,6 +24,7 @@ SYMBOLS = [
     "rg_score_batch", "rg_score_batch_dev", "rg_search", "rg_search_sharded", "rg_search_dev", "rg_search_wait", "rg_search_prepare", "rg_search_reuse_stats",
     "rg_gt_shard_dev", "rg_gt_merge_dev", "rg_groundtruth_mem", "rg_groundtruth",
     "rg_comm_unique_id", "rg_comm_init_rank", "rg_comm_init_local", "rg_comm_uses_rccl", "rg_comm_destroy", "rg_gt_exchange_plan", "rg_groundtruth_rank", "rg_build_roargraph", "rg_build_roargraph_gpu", "rg_build_schedule", "rg_build_prune_debug", "rg_projection_ep", "rg_projection_ep_dev",
+    "rg_softmax_workspace", "rg_softmax_shard_dev", "rg_softmax_merge_dev", "rg_softmax_grad_dev", "rg_q4_pack_dev", "rg_q4_unpack_dev", "rg_q4_score_dev",
 ]
 
 

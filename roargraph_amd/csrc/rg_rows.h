@@ -1,0 +1,46 @@
+// rg_rows.h -- what the operators over typed rows (rg_softmax*.hip, rg_q4.hip) share: element types, the guard around the current device.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <string>
+
+#include "rg.h"
+#include "rg_internal.h"
+
+#define RG_HIP(expr)                                                                                   \
+    do {                                                                                               \
+        hipError_t e_ = (expr);                                                                        \
+        if (e_ != hipSuccess)                                                                          \
+            return set_error(RG_ERR_DEVICE, std::string(#expr) + ": " + hipGetErrorString(e_));        \
+    } while (0)
+
+namespace rg {
+
+template <int DT> struct Elem;
+template <> struct Elem<RG_DTYPE_F32> { typedef float T; };
+template <> struct Elem<RG_DTYPE_F16> { typedef _Float16 T; };
+template <> struct Elem<RG_DTYPE_BF16> { typedef __bf16 T; };
+
+inline bool known_dtype(int dtype) { return dtype == RG_DTYPE_F32 || dtype == RG_DTYPE_F16 || dtype == RG_DTYPE_BF16; }
+inline uint32_t elem_bytes(int dtype) { return dtype == RG_DTYPE_F32 ? 4 : 2; }
+
+// makes `device` current for a call, and the caller's device current again afterwards
+struct OnDevice {
+    int before = -1;
+    rg_status st = RG_OK;
+    explicit OnDevice(int device) {
+        int n = 0;
+        if (hipGetDeviceCount(&n) != hipSuccess || n <= 0)
+            st = set_error(RG_ERR_DEVICE, "no HIP device visible: the gfx950 path cannot run (there is no CPU fallback)");
+        else if (device < 0 || device >= n)
+            st = set_error(RG_ERR_ARG, "no such device");
+        else if (hipGetDevice(&before) != hipSuccess || (before != device && hipSetDevice(device) != hipSuccess))
+            st = set_error(RG_ERR_DEVICE, "cannot use the device");
+        if (st != RG_OK || before == device) before = -1;
+    }
+    ~OnDevice() { if (before >= 0) (void)hipSetDevice(before); }
+    OnDevice(const OnDevice &) = delete;
+    OnDevice &operator=(const OnDevice &) = delete;
+};
+
+}  // namespace rg

@@ -1,0 +1,86 @@
+"""A base in 4 bits: codes with one fp16 scale (and, optionally, minimum) per group of elements of a row, scored exhaustively.
+
+    packed = q4_pack(base_t, group=32)             # an eighth of the fp32 bytes, and the scales
+    scores = q4_score(queries_t, packed)           # [nq, nb] fp32 inner products
+    rows = q4_unpack(packed, ids)                  # fp32 values of some rows, for an exact re-score
+
+Thin host layer over the C ABI (rg_q4_*, include/rg.h); everything is torch CUDA tensors, enqueued on the current stream.
+"""
+import ctypes as C
+from collections import namedtuple
+
+from ._lib import check, lib
+from .softmax import _device, _dtype_code, _ptr, _rows, _stream, _stride
+
+# codes uint8 [nb, >= ceil(dim / 8) * 4], scales fp16 [nb, ceil(dim / group)], mins alike or None (rg.h: "a base in 4 bits")
+Q4Base = namedtuple("Q4Base", "codes scales mins dim group")
+
+
+def _check_form(p):
+    import torch
+    groups = -(-p.dim // p.group)
+    nb = p.codes.shape[0]
+    if p.codes.dtype != torch.uint8 or p.codes.dim() != 2 or p.codes.stride(1) != 1 or not p.codes.is_cuda:
+        raise ValueError("codes: rows of uint8 on a GPU are wanted")
+    if p.codes.shape[1] < -(-p.dim // 8) * 4:
+        raise ValueError("codes: %d bytes a row, dim %d needs %d" % (p.codes.shape[1], p.dim, -(-p.dim // 8) * 4))
+    for t, name in ((p.scales, "scales"), (p.mins, "mins")):
+        if t is None and name == "mins":
+            continue
+        if t.dtype != torch.float16 or t.shape != (nb, groups) or t.device != p.codes.device or (groups > 1 and t.stride(1) != 1):
+            raise ValueError("%s: fp16 [%d, %d] on %s is wanted" % (name, nb, groups, p.codes.device))
+    if p.mins is not None and nb > 1 and p.mins.stride(0) != p.scales.stride(0):
+        raise ValueError("scales and mins have one row stride")
+
+
+def q4_pack(base_t, group=32, mins=False):
+    """rg_q4_pack_dev: rows (fp32 / fp16 / bf16) -> Q4Base."""
+    import torch
+    base_t = _rows(base_t, "base")
+    code = _dtype_code(base_t)
+    nb, dim = base_t.shape
+    if group not in (32, 64, 128):
+        raise ValueError("groups of 32, 64 or 128 elements")
+    groups = -(-dim // group)
+    codes = torch.empty((nb, -(-dim // 8) * 4), dtype=torch.uint8, device=base_t.device)
+    both = torch.empty((2 if mins else 1, nb, groups), dtype=torch.float16, device=base_t.device)
+    low = both[1] if mins else None
+    check(lib().rg_q4_pack_dev(_ptr(base_t), C.c_uint32(nb), _stride(base_t), C.c_uint32(dim), C.c_int(code), C.c_uint32(group), _ptr(codes),
+                               C.c_uint64(codes.shape[1]), _ptr(both[0]), _ptr(low), C.c_uint64(groups), C.c_int(_device(base_t)), _stream(base_t)))
+    return Q4Base(codes, both[0], low, dim, group)
+
+
+def q4_unpack(packed, ids=None):
+    """rg_q4_unpack_dev: fp32 values of all rows, or of the rows `ids` (int32 / int64 on the GPU; an id that is no row gives NaN)."""
+    import torch
+    _check_form(packed)
+    nb = packed.codes.shape[0]
+    if ids is not None:
+        if ids.dim() != 1 or ids.device != packed.codes.device or ids.dtype not in (torch.int32, torch.int64):
+            raise ValueError("ids: a vector of int32 or int64 on %s is wanted" % packed.codes.device)
+        ids = ids.to(torch.int32).contiguous()
+    n = nb if ids is None else ids.shape[0]
+    out = torch.empty((n, packed.dim), dtype=torch.float32, device=packed.codes.device)
+    check(lib().rg_q4_unpack_dev(_ptr(packed.codes), _stride(packed.codes), _ptr(packed.scales), _ptr(packed.mins), _stride(packed.scales), C.c_uint32(nb),
+                                 C.c_uint32(packed.dim), C.c_uint32(packed.group), _ptr(ids), C.c_uint32(n), _ptr(out), C.c_uint64(packed.dim),
+                                 C.c_int(_device(out)), _stream(out)))
+    return out
+
+
+def q4_score(queries_t, packed, out=None):
+    """rg_q4_score_dev: inner products [nq, nb], fp32, of the queries (fp32 / fp16 / bf16) with every row."""
+    import torch
+    _check_form(packed)
+    queries_t = _rows(queries_t, "queries")
+    code = _dtype_code(queries_t)
+    nq, nb = queries_t.shape[0], packed.codes.shape[0]
+    if queries_t.shape[1] != packed.dim or queries_t.device != packed.codes.device:
+        raise ValueError("queries: %d columns on %s are wanted, got %d on %s" % (packed.dim, packed.codes.device, queries_t.shape[1], queries_t.device))
+    if out is None:
+        out = torch.empty((nq, nb), dtype=torch.float32, device=queries_t.device)
+    elif out.shape != (nq, nb) or out.dtype != torch.float32 or out.device != queries_t.device or (nb > 1 and out.stride(1) != 1) or (nq > 1 and out.stride(0) < nb):
+        raise ValueError("out: fp32 rows [%d, %d] on %s are wanted" % (nq, nb, queries_t.device))
+    check(lib().rg_q4_score_dev(_ptr(packed.codes), _stride(packed.codes), _ptr(packed.scales), _ptr(packed.mins), _stride(packed.scales), C.c_uint32(nb),
+                                C.c_uint32(packed.dim), C.c_uint32(packed.group), _ptr(queries_t), C.c_uint32(nq), _stride(queries_t), C.c_int(code),
+                                _ptr(out), _stride(out), C.c_int(_device(out)), _stream(out)))
+    return out

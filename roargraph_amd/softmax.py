@@ -1,0 +1,172 @@
+"""Softmax cross entropy over ALL rows of a base: trains the tables and towers that the index serves.
+
+    loss = softmax_loss(queries, base, targets, scale=1 / temperature)      # [nq] fp32, differentiable in queries and base
+    loss.mean().backward()
+
+queries [nq, dim] and base [nb, dim] are torch CUDA tensors of one dtype (fp32, fp16, bf16); targets [nq] holds the row of the base that
+answers each query (e.g. column 0 of the ground truth; for cosine normalise the rows first), -1 where there is none (loss 0, no gradient).
+The nq x nb logits are never stored.  Thin host layer over the C ABI (rg_softmax_*, include/rg.h); the multi-GPU form holds a row shard of
+the base per rank, like the ground truth.
+"""
+import ctypes as C
+
+from ._lib import check, lib
+
+STATS, MEAN, GRAD = 0, 1, 2
+
+
+def _dtype_code(t):
+    import torch
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}.get(t.dtype)
+    if code is None:
+        raise TypeError("rows are fp32, fp16 or bf16, got %s" % t.dtype)
+    return code
+
+
+def _rows(t, name):
+    """t itself where its rows can be read in place, else a contiguous copy (transposed or broadcast tensors)."""
+    if t.dim() != 2:
+        raise ValueError("%s: a matrix of rows is wanted, got shape %s" % (name, tuple(t.shape)))
+    if t.stride(1) == 1 and t.stride(0) >= t.shape[1] or t.is_contiguous():
+        return t
+    return t.contiguous()
+
+
+def _stride(t):
+    return C.c_uint64(max(t.stride(0), t.shape[1]))     # (a single row's stride may be anything)
+
+
+def _ptr(t):
+    return C.c_void_p(t.data_ptr() if t is not None else None)
+
+
+def _stream(t):
+    import torch
+    return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+def _device(t):
+    return t.device.index or 0
+
+
+def _check_pair(queries, base):
+    if not queries.is_cuda or queries.device != base.device:
+        raise ValueError("queries and base live on one GPU, got %s and %s" % (queries.device, base.device))
+    if queries.dtype != base.dtype:
+        raise TypeError("queries and base have one dtype, got %s and %s" % (queries.dtype, base.dtype))
+    if queries.shape[1] != base.shape[1]:
+        raise ValueError("queries have %d columns, the base has %d" % (queries.shape[1], base.shape[1]))
+
+
+def _check_vector(t, n, dtype, like, name):
+    if t.dim() != 1 or t.shape[0] != n or t.dtype != dtype or t.device != like.device:
+        raise ValueError("%s: %d values of %s on %s are wanted, got %s of %s on %s" % (name, n, dtype, like.device, tuple(t.shape), t.dtype, t.device))
+    return t.contiguous()
+
+
+def _targets(targets, n, like):
+    """ids as 32 bits (int64 ids are narrowed: -1 and ids up to 2^32 - 2 keep their meaning)"""
+    import torch
+    if targets.dtype == torch.int64:
+        targets = targets.to(torch.int32)
+    return _check_vector(targets, n, torch.int32, like, "targets")
+
+
+def workspace(what, nb, nq, dim, dtype_code):
+    """rg_softmax_workspace: bytes of scratch of one call"""
+    n = C.c_uint64()
+    check(lib().rg_softmax_workspace(C.c_int(what), C.c_uint32(nb), C.c_uint32(nq), C.c_uint32(dim), C.c_int(dtype_code), C.byref(n)))
+    return n.value
+
+
+def _scratch(what, nb, nq, dim, like):
+    import torch
+    n = workspace(what, nb, nq, dim, _dtype_code(like))
+    return torch.empty(max(n, 256), dtype=torch.uint8, device=like.device), n
+
+
+def softmax_shard_dev(base_t, queries_t, targets_t, scale, id_base=0, want_mean=False):
+    """rg_softmax_shard_dev on the current stream: (rest, own, lse, loss, mean) of one row shard, fp32; lse and loss as if the shard were the
+    whole base; mean is None unless asked for."""
+    import torch
+    queries_t, base_t = _rows(queries_t, "queries"), _rows(base_t, "base")
+    _check_pair(queries_t, base_t)
+    nq, nb, dim = queries_t.shape[0], base_t.shape[0], base_t.shape[1]
+    targets_t = _targets(targets_t, nq, base_t)
+    rest, own, lse, loss = torch.empty((4, nq), dtype=torch.float32, device=base_t.device).unbind(0)
+    mean = torch.empty((nq, dim), dtype=torch.float32, device=base_t.device) if want_mean else None
+    work, n = _scratch(MEAN if want_mean else STATS, nb, nq, dim, base_t)
+    check(lib().rg_softmax_shard_dev(_ptr(base_t), C.c_uint32(nb), _stride(base_t), _ptr(queries_t), C.c_uint32(nq), _stride(queries_t),
+                                     C.c_uint32(dim), C.c_int(_dtype_code(base_t)), C.c_float(scale), _ptr(targets_t), C.c_uint32(id_base),
+                                     _ptr(rest), _ptr(own), _ptr(lse), _ptr(loss), _ptr(mean), _ptr(work), C.c_uint64(n), C.c_int(_device(base_t)),
+                                     _stream(base_t)))
+    return rest, own, lse, loss, mean
+
+
+def softmax_merge_dev(rest_in, own_in, targets_t):
+    """rg_softmax_merge_dev: statistics [nlists, nq] of the row shards -> (lse, loss) over the whole base."""
+    import torch
+    if rest_in.dim() != 2 or rest_in.shape != own_in.shape or rest_in.dtype != torch.float32 or own_in.dtype != torch.float32 or rest_in.device != own_in.device:
+        raise ValueError("rest and own: two fp32 matrices [nlists, nq] on one GPU are wanted")
+    rest_in, own_in = rest_in.contiguous(), own_in.contiguous()
+    targets_t = _targets(targets_t, rest_in.shape[1], rest_in)
+    lse, loss = torch.empty((2, rest_in.shape[1]), dtype=torch.float32, device=rest_in.device).unbind(0)
+    check(lib().rg_softmax_merge_dev(_ptr(rest_in), _ptr(own_in), C.c_uint32(rest_in.shape[0]), C.c_uint32(rest_in.shape[1]), _ptr(targets_t),
+                                     _ptr(lse), _ptr(loss), C.c_int(_device(rest_in)), _stream(rest_in)))
+    return lse, loss
+
+
+def softmax_grad_dev(base_t, queries_t, targets_t, scale, lse, loss, weights, rest=None, mean=None, id_base=0, want_dq=True, want_db=True):
+    """rg_softmax_grad_dev: (this shard's part of dq, the shard's rows of db).  lse, loss: over the whole base; rest, mean: this shard's
+    (for dq only); weights = dL/dloss [nq]."""
+    import torch
+    queries_t, base_t = _rows(queries_t, "queries"), _rows(base_t, "base")
+    _check_pair(queries_t, base_t)
+    nq, nb, dim = queries_t.shape[0], base_t.shape[0], base_t.shape[1]
+    targets_t = _targets(targets_t, nq, base_t)
+    lse, loss, weights = (_check_vector(t, nq, torch.float32, base_t, name) for t, name in ((lse, "lse"), (loss, "loss"), (weights, "weights")))
+    if want_dq:
+        if rest is None or mean is None or mean.shape != (nq, dim) or mean.dtype != torch.float32 or mean.device != base_t.device or not mean.is_contiguous():
+            raise ValueError("rest and mean: the results of softmax_shard_dev(..., want_mean=True) are wanted")
+        rest = _check_vector(rest, nq, torch.float32, base_t, "rest")
+    dq = torch.empty((nq, dim), dtype=base_t.dtype, device=base_t.device) if want_dq else None
+    db = torch.empty((nb, dim), dtype=base_t.dtype, device=base_t.device) if want_db else None
+    work, n = _scratch(GRAD, nb if want_db else 0, nq, dim, base_t)
+    check(lib().rg_softmax_grad_dev(_ptr(base_t), C.c_uint32(nb), _stride(base_t), _ptr(queries_t), C.c_uint32(nq), _stride(queries_t),
+                                    C.c_uint32(dim), C.c_int(_dtype_code(base_t)), C.c_float(scale), _ptr(targets_t), C.c_uint32(id_base),
+                                    _ptr(lse), _ptr(loss), _ptr(rest), _ptr(mean), _ptr(weights), _ptr(dq), C.c_uint64(dim), _ptr(db), C.c_uint64(dim),
+                                    _ptr(work), C.c_uint64(n), C.c_int(_device(base_t)), _stream(base_t)))
+    return dq, db
+
+
+_function = None
+
+
+def _softmax_function():
+    global _function
+    if _function is None:
+        import torch
+
+        class SoftmaxLoss(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, queries, base, targets, scale):
+                rest, _, lse, loss, mean = softmax_shard_dev(base, queries, targets, scale, want_mean=ctx.needs_input_grad[0])
+                ctx.save_for_backward(queries, base, targets, lse, loss, rest, mean)
+                ctx.scale = scale
+                return loss
+
+            @staticmethod
+            @torch.autograd.function.once_differentiable
+            def backward(ctx, weights):
+                queries, base, targets, lse, loss, rest, mean = ctx.saved_tensors
+                dq, db = softmax_grad_dev(base, queries, targets, ctx.scale, lse, loss, weights, rest=rest, mean=mean, want_dq=ctx.needs_input_grad[0], want_db=ctx.needs_input_grad[1])
+                return dq, db, None, None
+
+        _function = SoftmaxLoss
+    return _function
+
+
+def softmax_loss(queries, base, targets, scale=1.0):
+    """Cross entropy of softmax(scale * queries @ base.T) against `targets`, per query [nq] fp32; differentiable (once) in queries and base."""
+    targets = _targets(targets, queries.shape[0], base)
+    return _softmax_function().apply(queries, base, targets, float(scale))
