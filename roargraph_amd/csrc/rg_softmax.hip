@@ -20,112 +20,14 @@
 #include "rg.h"
 #include "rg_internal.h"
 #include "rg_rows.h"
+#include "rg_softmax_pass.h"
 
 namespace rg {
 namespace {
 
 constexpr uint32_t kMaxDim = 1024;
 constexpr uint32_t kCUs = 256;             // MI355X; the workspace query needs no device
-constexpr uint32_t kNoTarget = 0xffffffffu;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-enum { kStats = 0, kMean = 1, kRows = 2 };
-
-struct PassArgs {
-    const void *x, *y;                 // stationary and streamed rows
-    uint64_t xstride, ystride;
-    uint32_t nx, ny, dim;
-    float k;                           // scale * log2 e
-    uint32_t nsplit, rows_per_split;   // of y
-    float2 *ml;                        // [slot][nx] reference M and sum l
-    float *o;                          // [slot][nx][dim] (kMean, kRows)
-    const uint32_t *targets;           // kStats, kMean: per x (global ids)
-    uint32_t id_base;
-    float *own2;                       // kStats, kMean: z2 of the target, written where it is met
-    const float4 *yparam;              // kRows, per y: bias, log2(|w| (1 - p_target)), sign, target row of the shard (bits)
-    void *out;                         // kRows in one piece: the gradient itself
-    uint64_t ostride;
-    float oscale;
-};
-
-constexpr int kT = 16;
-
-template <int DT, int MODE>
-__global__ void __launch_bounds__(256) rg_softmax_pass_kernel(PassArgs A) {
-    typedef typename Elem<DT>::T T;
-    extern __shared__ float lds[];
-    const uint32_t dim = A.dim, pitch = dim + 1, tid = threadIdx.x, r = tid / kT, c = tid % kT;
-    float *X = lds, *Y = X + kT * pitch, *P = Y + kT * pitch;
-    const uint32_t ntx = (A.nx + kT - 1) / kT;
-    const uint32_t split = blockIdx.x / ntx, x0 = (blockIdx.x % ntx) * kT;
-    const uint32_t ybeg = min(A.ny, split * A.rows_per_split), yend = min(A.ny, ybeg + A.rows_per_split);
-    for (uint32_t i = c; i < dim; i += kT)
-        X[r * pitch + i] = x0 + r < A.nx ? (float)static_cast<const T *>(A.x)[(size_t)(x0 + r) * A.xstride + i] : 0.0f;
-    float M = -INFINITY, l = 0.0f, o[MODE == kStats ? 1 : kMaxDim / kT];
-#pragma unroll
-    for (int j = 0; j < (MODE == kStats ? 1 : (int)kMaxDim / kT); ++j) o[j] = 0.0f;
-    for (uint32_t y0 = ybeg; y0 < yend; y0 += kT) {
-        __syncthreads();
-        for (uint32_t i = c; i < dim; i += kT)
-            Y[r * pitch + i] = y0 + r < yend ? (float)static_cast<const T *>(A.y)[(size_t)(y0 + r) * A.ystride + i] : 0.0f;
-        __syncthreads();
-        const uint32_t y = y0 + c;                      // this thread's logit: row x0 + r against row y0 + c
-        float acc = 0.0f;
-        for (uint32_t i = 0; i < dim; ++i) acc = fmaf(X[r * pitch + i], Y[c * pitch + i], acc);
-        float z = acc * A.k, sgn = 1.0f;
-        if (MODE == kRows && y < yend) {
-            const float4 p = A.yparam[y];
-            if (__float_as_uint(p.w) == x0 + r) {
-                z = p.y;
-                sgn = -p.z;
-            } else {
-                z += p.x;
-                sgn = p.z;
-            }
-        }
-        if (MODE != kRows && y < yend && x0 + r < A.nx && A.targets[x0 + r] == A.id_base + y) {
-            A.own2[x0 + r] = z;
-            z = -INFINITY;
-        }
-        if (y >= yend) z = -INFINITY;
-        float m = z;
-        for (int s = 1; s < kT; s <<= 1) m = fmaxf(m, __shfl_xor(m, s));
-        m = fmaxf(M, m);
-        const float ref = m == -INFINITY ? 0.0f : m;
-        const float w = exp2f(z - ref), old = M == -INFINITY ? 0.0f : exp2f(M - ref);
-        M = m;
-        float t = w;
-        for (int s = 1; s < kT; s <<= 1) t += __shfl_xor(t, s);
-        l = l * old + t;
-        if (MODE != kStats) {
-            P[r * (kT + 1) + c] = w * sgn;
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < (int)kMaxDim / kT; ++j) {
-                const uint32_t i = j * kT + c;
-                if (i < dim) {
-                    float s = o[j] * old;
-                    for (uint32_t e = 0; e < kT; ++e) s = fmaf(P[r * (kT + 1) + e], Y[e * pitch + i], s);
-                    o[j] = s;
-                }
-            }
-        }
-    }
-    if (x0 + r >= A.nx) return;
-    if (MODE == kRows && A.nsplit == 1) {
-        const float s = M == -INFINITY ? 0.0f : exp2f(M) * A.oscale;
-#pragma unroll
-        for (int j = 0; j < (int)kMaxDim / kT; ++j)
-            if (j * kT + c < dim) static_cast<T *>(A.out)[(size_t)(x0 + r) * A.ostride + j * kT + c] = (T)(o[j] * s);
-        return;
-    }
-    const size_t at = (size_t)split * A.nx + x0 + r;
-    if (c == 0) A.ml[at] = make_float2(M, l);
-    if (MODE != kStats)
-#pragma unroll
-        for (int j = 0; j < (int)kMaxDim / kT; ++j)
-            if (j * kT + c < dim) A.o[at * dim + j * kT + c] = o[j];
-}
 
 __device__ __forceinline__ bool target_here(uint32_t t, uint32_t id_base, uint32_t nb) { return t != kNoTarget && t >= id_base && t - id_base < nb; }
 
@@ -133,21 +35,29 @@ __device__ __forceinline__ bool target_here(uint32_t t, uint32_t id_base, uint32
 __device__ __forceinline__ float softplus(float d) { return d > 15.0f ? d + log1pf(expf(-d)) : log1pf(expf(d)); }
 
 // joins the slots of a query: rest, target logit, lse, loss, mean of the others.  One workgroup per query.
-__global__ void __launch_bounds__(256) rg_softmax_join_kernel(const float2 *ml, const float *o, uint32_t nslots, uint32_t nq, uint32_t dim, uint32_t nb, uint32_t id_base, const float *own2,
+__global__ void __launch_bounds__(256) rg_softmax_join_kernel(const float4 *ml, const float *o, uint32_t opitch, uint32_t nslots, uint32_t nq, uint32_t dim, uint32_t nb, uint32_t id_base, const float *own2,
                                                               const uint32_t *targets, float *rest, float *own, float *lse, float *loss, float *mean) {
     const uint32_t i = blockIdx.x, tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
-    __shared__ float red[4];
-    float M = -INFINITY;
-    for (uint32_t s = tid; s < nslots; s += 256) M = fmaxf(M, ml[(size_t)s * nq + i].x);
-    for (int d = 1; d < 64; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
-    if (lane == 0) red[wave] = M;
+    __shared__ float red[8];
+    float M = kNothing, Mo = kNothing;
+    for (uint32_t s = tid; s < nslots; s += 256) {
+        const float4 v = ml[(size_t)s * nq + i];
+        M = fmaxf(M, v.x);
+        Mo = fmaxf(Mo, v.z);
+    }
+    for (int d = 1; d < 64; d <<= 1) {
+        M = fmaxf(M, __shfl_xor(M, d));
+        Mo = fmaxf(Mo, __shfl_xor(Mo, d));
+    }
+    if (lane == 0) { red[wave] = M; red[4 + wave] = Mo; }
     __syncthreads();
     M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float ref = M == -INFINITY ? 0.0f : M;
+    Mo = fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
+    const bool none = M == kNothing;       // no other row than the target
     float l = 0.0f;
     for (uint32_t s = tid; s < nslots; s += 256) {
-        const float2 v = ml[(size_t)s * nq + i];
-        l += v.y * exp2f(v.x - ref);       // an empty slot: 0 * 2^-inf
+        const float4 v = ml[(size_t)s * nq + i];
+        l += v.y * exp2f(v.x - M);
     }
     for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
     __syncthreads();
@@ -157,7 +67,7 @@ __global__ void __launch_bounds__(256) rg_softmax_join_kernel(const float2 *ml, 
     if (tid == 0) {
         const uint32_t t = targets[i];
         const bool here = target_here(t, id_base, nb);
-        const float r = M == -INFINITY ? -INFINITY : (M + log2f(l)) * kLn2;
+        const float r = none ? -INFINITY : (M + log2f(l)) * kLn2;
         const float z = here ? own2[i] * kLn2 : -INFINITY;
         const float v = here ? softplus(r - z) : t == kNoTarget ? 0.0f : INFINITY;
         rest[i] = r;
@@ -166,11 +76,11 @@ __global__ void __launch_bounds__(256) rg_softmax_join_kernel(const float2 *ml, 
         if (loss) loss[i] = v;
     }
     if (mean) {
-        const float inv = M == -INFINITY ? 0.0f : 1.0f / l;
+        const float f = none ? 0.0f : exp2f(Mo - M) / l;
         for (uint32_t k = tid; k < dim; k += 256) {
             float s = 0.0f;
-            for (uint32_t e = 0; e < nslots; ++e) s = fmaf(exp2f(ml[(size_t)e * nq + i].x - ref), o[((size_t)e * nq + i) * dim + k], s);
-            mean[(size_t)i * dim + k] = s * inv;
+            for (uint32_t e = 0; e < nslots; ++e) s = fmaf(exp2f(ml[(size_t)e * nq + i].z - Mo), o[((size_t)e * nq + i) * opitch + k], s);
+            mean[(size_t)i * dim + k] = s * f;
         }
     }
 }
@@ -220,49 +130,109 @@ __global__ void __launch_bounds__(64) rg_softmax_dq_kernel(const void *base, uin
 
 // db from the slots of the pass over the queries
 template <int DT>
-__global__ void __launch_bounds__(256) rg_softmax_db_kernel(const float2 *ml, const float *o, uint32_t nslots, uint32_t nb, uint32_t dim, float scale, void *db, uint64_t dbstride) {
+__global__ void __launch_bounds__(256) rg_softmax_db_kernel(const float4 *ml, const float *o, uint32_t opitch, uint32_t nslots, uint32_t nb, uint32_t dim, float scale, void *db, uint64_t dbstride) {
     typedef typename Elem<DT>::T T;
     for (uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x; at < (uint64_t)nb * dim; at += (uint64_t)gridDim.x * 256) {
         const uint32_t j = (uint32_t)(at / dim), k = (uint32_t)(at % dim);
         float s = 0.0f;
         for (uint32_t e = 0; e < nslots; ++e) {
-            const float M = ml[(size_t)e * nb + j].x;
-            if (M != -INFINITY) s = fmaf(exp2f(M), o[((size_t)e * nb + j) * dim + k], s);
+            const float f = exp2f(0.5f * ml[(size_t)e * nb + j].z);     // 2^M in two steps: it may lie below the normal range
+            s = fmaf(f, f * o[((size_t)e * nb + j) * opitch + k], s);
         }
         static_cast<T *>(db)[(size_t)j * dbstride + k] = (T)(s * scale);
     }
 }
 
-// how a pass is cut: slots = pieces of y whose partial results are joined afterwards
+// the instantiation a width runs in, as the smallest number of 32-element steps that holds it
+constexpr int kSteps[] = {2, 4, 7, 8, 12, 16, 24, 32};
+int steps_of(uint32_t dim) {
+    if (dim > 192 && dim <= 208) return 7;              // (its output blocks end at 208)
+    for (int ks : kSteps)
+        if (ks != 7 && dim <= 32u * ks) return ks;
+    return 32;
+}
+struct Shape {
+    int ks;
+    uint32_t xt, nslices, resident, lds;
+};
+template <int DT, int KS>
+Shape shape_at(uint32_t dim) {
+    typedef PassCfg<DT, KS> C;
+    return Shape{KS, (uint32_t)C::XT, (dim + 16 * C::OB - 1) / (16 * C::OB), kCUs * std::min<uint32_t>(C::WPS, 160 * 1024 / C::LDS), (uint32_t)C::LDS};
+}
+template <int DT>
+Shape shape_dt(uint32_t dim) {
+    switch (steps_of(dim)) {
+        case 2: return shape_at<DT, 2>(dim);
+        case 4: return shape_at<DT, 4>(dim);
+        case 7: return shape_at<DT, 7>(dim);
+        case 8: return shape_at<DT, 8>(dim);
+        case 12: return shape_at<DT, 12>(dim);
+        case 16: return shape_at<DT, 16>(dim);
+        case 24: return shape_at<DT, 24>(dim);
+        default: return shape_at<DT, 32>(dim);
+    }
+}
+Shape shape_of(int dtype, uint32_t dim, bool sums) {
+    Shape s = dtype == RG_DTYPE_F32 ? shape_dt<RG_DTYPE_F32>(dim) : dtype == RG_DTYPE_F16 ? shape_dt<RG_DTYPE_F16>(dim) : shape_dt<RG_DTYPE_BF16>(dim);
+    if (!sums) s.nslices = 1;
+    return s;
+}
+
+// how a pass is cut: slots = pieces of y whose partial results are joined afterwards.  As many as give every workgroup place of the device
+// the same work, of at least four tiles.
 struct Plan {
+    Shape shape;
     uint32_t nsplit, rows_per_split;
     uint64_t grid;
 };
-Plan plan_of(uint32_t nx, uint32_t ny) {
-    const uint64_t ntx = (nx + kT - 1) / kT;
-    uint32_t want = (uint32_t)std::max<uint64_t>(1, kCUs * 4 / std::max<uint64_t>(ntx, 1));
-    want = std::max(1u, std::min(want, (ny + 255) / 256));
+Plan plan_of(int dtype, uint32_t dim, uint32_t nx, uint32_t ny, bool sums) {
     Plan p;
-    p.rows_per_split = ((std::max(ny, 1u) + want - 1) / want + kT - 1) / kT * kT;
+    p.shape = shape_of(dtype, dim, sums);
+    const uint64_t nt = std::max<uint64_t>(1, ((uint64_t)nx + p.shape.xt - 1) / p.shape.xt) * p.shape.nslices, places = p.shape.resident;
+    const uint32_t most = std::max(1u, ny / 128);
+    uint32_t best = 1;
+    double best_use = 0;
+    for (uint32_t n = 1; n <= most && n * nt <= 2 * places + nt; ++n) {
+        const uint64_t rounds = (n * nt + places - 1) / places;
+        const double use = (double)(n * nt) / (double)(rounds * places) - 0.01 * (double)(rounds > 1 ? rounds - 1 : 0);
+        if (use > best_use + 0.02) { best_use = use; best = n; }
+    }
+    p.rows_per_split = ((std::max(ny, 1u) + best - 1) / best + 31) / 32 * 32;
     p.nsplit = std::max(1u, (ny + p.rows_per_split - 1) / p.rows_per_split);
-    p.grid = ntx * p.nsplit;
+    p.grid = nt * p.nsplit;
     return p;
 }
 
+uint32_t opitch_of(uint32_t dim) { return (dim + 15) / 16 * 16; }
 uint64_t up256(uint64_t n) { return (n + 255) / 256 * 256; }
+
+// the instantiations of a type and mode live in a unit of their own (rg_softmax_inst_*.hip)
+rg_status launch_softmax_pass(int dtype, int mode, int ks, const PassArgs &A, uint64_t grid, uint32_t lds, hipStream_t s) {
+    if (grid > 0xffffffull) return set_error(RG_ERR_ARG, "softmax over a base: too many rows for one launch");
+    typedef const void *(*Pick)(int);
+    static const Pick pick[3][3] = {{softmax_kernel_f32_stats, softmax_kernel_f32_mean, softmax_kernel_f32_rows},
+                                    {softmax_kernel_f16_stats, softmax_kernel_f16_mean, softmax_kernel_f16_rows},
+                                    {softmax_kernel_bf16_stats, softmax_kernel_bf16_mean, softmax_kernel_bf16_rows}};
+    const void *kern = pick[dtype][mode](ks);
+    RG_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    void *args[] = {const_cast<PassArgs *>(&A)};
+    RG_HIP(hipLaunchKernel(kern, dim3((uint32_t)grid), dim3(256), args, lds, s));
+    return RG_OK;
+}
 
 // bytes of the three parts of the scratch: M and l of the slots, sums of the slots, and per query the target's logit or the parameters
 struct Scratch {
     uint64_t ml, o, y;
     uint64_t total() const { return ml + o + y; }
 };
-Scratch scratch_of(int what, uint32_t nb, uint32_t nq, uint32_t dim) {
+Scratch scratch_of(int what, uint32_t nb, uint32_t nq, uint32_t dim, int dtype) {
     const uint32_t nx = what == RG_SOFTMAX_GRAD ? nb : nq, ny = what == RG_SOFTMAX_GRAD ? nq : nb;
-    const Plan p = plan_of(nx, ny);
+    const Plan p = plan_of(dtype, dim, nx, ny, what != RG_SOFTMAX_STATS);
     Scratch s;
     const bool pieces = what != RG_SOFTMAX_GRAD || p.nsplit > 1;
-    s.ml = pieces ? up256((uint64_t)p.nsplit * nx * 8) : 0;
-    s.o = pieces && what != RG_SOFTMAX_STATS ? up256((uint64_t)p.nsplit * nx * dim * 4) : 0;
+    s.ml = pieces ? up256((uint64_t)p.nsplit * nx * 16) : 0;
+    s.o = pieces && what != RG_SOFTMAX_STATS ? up256((uint64_t)p.nsplit * nx * opitch_of(dim) * 4) : 0;
     s.y = up256((uint64_t)nq * (what == RG_SOFTMAX_GRAD ? 16 : 4));
     return s;
 }
@@ -298,16 +268,6 @@ rg_status check_scratch(const void *work, uint64_t have, uint64_t need) {
     return RG_OK;
 }
 
-template <int DT, int MODE>
-rg_status launch_pass(const PassArgs &A, const Plan &p, hipStream_t s) {
-    auto kern = rg_softmax_pass_kernel<DT, MODE>;
-    const size_t lds = (2 * kT * (size_t)(A.dim + 1) + kT * (kT + 1)) * 4;
-    RG_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    hipLaunchKernelGGL(kern, dim3((uint32_t)p.grid), dim3(256), lds, s, A);
-    RG_HIP(hipGetLastError());
-    return RG_OK;
-}
-
 struct Call {      // the arguments of the entry points
     const void *base, *queries;
     uint64_t bstride, qstride;
@@ -320,34 +280,34 @@ struct Call {      // the arguments of the entry points
 
 template <int DT>
 rg_status shard(const Call &c, float *rest, float *own, float *lse, float *loss, float *mean) {
-    const Plan p = plan_of(c.nq, c.nb);
-    const Scratch sc = scratch_of(mean ? RG_SOFTMAX_MEAN : RG_SOFTMAX_STATS, c.nb, c.nq, c.dim);
+    const Plan p = plan_of(DT, c.dim, c.nq, c.nb, mean != nullptr);
+    const Scratch sc = scratch_of(mean ? RG_SOFTMAX_MEAN : RG_SOFTMAX_STATS, c.nb, c.nq, c.dim, DT);
     float *own2 = reinterpret_cast<float *>(c.work + sc.ml + sc.o);
-    PassArgs A{c.queries, c.base, c.qstride, c.bstride, c.nq, c.nb, c.dim, c.scale * kLog2e, p.nsplit, p.rows_per_split,
-               reinterpret_cast<float2 *>(c.work), reinterpret_cast<float *>(c.work + sc.ml), c.targets, c.id_base, own2, nullptr, nullptr, 0, 0.0f};
-    rg_status st = mean ? launch_pass<DT, kMean>(A, p, c.s) : launch_pass<DT, kStats>(A, p, c.s);
+    PassArgs A{c.queries, c.base, c.qstride, c.bstride, c.nq, c.nb, c.dim, c.scale * kLog2e, p.nsplit, p.rows_per_split, p.shape.nslices, opitch_of(c.dim),
+               reinterpret_cast<float4 *>(c.work), reinterpret_cast<float *>(c.work + sc.ml), c.targets, c.id_base, own2, nullptr, nullptr, 0, 0.0f};
+    rg_status st = launch_softmax_pass(DT, mean ? kMean : kStats, p.shape.ks, A, p.grid, p.shape.lds, c.s);
     if (st != RG_OK) return st;
-    hipLaunchKernelGGL(rg_softmax_join_kernel, dim3(c.nq), dim3(256), 0, c.s, A.ml, A.o, p.nsplit, c.nq, c.dim, c.nb, c.id_base, own2, c.targets, rest, own, lse, loss, mean);
+    hipLaunchKernelGGL(rg_softmax_join_kernel, dim3(c.nq), dim3(256), 0, c.s, A.ml, A.o, A.opitch, p.nsplit, c.nq, c.dim, c.nb, c.id_base, own2, c.targets, rest, own, lse, loss, mean);
     RG_HIP(hipGetLastError());
     return RG_OK;
 }
 
 template <int DT>
 rg_status grad(const Call &c, const float *lse, const float *loss, const float *rest, const float *mean, const float *weights, void *dq, uint64_t dqstride, void *db, uint64_t dbstride) {
-    const Plan p = plan_of(c.nb, c.nq);
-    const Scratch sc = scratch_of(RG_SOFTMAX_GRAD, c.nb, c.nq, c.dim);
+    const Plan p = plan_of(DT, c.dim, c.nb, c.nq, true);
+    const Scratch sc = scratch_of(RG_SOFTMAX_GRAD, c.nb, c.nq, c.dim, DT);
     float4 *yp = db ? reinterpret_cast<float4 *>(c.work + sc.ml + sc.o) : nullptr;
     if (c.nq) {
         hipLaunchKernelGGL((rg_softmax_dq_kernel<DT>), dim3(c.nq), dim3(64), 0, c.s, c.base, c.bstride, c.nb, c.id_base, c.nq, c.dim, c.scale, c.targets, lse, loss, rest, mean, weights, dq, dqstride, yp);
         RG_HIP(hipGetLastError());
     }
     if (!db || c.nb == 0) return RG_OK;
-    PassArgs A{c.base, c.queries, c.bstride, c.qstride, c.nb, c.nq, c.dim, c.scale * kLog2e, p.nsplit, p.rows_per_split,
-               reinterpret_cast<float2 *>(c.work), reinterpret_cast<float *>(c.work + sc.ml), nullptr, 0, nullptr, yp, db, dbstride, c.scale};
-    rg_status st = launch_pass<DT, kRows>(A, p, c.s);
+    PassArgs A{c.base, c.queries, c.bstride, c.qstride, c.nb, c.nq, c.dim, c.scale * kLog2e, p.nsplit, p.rows_per_split, p.shape.nslices, opitch_of(c.dim),
+               reinterpret_cast<float4 *>(c.work), reinterpret_cast<float *>(c.work + sc.ml), nullptr, 0, nullptr, yp, db, dbstride, c.scale};
+    rg_status st = launch_softmax_pass(DT, kRows, p.shape.ks, A, p.grid, p.shape.lds, c.s);
     if (st != RG_OK || p.nsplit == 1) return st;
     const uint64_t n = (uint64_t)c.nb * c.dim;
-    hipLaunchKernelGGL((rg_softmax_db_kernel<DT>), dim3((uint32_t)std::min<uint64_t>((n + 255) / 256, 1u << 20)), dim3(256), 0, c.s, A.ml, A.o, p.nsplit, c.nb, c.dim, c.scale, db, dbstride);
+    hipLaunchKernelGGL((rg_softmax_db_kernel<DT>), dim3((uint32_t)std::min<uint64_t>((n + 255) / 256, 1u << 20)), dim3(256), 0, c.s, A.ml, A.o, A.opitch, p.nsplit, c.nb, c.dim, c.scale, db, dbstride);
     RG_HIP(hipGetLastError());
     return RG_OK;
 }
@@ -364,7 +324,7 @@ rg_status rg_softmax_workspace(int what, uint32_t nb, uint32_t nq, uint32_t dim,
     if (what != RG_SOFTMAX_STATS && what != RG_SOFTMAX_MEAN && what != RG_SOFTMAX_GRAD) return set_error(RG_ERR_ARG, "unknown kind of call");
     rg_status st = check_shapes(nb, nq, dim, dtype);
     if (st != RG_OK) return st;
-    *bytes = scratch_of(what, nb, nq, dim).total();
+    *bytes = scratch_of(what, nb, nq, dim, dtype).total();
     return RG_OK;
 }
 
@@ -375,7 +335,7 @@ rg_status rg_softmax_shard_dev(const void *d_base, uint32_t nb, uint64_t bstride
     rg_status st = check_call(nb, d_base, bstride, nq, d_queries, qstride, dim, dtype, scale, id_base);
     if (st != RG_OK || nq == 0) return st;
     if (!d_targets || !d_rest || !d_own) return set_error(RG_ERR_ARG, "null argument");
-    st = check_scratch(d_work, work_bytes, scratch_of(d_mean ? RG_SOFTMAX_MEAN : RG_SOFTMAX_STATS, nb, nq, dim).total());
+    st = check_scratch(d_work, work_bytes, scratch_of(d_mean ? RG_SOFTMAX_MEAN : RG_SOFTMAX_STATS, nb, nq, dim, dtype).total());
     if (st != RG_OK) return st;
     OnDevice on(device);
     if (on.st != RG_OK) return on.st;
@@ -406,7 +366,7 @@ rg_status rg_softmax_grad_dev(const void *d_base, uint32_t nb, uint64_t bstride,
     if (st == RG_OK && d_db) st = check_rows(d_db, nb, dbstride, dim, dtype, "gradient of the base");
     if (st != RG_OK) return st;
     if (nq && (!d_targets || !d_lse || !d_loss || !d_weights || (d_dq && (!d_mean || !d_rest)))) return set_error(RG_ERR_ARG, "null argument");
-    st = check_scratch(d_work, work_bytes, scratch_of(RG_SOFTMAX_GRAD, d_db ? nb : 0, nq, dim).total());
+    st = check_scratch(d_work, work_bytes, scratch_of(RG_SOFTMAX_GRAD, d_db ? nb : 0, nq, dim, dtype).total());
     if (st != RG_OK) return st;
     OnDevice on(device);
     if (on.st != RG_OK) return on.st;
