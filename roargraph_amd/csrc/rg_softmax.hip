@@ -26,7 +26,6 @@ namespace rg {
 namespace {
 
 constexpr uint32_t kMaxDim = 1024;
-constexpr uint32_t kCUs = 256;             // MI355X; the workspace query needs no device
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ bool target_here(uint32_t t, uint32_t id_base, uint32_t nb) { return t != kNoTarget && t >= id_base && t - id_base < nb; }
@@ -102,18 +101,27 @@ __global__ void __launch_bounds__(256) rg_softmax_merge_kernel(const float *rest
     loss[i] = v;
 }
 
-// per query: what the pass over the rows needs of it, and dq.  One wave per query.
+// per query: what the pass over the rows needs of it (info and ytarget, padded to whole tiles), and dq.  One wave per query.
 template <int DT>
 __global__ void __launch_bounds__(64) rg_softmax_dq_kernel(const void *base, uint64_t bstride, uint32_t nb, uint32_t id_base, uint32_t nq, uint32_t dim, float scale,
                                                            const uint32_t *targets, const float *lse, const float *loss, const float *rest, const float *mean,
-                                                           const float *weights, void *dq, uint64_t dqstride, float4 *yparam) {
+                                                           const float *weights, void *dq, uint64_t dqstride, float4 *info, float *ytarget) {
     typedef typename Elem<DT>::T T;
-    const uint32_t i = blockIdx.x, t = targets[i], row = t - id_base;
+    const uint32_t i = blockIdx.x;
+    if (i >= nq) {
+        if (threadIdx.x == 0) {
+            info[i] = make_float4(1.0f, -INFINITY, 1.0f, __uint_as_float(kNoTarget));
+            ytarget[i] = -INFINITY;
+        }
+        return;
+    }
+    const uint32_t t = targets[i], row = t - id_base;
     const bool here = target_here(t, id_base, nb);
     const float w = t == kNoTarget ? 0.0f : weights[i], miss = here ? -expm1f(-loss[i]) : 0.0f;      // 1 - p_target
-    if (yparam && threadIdx.x == 0) {
+    if (info && threadIdx.x == 0) {
         const float lw = log2f(fabsf(w));
-        yparam[i] = make_float4(t == kNoTarget ? -INFINITY : lw - lse[i] * kLog2e, lw + log2f(miss), w < 0.0f ? -1.0f : 1.0f, __uint_as_float(here ? row : kNoTarget));
+        info[i] = make_float4(1.0f, t == kNoTarget ? -INFINITY : lw - lse[i] * kLog2e, w < 0.0f ? -1.0f : 1.0f, __uint_as_float(here ? row : kNoTarget));
+        ytarget[i] = lw + log2f(miss);
     }
     if (!dq) return;
     const float part = rest[i] == -INFINITY ? 0.0f : expf(rest[i] - lse[i]);
@@ -125,6 +133,53 @@ __global__ void __launch_bounds__(64) rg_softmax_dq_kernel(const void *base, uin
             v *= w * scale;
         }
         static_cast<T *>(dq)[(size_t)i * dqstride + k] = (T)v;
+    }
+}
+
+// rows as the wide pass streams them: 16-bit planes of 32 ks elements, zeros behind dim and behind the last row; fp32 as two halves scaled by the
+// row's power of two, whose factor and exponent go to `info` (`more`: the exponent is added to what the queries' parameters already hold).
+// 16 lanes per row, CI chunks of 8 elements a lane.
+template <int DT, int CI>
+__global__ void __launch_bounds__(256) rg_softmax_planes_kernel(const void *rows, uint64_t stride, uint32_t n, uint32_t npad, uint32_t dim, uint32_t ks, uint16_t *planes, float4 *info, float *ytarget,
+                                                                int more) {
+    typedef typename Elem<DT>::T T;
+    constexpr int NP = DT == RG_DTYPE_F32 ? 2 : 1;
+    const bool vec = ((uintptr_t)rows | stride * sizeof(T)) % 16 == 0;
+    const uint32_t lc = threadIdx.x % 16;
+    for (uint64_t r = (uint64_t)blockIdx.x * 16 + threadIdx.x / 16; r < npad; r += (uint64_t)gridDim.x * 16) {
+        const char *row = static_cast<const char *>(rows) + (size_t)r * stride * sizeof(T);
+        uint16_t *out = planes + (size_t)r * NP * ks * 32;
+        Chunk<DT> c[CI];
+#pragma unroll
+        for (int i = 0; i < CI; ++i) c[i] = load_chunk<DT>(row, 8 * (lc + 16 * i), r < n ? dim : 0, vec);
+        if constexpr (DT == RG_DTYPE_F32) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < CI; ++i) m = max(m, __float_as_uint(absmax(c[i])));
+#pragma unroll
+            for (int d = 1; d < 16; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
+            const float top = __uint_as_float(m);
+            const int e = row_exponent(top);
+#pragma unroll
+            for (int i = 0; i < CI; ++i) {
+                if (lc + 16 * i >= ks * 4) continue;
+                half8 hi, lo;
+                split8(c[i], top, pow2(-e), hi, lo);
+                *reinterpret_cast<half8 *>(out + 8 * (lc + 16 * i)) = hi;
+                *reinterpret_cast<half8 *>(out + ks * 32 + 8 * (lc + 16 * i)) = lo;
+            }
+            if (lc == 0) {
+                float4 v = more ? info[r] : make_float4(1.0f, 0.0f, 1.0f, __uint_as_float(kNoTarget));
+                v.x = row_factor(top, e);
+                v.y += (float)e;
+                info[r] = v;
+                if (more) ytarget[r] += (float)e;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < CI; ++i)
+                if (lc + 16 * i < ks * 4) *reinterpret_cast<u32x4 *>(out + 8 * (lc + 16 * i)) = c[i].v;
+        }
     }
 }
 
@@ -143,98 +198,120 @@ __global__ void __launch_bounds__(256) rg_softmax_db_kernel(const float4 *ml, co
     }
 }
 
-// the instantiation a width runs in, as the smallest number of 32-element steps that holds it
-constexpr int kSteps[] = {2, 4, 7, 8, 12, 16, 24, 32};
+uint64_t up256(uint64_t n) { return (n + 255) / 256 * 256; }
+uint32_t up32(uint32_t n) { return (n + 31) / 32 * 32; }
+uint32_t opitch_of(uint32_t dim) { return (dim + 15) / 16 * 16; }
+
+// the instantiation a width runs in, as the number of 32-element steps that holds it (7: its output blocks end at 208)
 int steps_of(uint32_t dim) {
-    if (dim > 192 && dim <= 208) return 7;              // (its output blocks end at 208)
-    for (int ks : kSteps)
-        if (ks != 7 && dim <= 32u * ks) return ks;
+    if (dim > 192 && dim <= 208) return 7;
+    for (int ks : {2, 4, 8, 12, 16, 24})
+        if (dim <= 32u * ks) return ks;
     return 32;
 }
-struct Shape {
+
+// at most this many bytes of planes at a time: a large base is streamed piece by piece
+constexpr uint64_t kPieceBytes = 1ull << 30;
+
+// how a pass is cut: into pieces of y that are made into planes one after another (planes), each split into slots whose partial results are
+// joined at the end -- as many as give every workgroup place of the device the same work, of at least four tiles
+struct Plan {
+    SoftmaxKernel k;
     int ks;
-    uint32_t xt, nslices, resident, lds;
-};
-template <int DT, int KS>
-Shape shape_at(uint32_t dim) {
-    typedef PassCfg<DT, KS> C;
-    return Shape{KS, (uint32_t)C::XT, (dim + 16 * C::OB - 1) / (16 * C::OB), kCUs * std::min<uint32_t>(C::WPS, 160 * 1024 / C::LDS), (uint32_t)C::LDS};
-}
-template <int DT>
-Shape shape_dt(uint32_t dim) {
-    switch (steps_of(dim)) {
-        case 2: return shape_at<DT, 2>(dim);
-        case 4: return shape_at<DT, 4>(dim);
-        case 7: return shape_at<DT, 7>(dim);
-        case 8: return shape_at<DT, 8>(dim);
-        case 12: return shape_at<DT, 12>(dim);
-        case 16: return shape_at<DT, 16>(dim);
-        case 24: return shape_at<DT, 24>(dim);
-        default: return shape_at<DT, 32>(dim);
+    bool thin, planes;
+    uint32_t nx, ny, ntx, nslices, piece, nslots;
+    uint64_t row_bytes;               // of a row of planes
+    struct Cut {
+        uint32_t nsplit, rows;
+    };
+    Cut cut(uint32_t rows) const {
+        const uint64_t nt = (uint64_t)ntx * nslices, places = 256ull * std::min<uint32_t>(k.wps, 160 * 1024 / k.lds);
+        const uint32_t most = std::max(1u, rows / 128);
+        uint32_t best = 1;
+        double best_use = 0;
+        for (uint32_t n = 1; n <= most && n * nt <= 2 * places + nt; ++n) {
+            const uint64_t rounds = (n * nt + places - 1) / places;
+            const double use = (double)(n * nt) / (double)(rounds * places) - 0.01 * (double)(rounds - 1);
+            if (use > best_use * 1.02) { best_use = use; best = n; }
+        }
+        Cut c;
+        c.rows = up32((std::max(rows, 1u) + best - 1) / best);
+        c.nsplit = std::max(1u, (rows + c.rows - 1) / c.rows);
+        return c;
     }
-}
-Shape shape_of(int dtype, uint32_t dim, bool sums) {
-    Shape s = dtype == RG_DTYPE_F32 ? shape_dt<RG_DTYPE_F32>(dim) : dtype == RG_DTYPE_F16 ? shape_dt<RG_DTYPE_F16>(dim) : shape_dt<RG_DTYPE_BF16>(dim);
-    if (!sums) s.nslices = 1;
-    return s;
+};
+
+SoftmaxKernel kernel_of(int dtype, int mode, bool thin, int ks) {
+    typedef SoftmaxKernel (*Pick)(int);
+    static const Pick wide[3][3] = {{softmax_wide_f32_stats, softmax_wide_f32_mean, softmax_wide_f32_rows},
+                                    {softmax_wide_f16_stats, softmax_wide_f16_mean, softmax_wide_f16_rows},
+                                    {softmax_wide_bf16_stats, softmax_wide_bf16_mean, softmax_wide_bf16_rows}};
+    static const Pick few[3][2] = {{softmax_thin_f32_stats, softmax_thin_f32_mean}, {softmax_thin_f16_stats, softmax_thin_f16_mean}, {softmax_thin_bf16_stats, softmax_thin_bf16_mean}};
+    return thin ? few[dtype][mode](ks) : wide[dtype][mode](ks);
 }
 
-// how a pass is cut: slots = pieces of y whose partial results are joined afterwards.  As many as give every workgroup place of the device
-// the same work, of at least four tiles.
-struct Plan {
-    Shape shape;
-    uint32_t nsplit, rows_per_split;
-    uint64_t grid;
-};
-Plan plan_of(int dtype, uint32_t dim, uint32_t nx, uint32_t ny, bool sums) {
+// direct: the streamed rows can be read where they lie (16-bit rows of whole 16-byte chunks, 16-byte aligned)
+Plan plan_of(int dtype, int mode, uint32_t dim, uint32_t nx, uint32_t ny, bool direct) {
     Plan p;
-    p.shape = shape_of(dtype, dim, sums);
-    const uint64_t nt = std::max<uint64_t>(1, ((uint64_t)nx + p.shape.xt - 1) / p.shape.xt) * p.shape.nslices, places = p.shape.resident;
-    const uint32_t most = std::max(1u, ny / 128);
-    uint32_t best = 1;
-    double best_use = 0;
-    for (uint32_t n = 1; n <= most && n * nt <= 2 * places + nt; ++n) {
-        const uint64_t rounds = (n * nt + places - 1) / places;
-        const double use = (double)(n * nt) / (double)(rounds * places) - 0.01 * (double)(rounds > 1 ? rounds - 1 : 0);
-        if (use > best_use + 0.02) { best_use = use; best = n; }
-    }
-    p.rows_per_split = ((std::max(ny, 1u) + best - 1) / best + 31) / 32 * 32;
-    p.nsplit = std::max(1u, (ny + p.rows_per_split - 1) / p.rows_per_split);
-    p.grid = nt * p.nsplit;
+    p.ks = steps_of(dim);
+    p.thin = mode != kRows && nx <= 64;
+    p.k = kernel_of(dtype, mode, p.thin, p.ks);
+    p.planes = !p.thin && !direct;
+    p.nx = nx;
+    p.ny = ny;
+    p.ntx = std::max(1u, (uint32_t)(((uint64_t)nx + p.k.xt - 1) / p.k.xt));
+    p.nslices = mode == kStats ? 1 : (dim + 16 * p.k.ob - 1) / (16 * p.k.ob);
+    p.row_bytes = (uint64_t)(dtype == RG_DTYPE_F32 ? 2 : 1) * p.ks * 64;
+    p.piece = ny;
+    if (p.planes && mode != kRows) p.piece = (uint32_t)std::min<uint64_t>(ny, kPieceBytes / p.row_bytes / 32 * 32);
+    p.nslots = 0;
+    for (uint64_t y = 0; y == 0 || y < ny; y += std::max(p.piece, 1u)) p.nslots += p.cut((uint32_t)std::min<uint64_t>(p.piece, ny - y)).nsplit;
     return p;
 }
 
-uint32_t opitch_of(uint32_t dim) { return (dim + 15) / 16 * 16; }
-uint64_t up256(uint64_t n) { return (n + 255) / 256 * 256; }
+// the parts of the scratch: references and sums of the slots, sums of rows of the slots, per query its target's logit or its parameters,
+// parameters of the streamed rows, planes
+struct Layout {
+    uint64_t ml, o, aux, info, planes, total;
+};
+Layout layout_of(const Plan &p, int mode, int dtype, uint32_t dim) {
+    Layout L;
+    const bool pieces = mode != kRows || p.nslots > 1;
+    uint64_t at = 0;
+    auto part = [&](uint64_t bytes) { const uint64_t was = at; at += up256(bytes); return was; };
+    L.ml = part(pieces ? (uint64_t)p.nslots * p.nx * 16 : 0);
+    L.o = part(pieces && mode != kStats ? (uint64_t)p.nslots * p.nx * opitch_of(dim) * 4 : 0);
+    L.aux = part(mode == kRows ? (uint64_t)up32(p.ny) * 4 : (uint64_t)p.nx * 4);
+    L.info = part(mode == kRows ? (uint64_t)up32(p.ny) * 16 : p.planes && dtype == RG_DTYPE_F32 ? (uint64_t)up32(p.piece) * 16 : 0);
+    L.planes = part(p.planes ? up32(p.piece) * p.row_bytes : 0);
+    L.total = at;
+    return L;
+}
+// of a call whose pointers are not known yet
+uint64_t scratch_of(int mode, uint32_t nb, uint32_t nq, uint32_t dim, int dtype) {
+    const uint32_t nx = mode == kRows ? nb : nq, ny = mode == kRows ? nq : nb;
+    uint64_t n = layout_of(plan_of(dtype, mode, dim, nx, ny, false), mode, dtype, dim).total;
+    if (dtype != RG_DTYPE_F32 && dim % 8 == 0) n = std::max(n, layout_of(plan_of(dtype, mode, dim, nx, ny, true), mode, dtype, dim).total);
+    return n;
+}
+bool direct_rows(const void *rows, uint64_t stride, uint32_t dim, int dtype) { return dtype != RG_DTYPE_F32 && dim % 8 == 0 && stride % 8 == 0 && (uintptr_t)rows % 16 == 0; }
 
-// the instantiations of a type and mode live in a unit of their own (rg_softmax_inst_*.hip)
-rg_status launch_softmax_pass(int dtype, int mode, int ks, const PassArgs &A, uint64_t grid, uint32_t lds, hipStream_t s) {
-    if (grid > 0xffffffull) return set_error(RG_ERR_ARG, "softmax over a base: too many rows for one launch");
-    typedef const void *(*Pick)(int);
-    static const Pick pick[3][3] = {{softmax_kernel_f32_stats, softmax_kernel_f32_mean, softmax_kernel_f32_rows},
-                                    {softmax_kernel_f16_stats, softmax_kernel_f16_mean, softmax_kernel_f16_rows},
-                                    {softmax_kernel_bf16_stats, softmax_kernel_bf16_mean, softmax_kernel_bf16_rows}};
-    const void *kern = pick[dtype][mode](ks);
-    RG_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-    void *args[] = {const_cast<PassArgs *>(&A)};
-    RG_HIP(hipLaunchKernel(kern, dim3((uint32_t)grid), dim3(256), args, lds, s));
+template <int DT>
+rg_status make_planes(const void *rows, uint64_t stride, uint32_t n, uint32_t dim, int ks, void *planes, float4 *info, float *ytarget, hipStream_t s) {
+    auto kern = ks <= 4 ? rg_softmax_planes_kernel<DT, 1> : ks <= 8 ? rg_softmax_planes_kernel<DT, 2> : ks <= 16 ? rg_softmax_planes_kernel<DT, 4> : rg_softmax_planes_kernel<DT, 8>;
+    const uint32_t npad = up32(n);
+    hipLaunchKernelGGL(kern, dim3(std::min(npad / 16, 1u << 16)), dim3(256), 0, s, rows, stride, n, npad, dim, (uint32_t)ks, static_cast<uint16_t *>(planes), info, ytarget, ytarget ? 1 : 0);
+    RG_HIP(hipGetLastError());
     return RG_OK;
 }
 
-// bytes of the three parts of the scratch: M and l of the slots, sums of the slots, and per query the target's logit or the parameters
-struct Scratch {
-    uint64_t ml, o, y;
-    uint64_t total() const { return ml + o + y; }
-};
-Scratch scratch_of(int what, uint32_t nb, uint32_t nq, uint32_t dim, int dtype) {
-    const uint32_t nx = what == RG_SOFTMAX_GRAD ? nb : nq, ny = what == RG_SOFTMAX_GRAD ? nq : nb;
-    const Plan p = plan_of(dtype, dim, nx, ny, what != RG_SOFTMAX_STATS);
-    Scratch s;
-    const bool pieces = what != RG_SOFTMAX_GRAD || p.nsplit > 1;
-    s.ml = pieces ? up256((uint64_t)p.nsplit * nx * 16) : 0;
-    s.o = pieces && what != RG_SOFTMAX_STATS ? up256((uint64_t)p.nsplit * nx * opitch_of(dim) * 4) : 0;
-    s.y = up256((uint64_t)nq * (what == RG_SOFTMAX_GRAD ? 16 : 4));
-    return s;
+rg_status launch_pass(const Plan &p, const PassArgs &A, hipStream_t s) {
+    const uint64_t grid = (uint64_t)p.ntx * p.nslices * A.nsplit;
+    if (grid > 0xffffffull) return set_error(RG_ERR_ARG, "softmax over a base: too many rows for one launch");
+    RG_HIP(hipFuncSetAttribute(p.k.kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.k.lds));
+    void *args[] = {const_cast<PassArgs *>(&A)};
+    RG_HIP(hipLaunchKernel(p.k.kern, dim3((uint32_t)grid), dim3(256), args, p.k.lds, s));
+    return RG_OK;
 }
 
 rg_status check_shapes(uint32_t nb, uint32_t nq, uint32_t dim, int dtype) {
@@ -280,34 +357,75 @@ struct Call {      // the arguments of the entry points
 
 template <int DT>
 rg_status shard(const Call &c, float *rest, float *own, float *lse, float *loss, float *mean) {
-    const Plan p = plan_of(DT, c.dim, c.nq, c.nb, mean != nullptr);
-    const Scratch sc = scratch_of(mean ? RG_SOFTMAX_MEAN : RG_SOFTMAX_STATS, c.nb, c.nq, c.dim, DT);
-    float *own2 = reinterpret_cast<float *>(c.work + sc.ml + sc.o);
-    PassArgs A{c.queries, c.base, c.qstride, c.bstride, c.nq, c.nb, c.dim, c.scale * kLog2e, p.nsplit, p.rows_per_split, p.shape.nslices, opitch_of(c.dim),
-               reinterpret_cast<float4 *>(c.work), reinterpret_cast<float *>(c.work + sc.ml), c.targets, c.id_base, own2, nullptr, nullptr, 0, 0.0f};
-    rg_status st = launch_softmax_pass(DT, mean ? kMean : kStats, p.shape.ks, A, p.grid, p.shape.lds, c.s);
-    if (st != RG_OK) return st;
-    hipLaunchKernelGGL(rg_softmax_join_kernel, dim3(c.nq), dim3(256), 0, c.s, A.ml, A.o, A.opitch, p.nsplit, c.nq, c.dim, c.nb, c.id_base, own2, c.targets, rest, own, lse, loss, mean);
+    const int mode = mean ? kMean : kStats;
+    const Plan p = plan_of(DT, mode, c.dim, c.nq, c.nb, direct_rows(c.base, c.bstride, c.dim, DT));
+    const Layout L = layout_of(p, mode, DT, c.dim);
+    PassArgs A{};
+    A.x = c.queries; A.xstride = c.qstride; A.nx = c.nq;
+    A.dim = A.ydim = c.dim;
+    A.k = c.scale * kLog2e;
+    A.nslices = p.nslices; A.opitch = opitch_of(c.dim);
+    A.targets = c.targets; A.own2 = reinterpret_cast<float *>(c.work + L.aux);
+    float4 *ml = reinterpret_cast<float4 *>(c.work + L.ml);
+    float *o = reinterpret_cast<float *>(c.work + L.o);
+    uint32_t slot = 0;
+    for (uint64_t y = 0; y == 0 || y < c.nb; y += std::max(p.piece, 1u)) {
+        const uint32_t n = (uint32_t)std::min<uint64_t>(p.piece, c.nb - y);
+        const Plan::Cut cut = p.cut(n);
+        A.y = static_cast<const char *>(c.base) + y * c.bstride * sizeof(typename Elem<DT>::T);
+        A.ystride = c.bstride; A.ny = n;
+        A.id_base = c.id_base + (uint32_t)y;
+        A.nsplit = cut.nsplit; A.rows_per_split = cut.rows;
+        A.ml = ml + (size_t)slot * c.nq;
+        A.o = o + (size_t)slot * c.nq * A.opitch;
+        if (p.planes && n) {
+            float4 *info = reinterpret_cast<float4 *>(c.work + L.info);
+            rg_status st = make_planes<DT>(A.y, c.bstride, n, c.dim, p.ks, c.work + L.planes, info, nullptr, c.s);
+            if (st != RG_OK) return st;
+            A.y = c.work + L.planes; A.ystride = p.row_bytes / 2; A.ydim = 32 * p.ks; A.yinfo = info;
+        }
+        rg_status st = launch_pass(p, A, c.s);
+        if (st != RG_OK) return st;
+        slot += cut.nsplit;
+    }
+    hipLaunchKernelGGL(rg_softmax_join_kernel, dim3(c.nq), dim3(256), 0, c.s, ml, o, A.opitch, p.nslots, c.nq, c.dim, c.nb, c.id_base, A.own2, c.targets, rest, own, lse, loss, mean);
     RG_HIP(hipGetLastError());
     return RG_OK;
 }
 
 template <int DT>
 rg_status grad(const Call &c, const float *lse, const float *loss, const float *rest, const float *mean, const float *weights, void *dq, uint64_t dqstride, void *db, uint64_t dbstride) {
-    const Plan p = plan_of(DT, c.dim, c.nb, c.nq, true);
-    const Scratch sc = scratch_of(RG_SOFTMAX_GRAD, c.nb, c.nq, c.dim, DT);
-    float4 *yp = db ? reinterpret_cast<float4 *>(c.work + sc.ml + sc.o) : nullptr;
+    const uint32_t rows = db ? c.nb : 0;
+    const Plan p = plan_of(DT, kRows, c.dim, rows, c.nq, direct_rows(c.queries, c.qstride, c.dim, DT));
+    const Layout L = layout_of(p, kRows, DT, c.dim);
+    float4 *info = rows ? reinterpret_cast<float4 *>(c.work + L.info) : nullptr;
+    float *ytarget = rows ? reinterpret_cast<float *>(c.work + L.aux) : nullptr;
     if (c.nq) {
-        hipLaunchKernelGGL((rg_softmax_dq_kernel<DT>), dim3(c.nq), dim3(64), 0, c.s, c.base, c.bstride, c.nb, c.id_base, c.nq, c.dim, c.scale, c.targets, lse, loss, rest, mean, weights, dq, dqstride, yp);
+        hipLaunchKernelGGL((rg_softmax_dq_kernel<DT>), dim3(rows ? up32(c.nq) : c.nq), dim3(64), 0, c.s, c.base, c.bstride, c.nb, c.id_base, c.nq, c.dim, c.scale, c.targets, lse, loss, rest, mean, weights,
+                           dq, dqstride, info, ytarget);
         RG_HIP(hipGetLastError());
     }
-    if (!db || c.nb == 0) return RG_OK;
-    PassArgs A{c.base, c.queries, c.bstride, c.qstride, c.nb, c.nq, c.dim, c.scale * kLog2e, p.nsplit, p.rows_per_split, p.shape.nslices, opitch_of(c.dim),
-               reinterpret_cast<float4 *>(c.work), reinterpret_cast<float *>(c.work + sc.ml), nullptr, 0, nullptr, yp, db, dbstride, c.scale};
-    rg_status st = launch_softmax_pass(DT, kRows, p.shape.ks, A, p.grid, p.shape.lds, c.s);
-    if (st != RG_OK || p.nsplit == 1) return st;
-    const uint64_t n = (uint64_t)c.nb * c.dim;
-    hipLaunchKernelGGL((rg_softmax_db_kernel<DT>), dim3((uint32_t)std::min<uint64_t>((n + 255) / 256, 1u << 20)), dim3(256), 0, c.s, A.ml, A.o, A.opitch, p.nsplit, c.nb, c.dim, c.scale, db, dbstride);
+    if (!rows) return RG_OK;
+    const Plan::Cut cut = p.cut(c.nq);
+    PassArgs A{};
+    A.x = c.base; A.xstride = c.bstride; A.nx = rows;
+    A.y = c.queries; A.ystride = c.qstride; A.ny = c.nq;
+    A.dim = A.ydim = c.dim;
+    A.k = c.scale * kLog2e;
+    A.nsplit = cut.nsplit; A.rows_per_split = cut.rows; A.nslices = p.nslices; A.opitch = opitch_of(c.dim);
+    A.ml = reinterpret_cast<float4 *>(c.work + L.ml);
+    A.o = reinterpret_cast<float *>(c.work + L.o);
+    A.yinfo = info; A.ytarget = ytarget;
+    A.out = db; A.ostride = dbstride; A.oscale = c.scale;
+    if (p.planes && c.nq) {
+        rg_status st = make_planes<DT>(c.queries, c.qstride, c.nq, c.dim, p.ks, c.work + L.planes, info, ytarget, c.s);
+        if (st != RG_OK) return st;
+        A.y = c.work + L.planes; A.ystride = p.row_bytes / 2; A.ydim = 32 * p.ks;
+    }
+    rg_status st = launch_pass(p, A, c.s);
+    if (st != RG_OK || cut.nsplit == 1) return st;
+    const uint64_t n = (uint64_t)rows * c.dim;
+    hipLaunchKernelGGL((rg_softmax_db_kernel<DT>), dim3((uint32_t)std::min<uint64_t>((n + 255) / 256, 1u << 20)), dim3(256), 0, c.s, A.ml, A.o, A.opitch, cut.nsplit, rows, c.dim, c.scale, db, dbstride);
     RG_HIP(hipGetLastError());
     return RG_OK;
 }
@@ -324,7 +442,7 @@ rg_status rg_softmax_workspace(int what, uint32_t nb, uint32_t nq, uint32_t dim,
     if (what != RG_SOFTMAX_STATS && what != RG_SOFTMAX_MEAN && what != RG_SOFTMAX_GRAD) return set_error(RG_ERR_ARG, "unknown kind of call");
     rg_status st = check_shapes(nb, nq, dim, dtype);
     if (st != RG_OK) return st;
-    *bytes = scratch_of(what, nb, nq, dim, dtype).total();
+    *bytes = scratch_of(what, nb, nq, dim, dtype);
     return RG_OK;
 }
 
@@ -335,7 +453,7 @@ rg_status rg_softmax_shard_dev(const void *d_base, uint32_t nb, uint64_t bstride
     rg_status st = check_call(nb, d_base, bstride, nq, d_queries, qstride, dim, dtype, scale, id_base);
     if (st != RG_OK || nq == 0) return st;
     if (!d_targets || !d_rest || !d_own) return set_error(RG_ERR_ARG, "null argument");
-    st = check_scratch(d_work, work_bytes, scratch_of(d_mean ? RG_SOFTMAX_MEAN : RG_SOFTMAX_STATS, nb, nq, dim, dtype).total());
+    st = check_scratch(d_work, work_bytes, scratch_of(d_mean ? kMean : kStats, nb, nq, dim, dtype));
     if (st != RG_OK) return st;
     OnDevice on(device);
     if (on.st != RG_OK) return on.st;
@@ -366,7 +484,7 @@ rg_status rg_softmax_grad_dev(const void *d_base, uint32_t nb, uint64_t bstride,
     if (st == RG_OK && d_db) st = check_rows(d_db, nb, dbstride, dim, dtype, "gradient of the base");
     if (st != RG_OK) return st;
     if (nq && (!d_targets || !d_lse || !d_loss || !d_weights || (d_dq && (!d_mean || !d_rest)))) return set_error(RG_ERR_ARG, "null argument");
-    st = check_scratch(d_work, work_bytes, scratch_of(RG_SOFTMAX_GRAD, d_db ? nb : 0, nq, dim, dtype).total());
+    st = check_scratch(d_work, work_bytes, scratch_of(kRows, d_db ? nb : 0, nq, dim, dtype));
     if (st != RG_OK) return st;
     OnDevice on(device);
     if (on.st != RG_OK) return on.st;

@@ -1,13 +1,25 @@
-// instantiations of the softmax pass: f16 rows, mode kMean
-#include "rg_softmax_pass.h"
+// instantiations of the softmax pass: f16 rows, statistics and mean rows
+#include "rg_softmax_thin.h"
+#include "rg_softmax_wide.h"
 
 namespace rg {
-const void *softmax_kernel_f16_mean(int ks) {
+
+SoftmaxKernel softmax_wide_f16_mean(int ks) {
     switch (ks) {
-#define RG_KS(K) case K: return reinterpret_cast<const void *>(rg_softmax_pass_kernel<RG_DTYPE_F16, K, kMean>);
-        RG_KS(2) RG_KS(4) RG_KS(7) RG_KS(8) RG_KS(12) RG_KS(16) RG_KS(24)
+#define RG_KS(K) case K: return {reinterpret_cast<const void *>(rg_softmax_wide_kernel<RG_DTYPE_F16, K, kMean>), (uint32_t)WideCfg<RG_DTYPE_F16, K, kMean>::XT, (uint32_t)WideCfg<RG_DTYPE_F16, K, kMean>::OB, (uint32_t)WideCfg<RG_DTYPE_F16, K, kMean>::LDS, 1u};
+        RG_KS(2) RG_KS(4) RG_KS(7) RG_KS(8) RG_KS(12) RG_KS(16) RG_KS(24) RG_KS(32)
 #undef RG_KS
-        default: return reinterpret_cast<const void *>(rg_softmax_pass_kernel<RG_DTYPE_F16, 32, kMean>);
+        default: return {};
     }
 }
+
+SoftmaxKernel softmax_thin_f16_mean(int ks) {
+    switch (ks) {
+#define RG_KS(K) case K: return {reinterpret_cast<const void *>(rg_softmax_thin_kernel<RG_DTYPE_F16, K, kMean>), (uint32_t)ThinCfg<RG_DTYPE_F16, K>::XT, (uint32_t)ThinCfg<RG_DTYPE_F16, K>::OB, (uint32_t)ThinCfg<RG_DTYPE_F16, K>::LDS, (uint32_t)ThinCfg<RG_DTYPE_F16, K>::WPS};
+        RG_KS(2) RG_KS(4) RG_KS(7) RG_KS(8) RG_KS(12) RG_KS(16) RG_KS(24) RG_KS(32)
+#undef RG_KS
+        default: return {};
+    }
+}
+
 }  // namespace rg

@@ -1,0 +1,314 @@
+// rg_softmax_thin.h -- the pass of the softmax operators for few stationary rows (at most 64): bound by memory, so the streamed rows are
+// read once in the caller's type and layout, through registers (where fp32 rows are split), and every wave holds one block of 16 rows x.
+// rg_softmax_pass.h has the mathematics, the operand layouts and the LDS swizzle.
+#pragma once
+#include "rg_softmax_pass.h"
+
+namespace rg {
+
+template <int DT, int KS>
+struct ThinCfg {
+    static constexpr int NP = DT == RG_DTYPE_F32 ? 2 : 1;
+    static constexpr int OB = KS == 7 ? 13 : (DT == RG_DTYPE_F32 && KS == 32) ? 32 : 2 * KS;
+    static constexpr int XT = 64;
+    static constexpr int TY = 32;
+    static constexpr int PITCH = (KS * 64 + 255) / 256 * 256;
+    static constexpr int PLANE = TY * PITCH;
+    static constexpr int BUF = NP * PLANE;
+    static constexpr int NBUF = 2 * BUF <= 128 * 1024 ? 2 : 1;
+    static constexpr int LDS = NBUF * (BUF + TY * 8);           // a factor and a bias per row
+    static constexpr int WPS = (DT == RG_DTYPE_F32 ? KS <= 8 : KS <= 16) ? 2 : 1;
+};
+
+template <int DT, int KS, int MODE>
+__global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_kernel(PassArgs A) {
+    typedef ThinCfg<DT, KS> C;
+    typedef typename Elem<DT>::T T;
+    typedef typename Frag<DT>::V V;
+    constexpr int NP = C::NP, NX = 1, OB = C::OB, PITCH = C::PITCH, CI = (KS + 3) / 4;
+    constexpr bool F32 = DT == RG_DTYPE_F32;
+    constexpr float kTop = 15.0f, kStart = DT == RG_DTYPE_BF16 ? 0.0f : 7.0f;   // a weight is at most 2^15; the first largest one 2^0 / 2^7
+    extern __shared__ char lds[];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
+    const uint32_t b = xcd_block(blockIdx.x, gridDim.x);
+    const uint32_t slice = MODE == kStats ? 0 : b % A.nslices, split = MODE == kStats ? b : b / A.nslices;
+    const uint32_t ybeg = min(A.ny, split * A.rows_per_split), yend = min(A.ny, ybeg + A.rows_per_split);
+    const uint32_t x0 = wave * 16;
+    const bool live = x0 < A.nx;                                // waves behind the last row only help to load
+    const uint32_t dim = A.dim;
+    const size_t esz = sizeof(T);
+    const bool xvec = ((uintptr_t)A.x | A.xstride * esz) % 16 == 0, yvec = ((uintptr_t)A.y | A.ystride * esz) % 16 == 0;
+
+    V X[NX][KS][NP];
+    float kx[NX];
+    uint32_t target[NX];
+#pragma unroll
+    for (int j = 0; j < NX; ++j) {
+        const uint32_t x = x0 + j * 16 + n;
+        kx[j] = load_stationary<DT, KS>(A, x, g, xvec, X[j]);
+        target[j] = kNoTarget;
+        if (x < A.nx) {
+            const uint32_t t = A.targets[x];
+            if (t != kNoTarget && t >= A.id_base && t - A.id_base >= ybeg && t - A.id_base < yend) target[j] = t - A.id_base;
+        }
+    }
+
+    f32x4 O[MODE == kStats ? 1 : OB][NX];
+    // M: reference of the weights of O; with fp32 rows those carry the rows' scales, so that the sum l has a reference Ml of its own
+    constexpr bool TWO = F32 && MODE == kMean;
+    float M[NX], l[NX], Ml[NX];
+#pragma unroll
+    for (int j = 0; j < NX; ++j) {
+        M[j] = Ml[j] = kNothing;
+        l[j] = 0.0f;
+        if (MODE != kStats)
+#pragma unroll
+            for (int ob = 0; ob < OB; ++ob) O[ob][j] = f32x4{0, 0, 0, 0};
+    }
+
+    // streaming: 16 lanes per row, two rows per thread (r, r + 16)
+    const uint32_t lr = tid >> 4, lc = tid & 15;
+    Chunk<DT> stage[2][CI];
+    auto fetch = [&](uint32_t y0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t y = y0 + lr + 16 * h;
+            const char *row = static_cast<const char *>(A.y) + (size_t)y * A.ystride * esz;
+#pragma unroll
+            for (int i = 0; i < CI; ++i) stage[h][i] = load_chunk<DT>(row, 8 * (lc + 16 * i), y < yend ? dim : 0, yvec);
+        }
+    };
+    auto commit = [&](uint32_t buf) {
+        char *tile = lds + buf * C::BUF;
+        float *yv = reinterpret_cast<float *>(lds + C::NBUF * C::BUF) + buf * C::TY * 2;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t r = lr + 16 * h, sw = ((r & 7) << 1) | ((r >> 3) & 1);
+            int e = 0;
+            float top = 0.0f;
+            if constexpr (F32) {
+                uint32_t m = 0;
+#pragma unroll
+                for (int i = 0; i < CI; ++i) m = max(m, __float_as_uint(absmax(stage[h][i])));
+#pragma unroll
+                for (int d = 1; d < 16; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
+                top = __uint_as_float(m);
+                e = row_exponent(top);
+            }
+            const float s = F32 ? pow2(-e) : 1.0f;
+#pragma unroll
+            for (int i = 0; i < CI; ++i) {
+                const uint32_t c = lc + 16 * i;
+                if (KS * 4 % 16 == 0 || c < (uint32_t)KS * 4) {
+                    char *at = tile + r * PITCH + i * 256 + ((lc ^ sw) << 4);
+                    if constexpr (F32) {
+                        half8 hi, lo;
+                        split8(stage[h][i], top, s, hi, lo);
+                        *reinterpret_cast<half8 *>(at) = hi;
+                        *reinterpret_cast<half8 *>(at + C::PLANE) = lo;
+                    } else {
+                        *reinterpret_cast<u32x4 *>(at) = stage[h][i].v;
+                    }
+                }
+            }
+            if (F32 && lc == 0) {
+                yv[r] = row_factor(top, e);
+                yv[32 + r] = MODE == kMean ? (float)e : 0.0f;
+            }
+        }
+    };
+
+    auto compute = [&](uint32_t buf, uint32_t y0) {
+        const char *tile = lds + buf * C::BUF;
+        const float *yv = reinterpret_cast<const float *>(lds + C::NBUF * C::BUF) + buf * C::TY * 2;
+        f32x4 S[2][NX];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < NX; ++j) S[h][j] = f32x4{0, 0, 0, 0};
+        {
+            const uint32_t sw = ((n & 7) << 1) | (n >> 3);      // (row + 16: the same swizzle)
+            const char *row = tile + n * PITCH;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const uint32_t c = 4 * ks + g;
+                const char *at = row + (c & ~15u) * 16 + (((c & 15) ^ sw) << 4);
+                V a[2][NP];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int p = 0; p < NP; ++p) a[h][p] = *reinterpret_cast<const V *>(at + h * 16 * PITCH + p * C::PLANE);
+                if constexpr (F32) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int j = 0; j < NX; ++j) S[h][j] = mma(a[h][1], X[j][ks][0], S[h][j]);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int j = 0; j < NX; ++j) S[h][j] = mma(a[h][0], X[j][ks][1], S[h][j]);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < NX; ++j) S[h][j] = mma(a[h][0], X[j][ks][0], S[h][j]);
+            }
+        }
+        f32x4 ky[2], bias[2];
+        if (F32)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                ky[h] = *reinterpret_cast<const f32x4 *>(yv + 16 * h + 4 * g);
+                bias[h] = *reinterpret_cast<const f32x4 *>(yv + 32 + 16 * h + 4 * g);
+            }
+        const bool tail = y0 + 32 > yend;
+        const bool met = __any(target[0] - y0 < 32);            // a target of these rows lies in the tile
+#pragma unroll
+        for (int j = 0; j < NX; ++j) {
+            const uint32_t x = x0 + j * 16 + n;
+            uint32_t dead = 0;                                  // bits of the elements (h, i) that take no part
+            if (met || tail) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t r = 16 * h + 4 * g + i;
+                        if (y0 + r == target[j]) {
+                            float z = S[h][j][i];
+                            if (F32) z *= ky[h][i];
+                            if (slice == 0) A.own2[x] = z * kx[j];
+                            dead |= 1u << (4 * h + i);
+                        }
+                        if (y0 + r >= yend) dead |= 1u << (4 * h + i);
+                    }
+            }
+            // the logit of element (h, i), in units of log 2, minus a reference
+            auto logit = [&](int h, int i, bool biased, float ref) {
+                float z = S[h][j][i];
+                if (F32) z *= ky[h][i];
+                z = fmaf(z, kx[j], biased ? bias[h][i] - ref : -ref);
+                if (met || tail)
+                    if (dead >> (4 * h + i) & 1) z = -INFINITY;
+                return z;
+            };
+            // weights 2^(logit - ref) under a reference that moves where one would pass 2^kTop; true where it moved, by a factor `old`
+            auto weigh = [&](bool biased, float &ref, float &old, float (&p)[2][4]) {
+                float top = kNothing;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        p[h][i] = logit(h, i, biased, ref);
+                        top = fmaxf(top, p[h][i]);
+                    }
+                const bool move = __any(top > kTop);
+                if (move) {
+                    float z = kNothing;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            p[h][i] = logit(h, i, biased, 0.0f);
+                            z = fmaxf(z, p[h][i]);
+                        }
+                    z = fmaxf(z, __shfl_xor(z, 16));
+                    z = fmaxf(z, __shfl_xor(z, 32));
+                    const float to = z - ref > kTop ? z - kStart : ref;
+                    old = exp2_hw(ref - to);
+                    ref = to;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) p[h][i] -= to;
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) p[h][i] = exp2_hw(p[h][i]);
+                return move;
+            };
+            float p[2][4], old = 1.0f;
+            if (TWO) {
+                if (weigh(false, Ml[j], old, p)) l[j] *= old;
+                l[j] += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
+            }
+            if (weigh(TWO, M[j], old, p)) {
+                if (!TWO) l[j] *= old;
+                if (MODE != kStats)
+#pragma unroll
+                    for (int ob = 0; ob < OB; ++ob) O[ob][j] *= old;
+            }
+            if (!TWO) l[j] += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
+            if constexpr (MODE != kStats) {
+                V w, wl;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if constexpr (DT == RG_DTYPE_BF16) {
+                            w[4 * h + i] = (__bf16)p[h][i];
+                        } else {
+                            w[4 * h + i] = (_Float16)p[h][i];
+                            if (F32) wl[4 * h + i] = (_Float16)(p[h][i] - (float)w[4 * h + i]);
+                        }
+                    }
+                S[0][j] = __builtin_bit_cast(f32x4, w);
+                if (F32) S[1][j] = __builtin_bit_cast(f32x4, wl);
+            }
+        }
+        if constexpr (MODE != kStats) {
+            // lane (n, g) reads 8 bytes of row 4 g + n / 4 (and + 16) at dims 4 (n % 4) of the block, and receives dim n of rows 4 g .. + 3
+            typedef __attribute__((address_space(3))) s16x4 *tr_ptr;
+            const uint32_t r = 4 * g + (n >> 2), sw = ((r & 7) << 1) | ((r >> 3) & 1);     // (row + 16: the same swizzle)
+            const char *row = tile + r * PITCH + (n & 1) * 8;
+#pragma unroll
+            for (int ob = 0; ob < OB; ++ob) {
+                const uint32_t c = 2 * (slice * OB + ob) + ((n >> 1) & 1);
+                const char *at = row + (c & ~15u) * 16 + (((c & 15) ^ sw) << 4);
+                V a[NP];
+#pragma unroll
+                for (int p = 0; p < NP; ++p) {
+                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(const_cast<char *>(at) + p * C::PLANE));
+                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(const_cast<char *>(at) + p * C::PLANE + 16 * PITCH));
+                    a[p] = __builtin_bit_cast(V, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+#pragma unroll
+                for (int j = 0; j < NX; ++j) {
+                    if constexpr (F32) {
+                        O[ob][j] = mma(a[1], __builtin_bit_cast(V, S[0][j]), O[ob][j]);
+                        O[ob][j] = mma(a[0], __builtin_bit_cast(V, S[1][j]), O[ob][j]);
+                    }
+                    O[ob][j] = mma(a[0], __builtin_bit_cast(V, S[0][j]), O[ob][j]);
+                }
+            }
+        }
+    };
+
+    if (ybeg < yend) {
+        if constexpr (C::NBUF == 2) {
+            fetch(ybeg);
+            commit(0);
+            __syncthreads();
+            uint32_t buf = 0;
+            for (uint32_t y0 = ybeg; y0 < yend; y0 += 32, buf ^= 1) {
+                const bool more = y0 + 32 < yend;
+                if (more) fetch(y0 + 32);
+                if (live) compute(buf, y0);
+                if (more) commit(buf ^ 1);
+                __syncthreads();
+            }
+        } else {
+            for (uint32_t y0 = ybeg; y0 < yend; y0 += 32) {
+                fetch(y0);
+                commit(0);
+                __syncthreads();
+                if (live) compute(0, y0);
+                __syncthreads();
+            }
+        }
+    }
+
+    finish<DT, MODE, OB, NX>(A, x0, n, g, slice, split, M, TWO ? Ml : M, l, O);
+}
+
+}  // namespace rg
