@@ -225,7 +225,7 @@ struct Plan {
         uint32_t nsplit, rows;
     };
     Cut cut(uint32_t rows) const {
-        const uint64_t nt = (uint64_t)ntx * nslices, places = 256ull * std::min<uint32_t>(k.wps, 160 * 1024 / k.lds);
+        const uint64_t nt = (uint64_t)ntx * nslices, places = 256ull * std::min<uint32_t>(k.wps * 256 / k.threads, 160 * 1024 / k.lds);     // (256 CUs)
         const uint32_t most = std::max(1u, rows / 128);
         uint32_t best = 1;
         double best_use = 0;
@@ -294,7 +294,11 @@ uint64_t scratch_of(int mode, uint32_t nb, uint32_t nq, uint32_t dim, int dtype)
     if (dtype != RG_DTYPE_F32 && dim % 8 == 0) n = std::max(n, layout_of(plan_of(dtype, mode, dim, nx, ny, true), mode, dtype, dim).total);
     return n;
 }
-bool direct_rows(const void *rows, uint64_t stride, uint32_t dim, int dtype) { return dtype != RG_DTYPE_F32 && dim % 8 == 0 && stride % 8 == 0 && (uintptr_t)rows % 16 == 0; }
+bool direct_rows(const void *rows, uint64_t stride, uint32_t dim, int dtype) {
+    return dtype != RG_DTYPE_F32 && dim % 8 == 0 && stride % 8 == 0 && stride < (1u << 25) && (uintptr_t)rows % 16 == 0;     // (32 rows' bytes in 32 bits)
+}
+// scale in units of log 2; a scale of zero becomes one that no product makes visible (replaced products are divided by it)
+float k_of(float scale) { return scale == 0.0f ? 1e-30f : scale * kLog2e; }
 
 template <int DT>
 rg_status make_planes(const void *rows, uint64_t stride, uint32_t n, uint32_t dim, int ks, void *planes, float4 *info, float *ytarget, hipStream_t s) {
@@ -310,7 +314,7 @@ rg_status launch_pass(const Plan &p, const PassArgs &A, hipStream_t s) {
     if (grid > 0xffffffull) return set_error(RG_ERR_ARG, "softmax over a base: too many rows for one launch");
     RG_HIP(hipFuncSetAttribute(p.k.kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.k.lds));
     void *args[] = {const_cast<PassArgs *>(&A)};
-    RG_HIP(hipLaunchKernel(p.k.kern, dim3((uint32_t)grid), dim3(256), args, p.k.lds, s));
+    RG_HIP(hipLaunchKernel(p.k.kern, dim3((uint32_t)grid), dim3(p.k.threads), args, p.k.lds, s));
     return RG_OK;
 }
 
@@ -363,7 +367,7 @@ rg_status shard(const Call &c, float *rest, float *own, float *lse, float *loss,
     PassArgs A{};
     A.x = c.queries; A.xstride = c.qstride; A.nx = c.nq;
     A.dim = A.ydim = c.dim;
-    A.k = c.scale * kLog2e;
+    A.k = k_of(c.scale);
     A.nslices = p.nslices; A.opitch = opitch_of(c.dim);
     A.targets = c.targets; A.own2 = reinterpret_cast<float *>(c.work + L.aux);
     float4 *ml = reinterpret_cast<float4 *>(c.work + L.ml);
@@ -411,7 +415,7 @@ rg_status grad(const Call &c, const float *lse, const float *loss, const float *
     A.x = c.base; A.xstride = c.bstride; A.nx = rows;
     A.y = c.queries; A.ystride = c.qstride; A.ny = c.nq;
     A.dim = A.ydim = c.dim;
-    A.k = c.scale * kLog2e;
+    A.k = k_of(c.scale);
     A.nsplit = cut.nsplit; A.rows_per_split = cut.rows; A.nslices = p.nslices; A.opitch = opitch_of(c.dim);
     A.ml = reinterpret_cast<float4 *>(c.work + L.ml);
     A.o = reinterpret_cast<float *>(c.work + L.o);

@@ -6,7 +6,7 @@ namespace rg {
 
 SoftmaxKernel softmax_wide_f16_stats(int ks) {
     switch (ks) {
-#define RG_KS(K) case K: return {reinterpret_cast<const void *>(rg_softmax_wide_kernel<RG_DTYPE_F16, K, kStats>), (uint32_t)WideCfg<RG_DTYPE_F16, K, kStats>::XT, (uint32_t)WideCfg<RG_DTYPE_F16, K, kStats>::OB, (uint32_t)WideCfg<RG_DTYPE_F16, K, kStats>::LDS, 1u};
+#define RG_KS(K) case K: return {reinterpret_cast<const void *>(rg_softmax_wide_kernel<RG_DTYPE_F16, K, kStats>), (uint32_t)WideCfg<RG_DTYPE_F16, K, kStats>::XT, (uint32_t)WideCfg<RG_DTYPE_F16, K, kStats>::OB, (uint32_t)WideCfg<RG_DTYPE_F16, K, kStats>::LDS, (uint32_t)WideCfg<RG_DTYPE_F16, K, kStats>::WPS, (uint32_t)WideCfg<RG_DTYPE_F16, K, kStats>::NT};
         RG_KS(2) RG_KS(4) RG_KS(7) RG_KS(8) RG_KS(12) RG_KS(16) RG_KS(24) RG_KS(32)
 #undef RG_KS
         default: return {};
@@ -15,7 +15,7 @@ SoftmaxKernel softmax_wide_f16_stats(int ks) {
 
 SoftmaxKernel softmax_thin_f16_stats(int ks) {
     switch (ks) {
-#define RG_KS(K) case K: return {reinterpret_cast<const void *>(rg_softmax_thin_kernel<RG_DTYPE_F16, K, kStats>), (uint32_t)ThinCfg<RG_DTYPE_F16, K>::XT, (uint32_t)ThinCfg<RG_DTYPE_F16, K>::OB, (uint32_t)ThinCfg<RG_DTYPE_F16, K>::LDS, (uint32_t)ThinCfg<RG_DTYPE_F16, K>::WPS};
+#define RG_KS(K) case K: return {reinterpret_cast<const void *>(rg_softmax_thin_kernel<RG_DTYPE_F16, K, kStats>), (uint32_t)ThinCfg<RG_DTYPE_F16, K>::XT, (uint32_t)ThinCfg<RG_DTYPE_F16, K>::OB, (uint32_t)ThinCfg<RG_DTYPE_F16, K>::LDS, (uint32_t)ThinCfg<RG_DTYPE_F16, K>::WPS, 256u};
         RG_KS(2) RG_KS(4) RG_KS(7) RG_KS(8) RG_KS(12) RG_KS(16) RG_KS(24) RG_KS(32)
 #undef RG_KS
         default: return {};

@@ -49,10 +49,10 @@ struct PassArgs {
     float oscale;
 };
 
-// an instantiation: rows x of a workgroup, blocks of 16 output dims per slice, bytes of LDS, waves per SIMD (rg_softmax_inst_*.hip)
+// an instantiation: rows x of a workgroup, blocks of 16 output dims per slice, bytes of LDS, waves per SIMD, threads (rg_softmax_inst_*.hip)
 struct SoftmaxKernel {
     const void *kern;
-    uint32_t xt, ob, lds, wps;
+    uint32_t xt, ob, lds, wps, threads;
 };
 #define RG_SOFTMAX_KERNELS(DT)                    \
     SoftmaxKernel softmax_thin_##DT##_stats(int ks); \

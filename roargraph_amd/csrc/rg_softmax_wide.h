@@ -17,32 +17,54 @@
 
 namespace rg {
 
+struct WideChoice {
+    int nx, waves, wps;
+    bool loop3;
+};
+constexpr WideChoice softmax_wide_cfg(int dt, int ks, int mode) {
+    const bool f32 = dt == RG_DTYPE_F32;
+#ifdef RG_WIDE_CFG
+    return RG_WIDE_CFG;
+#else
+    if (mode == kStats) {
+        if (f32) return ks <= 4 ? WideChoice{3, 8, 2, false} : ks <= 7 ? WideChoice{2, 8, 2, false} : ks <= 16 ? WideChoice{1, 8, 2, false} : WideChoice{1, 4, 1, false};
+        return ks <= 7 ? WideChoice{4, 8, 2, false} : ks <= 8 ? WideChoice{3, 8, 2, false} : ks <= 16 ? WideChoice{2, 8, 2, false} : WideChoice{1, 8, 2, false};
+    }
+    if (f32) return ks <= 4 ? WideChoice{2, 8, 2, false} : ks <= 8 ? WideChoice{1, 8, 2, false} : ks <= 12 ? WideChoice{2, 4, 1, false} : WideChoice{1, 4, 1, false};
+    return ks <= 4 ? WideChoice{3, 8, 2, false} : ks <= 7 ? WideChoice{2, 8, 2, false} : ks <= 16 ? WideChoice{1, 8, 2, false} : WideChoice{1, 4, 1, false};
+#endif
+}
+
 template <int DT, int KS, int MODE>
 struct WideCfg {
     static constexpr bool F32 = DT == RG_DTYPE_F32;
     static constexpr int NP = F32 ? 2 : 1;
     static constexpr int OB = KS == 7 ? 13 : F32 && KS == 32 ? 32 : 2 * KS;
-    // registers of a lane: X 4 NP KS per block, O 4 OB, logits 16, weights 4 NP
-    static constexpr int NX = MODE == kStats ? (F32 ? (KS <= 8 ? 4 : KS <= 12 ? 3 : KS <= 16 ? 2 : 1) : (KS <= 8 ? 6 : KS <= 12 ? 5 : KS <= 16 ? 4 : KS <= 24 ? 3 : 2))
-                              : F32          ? (KS <= 4 ? 4 : KS <= 8 ? 2 : 1)
-                                             : (KS <= 4 ? 4 : KS <= 7 ? 3 : KS <= 12 ? 2 : 1);
-    static constexpr int XT = 64 * NX;
+    static constexpr int NX = softmax_wide_cfg(DT, KS, MODE).nx, WAVES = softmax_wide_cfg(DT, KS, MODE).waves, WPS = softmax_wide_cfg(DT, KS, MODE).wps;
+    static constexpr bool LOOP3 = softmax_wide_cfg(DT, KS, MODE).loop3;
+    static constexpr int NT = 64 * WAVES;
+    static constexpr int XT = 16 * NX * WAVES;
     static constexpr int TY = 32;
     static constexpr int PITCH = (KS * 64 + 255) / 256 * 256;
     static constexpr int PLANE = TY * PITCH;
     static constexpr int BUF = NP * PLANE;
     static constexpr bool INFO = F32 || MODE == kRows;
-    static constexpr int NI = BUF / 4096 + (INFO ? 1 : 0);      // loads of a tile, per wave
-    static constexpr int FIT = 160 * 1024 / (BUF + (INFO ? TY * 16 : 0));
+    static constexpr int NI = BUF / (16 * NT) + (INFO ? 1 : 0);      // loads of a tile, per wave
+    static constexpr int FIT = 160 * 1024 * WAVES / (4 * WPS) / (BUF + (INFO ? TY * 16 : 0));
     static constexpr int NBUF = FIT > 8 ? 8 : FIT;
-    static constexpr bool PIPE = MODE != kStats && NBUF >= 6;
+    static constexpr bool PIPE = LOOP3 && NBUF >= 6;
     static constexpr int LDS = NBUF * (BUF + (INFO ? TY * 16 : 0));
 };
 
-__device__ const u32x4 g_zero16 = {0, 0, 0, 0};
+// 16 bytes a lane from base + off to LDS at `to` + 16 * lane.  Written as assembly because the compiler, which cannot tell the ring's buffers
+// apart, makes every LDS read wait for all such loads; the waits are the kernel's own (`arrived`).  m0 holds the LDS address and is put back.
+__device__ __forceinline__ void load_lds16(const void *base, uint32_t off, uint32_t to) {
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0" : "=&s"(m0) : "v"(off), "s"(base), "s"(to) : "memory");
+}
 
 template <int DT, int KS, int MODE>
-__global__ void __launch_bounds__(256, 1) rg_softmax_wide_kernel(PassArgs A) {
+__global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, MODE>::WPS)) rg_softmax_wide_kernel(PassArgs A) {
     typedef WideCfg<DT, KS, MODE> C;
     typedef typename Elem<DT>::T T;
     typedef typename Frag<DT>::V V;
@@ -65,36 +87,51 @@ __global__ void __launch_bounds__(256, 1) rg_softmax_wide_kernel(PassArgs A) {
     const uint32_t x0 = xt * C::XT + wave * 16 * NX;
     const bool live = x0 < A.nx;
 
-    // tile t of this piece into buffer `buf`: 16-byte slot q of the tile is (plane, row, slot of the row)
-    constexpr int SR = PITCH / 16;
-    const uint32_t nchunks = A.ydim / 8;
-    // (a tile behind the last is loaded as zeros, so that the number of loads on their way is always known)
-    auto load = [&](uint32_t t) {
-        const uint32_t buf = t % NBUF, y0 = ybeg + 32 * t, left = y0 < yend ? yend - y0 : 0;
-        const char *first = static_cast<const char *>(A.y) + (size_t)y0 * A.ystride * 2;
-#pragma unroll
-        for (int i = 0; i < C::BUF / 4096; ++i) {
-            const uint32_t q = i * 256 + tid, row = q / SR, slot = q % SR, r = row & 31, p = row >> 5;
-            const uint32_t c = (slot & ~15u) | ((slot & 15) ^ (((r & 7) << 1) | (r >> 3 & 1)));
-            const char *at = first + (size_t)r * A.ystride * 2 + p * (KS * 64) + c * 16;
-            if (c >= nchunks || r >= left) at = reinterpret_cast<const char *>(&g_zero16);
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)at,
-                                             (__attribute__((address_space(3))) void *)(lds + buf * C::BUF + (i * 256 + wave * 64) * 16), 16, 0, 0);
-        }
-        if (INFO && lane < 8) {
-            const float4 *at = A.yinfo + (left ? y0 : ybeg) + wave * 8 + lane;
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)at, (__attribute__((address_space(3))) void *)(lds + NBUF * C::BUF + buf * 512 + wave * 128), 16, 0, 0);
-        }
+    // tile t of this piece into its buffer: 16-byte slot q of a plane of the tile is (row, slot of the row).  Rows behind the last one are
+    // loaded as the last (they take no part); chunks behind the rows' elements are not loaded and stay zero.
+    constexpr int SR = PITCH / 16, PER = 32 * SR / C::NT;
+    const uint32_t nchunks = A.ydim / 8, ystep = (uint32_t)A.ystride * 2;           // (32 rows' bytes fit 32 bits: the host's rule)
+    const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    auto offset = [&](int i, uint32_t rows) {
+        const uint32_t q = i * C::NT + tid, r = q / SR, slot = q % SR;
+        const uint32_t c = (slot & ~15u) | ((slot & 15) ^ (((r & 7) << 1) | (r >> 3 & 1)));
+        return c < nchunks ? min(r, rows - 1) * ystep + c * 16 : c < 4 * KS ? 0xffffffffu : min(r, rows - 1) * ystep;
     };
-    // all but the last `newer` tiles' loads have landed, for all waves (loads land in the order they were issued)
-    auto arrived = [&](auto newer) {
+    uint32_t off[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) off[i] = offset(i, 32);
+    const bool holes = nchunks < 4 * KS;
+    if (holes) {                                    // what no load writes
+        for (uint32_t i = tid; i < NBUF * C::BUF / 16; i += C::NT) reinterpret_cast<u32x4 *>(lds)[i] = u32x4{0, 0, 0, 0};
+        __syncthreads();
+    }
+    auto load = [&](uint32_t t) {
+        const uint32_t buf = t % NBUF, y0 = ybeg + 32 * t, to = __builtin_amdgcn_readfirstlane(ring + buf * C::BUF + wave * 1024);
+        const char *first = static_cast<const char *>(A.y) + (size_t)y0 * A.ystride * 2;
+        const uint32_t rows = yend - y0;
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const uint32_t o = rows < 32 ? offset(i, rows) : off[i];
+                if (!holes || o != 0xffffffffu) load_lds16(first + p * (KS * 64), o, to + (p * PER + i) * (16 * C::NT));
+            }
+        constexpr uint32_t each = 32 / C::WAVES;
+        if (INFO && lane < each) load_lds16(A.yinfo + y0 + wave * each, lane * 16, __builtin_amdgcn_readfirstlane(ring + NBUF * C::BUF + buf * 512 + wave * each * 16));
+    };
+    // tile t has landed, for all waves; `newer` tiles may still be on their way (loads land in the order they were issued; near the end,
+    // where fewer are, all are waited for)
+    auto arrived = [&](uint32_t t, auto newer) {
         constexpr int N = decltype(newer)::value * C::NI;
         static_assert(N >= 0 && N < 64, "vmcnt");
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+        if (t + decltype(newer)::value < ntiles)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
     };
     if (ntiles)
-        for (uint32_t t = 0; t + 1 < (NBUF > 1 ? NBUF : 2); ++t) load(t);
+        for (uint32_t t = 0; t + 1 < (NBUF > 1 ? NBUF : 2) && t < ntiles; ++t) load(t);
 
     V X[NX][KS][NP];
     float kx[NX];
@@ -110,6 +147,7 @@ __global__ void __launch_bounds__(256, 1) rg_softmax_wide_kernel(PassArgs A) {
             if (tg != kNoTarget && tg >= A.id_base && tg - A.id_base >= ybeg && tg - A.id_base < yend) target[j] = tg - A.id_base;
         }
     }
+    __builtin_amdgcn_s_waitcnt(0x0f70);             // the compiler's own loads (vmcnt(0)): none of its waits is left for the loop
     f32x4 O[MODE == kStats ? 1 : OB][NX];
     float M[NX], l[NX], Ml[NX];
 #pragma unroll
@@ -122,109 +160,133 @@ __global__ void __launch_bounds__(256, 1) rg_softmax_wide_kernel(PassArgs A) {
             for (int ob = 0; ob < OB; ++ob) O[ob][j] = f32x4{0, 0, 0, 0};
     }
 
+    // LDS operands are asked for AHEAD steps before the products that take them, and the compiler is kept from moving the reads back
+    // (vector and scalar instructions may still move between the products)
+    auto keep_order = [] { __builtin_amdgcn_sched_barrier(0x6); };
     auto first_product = [&](uint32_t buf, f32x4 (&S)[NX][2]) {
+        constexpr int AHEAD = C::WPS == 1 ? 2 : 1;
         const char *row = lds + buf * C::BUF + n * PITCH;
         const uint32_t sw = ((n & 7) << 1) | (n >> 3);
-#pragma unroll
-        for (int j = 0; j < NX; ++j) S[j][0] = S[j][1] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
+        V a[AHEAD + 1][2][NP];
+        auto read = [&](int ks) {
             const uint32_t c = 4 * ks + g;
             const char *at = row + (c & ~15u) * 16 + (((c & 15) ^ sw) << 4);
-            V a[2][NP];
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int p = 0; p < NP; ++p) a[h][p] = *reinterpret_cast<const V *>(at + h * 16 * PITCH + p * C::PLANE);
+                for (int p = 0; p < NP; ++p) a[ks % (AHEAD + 1)][h][p] = *reinterpret_cast<const V *>(at + h * 16 * PITCH + p * C::PLANE);
+        };
+#pragma unroll
+        for (int j = 0; j < NX; ++j) S[j][0] = S[j][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int ks = 0; ks < AHEAD && ks < KS; ++ks) read(ks);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            if (ks + AHEAD < KS) read(ks + AHEAD);
+            keep_order();
+            const V(&v)[2][NP] = a[ks % (AHEAD + 1)];
             if constexpr (F32) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int j = 0; j < NX; ++j) S[j][h] = mma(a[h][1], X[j][ks][0], S[j][h]);
+                    for (int j = 0; j < NX; ++j) S[j][h] = mma(v[h][1], X[j][ks][0], S[j][h]);
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int j = 0; j < NX; ++j) S[j][h] = mma(a[h][0], X[j][ks][1], S[j][h]);
+                    for (int j = 0; j < NX; ++j) S[j][h] = mma(v[h][0], X[j][ks][1], S[j][h]);
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int j = 0; j < NX; ++j) S[j][h] = mma(a[h][0], X[j][ks][0], S[j][h]);
+                for (int j = 0; j < NX; ++j) S[j][h] = mma(v[h][0], X[j][ks][0], S[j][h]);
+            keep_order();
         }
     };
     auto second_product = [&](uint32_t buf, const V (&W)[NX][NP]) {
         if constexpr (MODE != kStats) {
             typedef __attribute__((address_space(3))) s16x4 *tr_ptr;
+            constexpr int AHEAD = C::WPS == 1 && !F32 ? 3 : 2;
             const uint32_t r = 4 * g + (n >> 2), sw = ((r & 7) << 1) | ((r >> 3) & 1);
             const char *row = lds + buf * C::BUF + r * PITCH + (n & 1) * 8;
-#pragma unroll
-            for (int ob = 0; ob < OB; ++ob) {
+            s16x4 a[AHEAD + 1][NP][2];
+            auto read = [&](int ob) {
                 const uint32_t c = 2 * (slice * OB + ob) + ((n >> 1) & 1);
                 const char *at = row + (c & ~15u) * 16 + (((c & 15) ^ sw) << 4);
-                V a[NP];
 #pragma unroll
-                for (int p = 0; p < NP; ++p) {
-                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(const_cast<char *>(at) + p * C::PLANE));
-                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(const_cast<char *>(at) + p * C::PLANE + 16 * PITCH));
-                    a[p] = __builtin_bit_cast(V, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-                }
+                for (int p = 0; p < NP; ++p)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) a[ob % (AHEAD + 1)][p][h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(const_cast<char *>(at) + p * C::PLANE + h * 16 * PITCH));
+            };
+#pragma unroll
+            for (int ob = 0; ob < AHEAD && ob < OB; ++ob) read(ob);
+#pragma unroll
+            for (int ob = 0; ob < OB; ++ob) {
+                if (ob + AHEAD < OB) read(ob + AHEAD);
+                keep_order();
+                V v[NP];
+#pragma unroll
+                for (int p = 0; p < NP; ++p) v[p] = __builtin_bit_cast(V, __builtin_shufflevector(a[ob % (AHEAD + 1)][p][0], a[ob % (AHEAD + 1)][p][1], 0, 1, 2, 3, 4, 5, 6, 7));
                 if constexpr (F32) {
 #pragma unroll
-                    for (int j = 0; j < NX; ++j) O[ob][j] = mma(a[1], W[j][0], O[ob][j]);
+                    for (int j = 0; j < NX; ++j) O[ob][j] = mma(v[1], W[j][0], O[ob][j]);
 #pragma unroll
-                    for (int j = 0; j < NX; ++j) O[ob][j] = mma(a[0], W[j][1], O[ob][j]);
+                    for (int j = 0; j < NX; ++j) O[ob][j] = mma(v[0], W[j][1], O[ob][j]);
                 }
 #pragma unroll
-                for (int j = 0; j < NX; ++j) O[ob][j] = mma(a[0], W[j][0], O[ob][j]);
+                for (int j = 0; j < NX; ++j) O[ob][j] = mma(v[0], W[j][0], O[ob][j]);
+                keep_order();
             }
         }
     };
 
-    // the logits of a tile, in units of log 2, minus a reference; elements (h, i) of a lane are rows 16 h + 4 g + i
+    // a tile's rows: elements (h, i) of a lane are rows 16 h + 4 g + i
     struct Tile {
         uint32_t y0, slot;          // first row; where its info lies
-        bool met, neg, tail;        // a target of these rows lies in the tile; a weight is negative; rows behind the last
+        bool rare, neg;             // a target of these rows, or rows behind the last, lie in the tile; a weight is negative
     };
     auto info = [&](const Tile &t, uint32_t r) { return *reinterpret_cast<const f32x4 *>(lds + NBUF * C::BUF + t.slot * 512 + r * 16); };
     auto look = [&](uint32_t t) {
-        Tile k{ybeg + 32 * t, t % NBUF, false, false, false};
-        k.tail = k.y0 + 32 > yend;
+        Tile k{ybeg + 32 * t, t % NBUF, false, false};
+        bool met = false;
         if (MODE != kRows) {
-            bool met = false;
 #pragma unroll
             for (int j = 0; j < NX; ++j) met |= target[j] - k.y0 < 32;
-            k.met = __any(met);
         } else {
             const f32x4 v = info(k, lane & 31);
-            k.met = __any(__float_as_uint(v[3]) - x0 < 16 * NX);
+            met = __float_as_uint(v[3]) - x0 < 16 * NX;
             k.neg = __any(v[2] < 0.0f);
         }
+        k.rare = __any(met) || k.y0 + 32 > yend;
         return k;
     };
-    uint32_t dead[NX], hit[NX];     // rare: bits of the elements that take no part / that are a query's own row
-    auto special = [&](const Tile &k, const f32x4 (&S)[NX][2]) {
+    // Rare: products are replaced so that the logits made of them come out as they should -- minus infinity for a target (whose logit is
+    // set aside) and for rows behind the last; for a query's own row the logarithm of its weight, whose sign `flip` keeps.
+    uint32_t flip[NX];
+    auto special = [&](const Tile &k, f32x4 (&S)[NX][2]) {
 #pragma unroll
         for (int j = 0; j < NX; ++j) {
-            dead[j] = hit[j] = 0;
+            flip[j] = 0;
+            const uint32_t x = x0 + j * 16 + n;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t r = 16 * h + 4 * g + i, x = x0 + j * 16 + n;
+                    const uint32_t r = 16 * h + 4 * g + i;
+                    f32x4 v{1.0f, 0.0f, 1.0f, 0.0f};
+                    if (INFO) v = info(k, r);
+                    const float f = kx[j] * v[0];
+                    bool dead = k.y0 + r >= yend;
                     if (MODE != kRows && k.y0 + r == target[j]) {
-                        float z = S[j][h][i];
-                        if (F32) z *= info(k, r)[0];
-                        if (slice == 0) A.own2[x] = z * kx[j];
-                        dead[j] |= 1u << (4 * h + i);
+                        if (slice == 0) A.own2[x] = S[j][h][i] * v[0] * kx[j];
+                        dead = true;
                     }
-                    if (MODE == kRows && __float_as_uint(info(k, r)[3]) == x) hit[j] |= 1u << (4 * h + i);
-                    if (k.y0 + r >= yend) dead[j] |= 1u << (4 * h + i);
+                    if (MODE == kRows && __float_as_uint(v[3]) == x) {
+                        if (v[1] > -INFINITY) S[j][h][i] = (A.ytarget[k.y0 + r] - v[1]) / f;
+                        flip[j] |= 1u << (4 * h + i);
+                    }
+                    if (dead) S[j][h][i] = copysignf(INFINITY, -f);
                 }
         }
-    };
-    auto fix = [&](const Tile &k, int j, int h, int i, float z, float ref) {
-        if (MODE == kRows && (hit[j] >> (4 * h + i) & 1)) z = A.ytarget[k.y0 + 16 * h + 4 * g + i] - ref;
-        return dead[j] >> (4 * h + i) & 1 ? -INFINITY : z;
     };
     auto logits = [&](const Tile &k, const f32x4 (&S)[NX][2], bool biased, const float (&ref)[NX], float (&p)[NX][2][4]) {
 #pragma unroll
@@ -236,13 +298,6 @@ __global__ void __launch_bounds__(256, 1) rg_softmax_wide_kernel(PassArgs A) {
 #pragma unroll
                 for (int j = 0; j < NX; ++j) p[j][h][i] = fmaf(F32 ? S[j][h][i] * v[0] : S[j][h][i], kx[j], biased ? v[1] - ref[j] : -ref[j]);
             }
-        if (k.met || k.tail)
-#pragma unroll
-            for (int j = 0; j < NX; ++j)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) p[j][h][i] = fix(k, j, h, i, p[j][h][i], ref[j]);
     };
     auto over = [&](const float (&p)[NX][2][4]) {
         float top = kNothing;
@@ -252,9 +307,9 @@ __global__ void __launch_bounds__(256, 1) rg_softmax_wide_kernel(PassArgs A) {
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) top = fmaxf(top, p[j][h][i]);
-        return __any(top > kTop);
+        return top > kTop;
     };
-    // moves the references of the rows that need it; returns the logits minus the new ones, and what the sums so far are multiplied by
+    // moves the references of the rows that need it; leaves the logits minus the new ones, and what the sums so far are multiplied by
     auto move = [&](const Tile &k, const f32x4 (&S)[NX][2], bool biased, float (&ref)[NX], float (&p)[NX][2][4], float (&old)[NX]) {
         float zero[NX];
 #pragma unroll
@@ -287,16 +342,7 @@ __global__ void __launch_bounds__(256, 1) rg_softmax_wide_kernel(PassArgs A) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) p[j][h][i] = exp2_hw(p[j][h][i]);
     };
-    auto pack = [&](const Tile &k, float (&p)[NX][2][4], V (&W)[NX][NP]) {
-        if (MODE == kRows && (k.neg || k.met))
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float s = info(k, 16 * h + 4 * g + i)[2];
-#pragma unroll
-                    for (int j = 0; j < NX; ++j) p[j][h][i] *= k.met && (hit[j] >> (4 * h + i) & 1) ? -s : s;
-                }
+    auto pack = [&](const float (&p)[NX][2][4], V (&W)[NX][NP]) {
 #pragma unroll
         for (int j = 0; j < NX; ++j)
 #pragma unroll
@@ -311,53 +357,75 @@ __global__ void __launch_bounds__(256, 1) rg_softmax_wide_kernel(PassArgs A) {
                     }
                 }
     };
-    // the weights of a tile; `pending`: what has to be added to O before it is rescaled
-    auto weigh = [&](const Tile &k, const f32x4 (&S)[NX][2], auto &&pending, float (&p)[NX][2][4]) {
-        if (k.met || k.tail) special(k, S);
+    auto signs = [&](const Tile &k, V (&W)[NX][NP]) {           // rare, kRows
+        uint32_t minus[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) minus[e / 2] |= (__float_as_uint(info(k, 16 * (e / 4) + 4 * g + e % 4)[2]) & 0x80000000u) >> (e % 2 ? 0 : 16);
+#pragma unroll
+        for (int j = 0; j < NX; ++j) {
+            const uint32_t f = k.rare ? flip[j] : 0;
+#pragma unroll
+            for (int q = 0; q < NP; ++q) {
+                u32x4 v = __builtin_bit_cast(u32x4, W[j][q]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] ^= minus[e] ^ ((f >> (2 * e) & 1) << 15 | (f >> (2 * e + 1) & 1) << 31);
+                W[j][q] = __builtin_bit_cast(V, v);
+            }
+        }
+    };
+    // the weights of a tile, in two halves; `pending`: what has to be added to O before it is rescaled
+    float pl[TWO ? NX : 1][2][4];
+    auto weigh_first = [&](const Tile &k, const f32x4 (&S)[NX][2], float (&p)[NX][2][4]) {
+        if constexpr (TWO) logits(k, S, false, Ml, pl);
+        logits(k, S, BIAS, M, p);
+        bool o = !NOREF && over(p);
+        if constexpr (TWO) o |= over(pl);
+        return !NOREF && __any(o);
+    };
+    auto move_all = [&](const Tile &k, const f32x4 (&S)[NX][2], auto &&pending, float (&p)[NX][2][4]) {
         float old[NX];
         if constexpr (TWO) {
-            logits(k, S, false, Ml, p);
-            if (over(p)) {
-                move(k, S, false, Ml, p, old);
+            move(k, S, false, Ml, pl, old);
 #pragma unroll
-                for (int j = 0; j < NX; ++j) l[j] *= old[j];
-            }
-            exps(p);
-#pragma unroll
-            for (int j = 0; j < NX; ++j) l[j] += sum(p[j]);
+            for (int j = 0; j < NX; ++j) l[j] *= old[j];
         }
-        logits(k, S, BIAS, M, p);
-        if (!NOREF && over(p)) {
-            pending();
-            move(k, S, BIAS, M, p, old);
+        pending();
+        move(k, S, BIAS, M, p, old);
+#pragma unroll
+        for (int j = 0; j < NX; ++j) {
+            if (!TWO) l[j] *= old[j];
+            if (MODE != kStats)
+#pragma unroll
+                for (int ob = 0; ob < OB; ++ob) O[ob][j] *= old[j];
+        }
+    };
+    auto weigh_second = [&](float (&p)[NX][2][4]) {
+        exps(p);
+        if constexpr (TWO) exps(pl);
+        if (MODE != kRows)
 #pragma unroll
             for (int j = 0; j < NX; ++j) {
-                if (!TWO) l[j] *= old[j];
-                if (MODE != kStats)
-#pragma unroll
-                    for (int ob = 0; ob < OB; ++ob) O[ob][j] *= old[j];
+                if constexpr (TWO) l[j] += sum(pl[j]);
+                else l[j] += sum(p[j]);
             }
-        }
-        exps(p);
-        if (MODE != kRows && !TWO)
-#pragma unroll
-            for (int j = 0; j < NX; ++j) l[j] += sum(p[j]);
     };
 
     if (ntiles) {
-        typedef std::integral_constant<int, 0> Zero;
         if constexpr (MODE == kStats && NBUF >= 3) {
             // first product of the next tile beside the weights of this one; tile t + NBUF - 1 takes the place of tile t - 1
             f32x4 S[NX][2], next[NX][2];
-            arrived(std::integral_constant<int, NBUF - 2>{});
+            arrived(0, std::integral_constant<int, NBUF - 2>{});
             if (live) first_product(0, S);
             for (uint32_t t = 0; t < ntiles; ++t) {
-                arrived(std::integral_constant<int, NBUF - 3>{});      // tile t + 1; every wave is through with tile t - 1
-                load(t + NBUF - 1);
+                arrived(t + 1, std::integral_constant<int, NBUF - 3>{});       // (every wave is through with tile t - 1)
+                if (t + NBUF - 1 < ntiles) load(t + NBUF - 1);
                 if (live) {
                     float p[NX][2][4];
-                    first_product((t + 1) % NBUF, next);
-                    weigh(look(t), S, [] {}, p);
+                    const Tile k = look(t);
+                    if (k.rare) special(k, S);
+                    first_product((t + 1) % NBUF, next);                       // (behind the last tile: of old rows, for nobody)
+                    if (weigh_first(k, S, p)) move_all(k, S, [] {}, p);
+                    weigh_second(p);
 #pragma unroll
                     for (int j = 0; j < NX; ++j) { S[j][0] = next[j][0]; S[j][1] = next[j][1]; }
                 }
@@ -370,26 +438,30 @@ __global__ void __launch_bounds__(256, 1) rg_softmax_wide_kernel(PassArgs A) {
             for (int j = 0; j < NX; ++j)
 #pragma unroll
                 for (int p = 0; p < NP; ++p) W[j][p] = __builtin_bit_cast(V, u32x4{0, 0, 0, 0});
-            arrived(std::integral_constant<int, NBUF - 2>{});
+            arrived(0, std::integral_constant<int, NBUF - 2>{});
             if (live) first_product(0, S);
             for (uint32_t t = 0; t < ntiles; ++t) {
-                arrived(std::integral_constant<int, NBUF - 4>{});      // tile t + 1; every wave is through with tile t - 2
-                if (t) load(t + NBUF - 2);
+                arrived(t + 1, std::integral_constant<int, NBUF - 4>{});       // (every wave is through with tile t - 2)
+                if (t && t + NBUF - 2 < ntiles) load(t + NBUF - 2);
                 if (live) {
                     float p[NX][2][4];
                     const Tile k = look(t);
+                    if (k.rare) special(k, S);
                     // (the first time round the pending product is of no rows: weights of zero, and tile 0 so that no stale bits are read)
                     const uint32_t before = t ? (t - 1) % NBUF : 0;
-                    first_product((t + 1) % NBUF, next);
-                    weigh(k, S, [&] {
-                        second_product(before, W);
+                    first_product(t + 1 < ntiles ? (t + 1) % NBUF : t % NBUF, next);
+                    if (weigh_first(k, S, p))
+                        move_all(k, S, [&] {
+                            second_product(before, W);
 #pragma unroll
-                        for (int j = 0; j < NX; ++j)
+                            for (int j = 0; j < NX; ++j)
 #pragma unroll
-                            for (int q = 0; q < NP; ++q) W[j][q] = __builtin_bit_cast(V, u32x4{0, 0, 0, 0});
-                    }, p);
+                                for (int q = 0; q < NP; ++q) W[j][q] = __builtin_bit_cast(V, u32x4{0, 0, 0, 0});
+                        }, p);
                     second_product(before, W);
-                    pack(k, p, W);
+                    weigh_second(p);
+                    pack(p, W);
+                    if (MODE == kRows && (k.rare || k.neg)) signs(k, W);
 #pragma unroll
                     for (int j = 0; j < NX; ++j) { S[j][0] = next[j][0]; S[j][1] = next[j][1]; }
                 }
@@ -400,18 +472,17 @@ __global__ void __launch_bounds__(256, 1) rg_softmax_wide_kernel(PassArgs A) {
             V W[NX][NP];
             float p[NX][2][4];
             for (uint32_t t = 0; t < ntiles; ++t) {
-                if constexpr (NBUF > 1) {
-                    arrived(std::integral_constant<int, NBUF - 2>{});  // tile t; every wave is through with tile t - 1
-                    load(t + NBUF - 1);
-                } else {
-                    arrived(Zero{});
-                }
+                arrived(t, std::integral_constant<int, (NBUF > 1 ? NBUF - 2 : 0)>{});     // (every wave is through with tile t - 1)
+                if (NBUF > 1 && t + NBUF - 1 < ntiles) load(t + NBUF - 1);
                 if (live) {
                     const Tile k = look(t);
                     first_product(t % NBUF, S);
-                    weigh(k, S, [] {}, p);
+                    if (k.rare) special(k, S);
+                    if (weigh_first(k, S, p)) move_all(k, S, [] {}, p);
+                    weigh_second(p);
                     if (MODE != kStats) {
-                        pack(k, p, W);
+                        pack(p, W);
+                        if (MODE == kRows && (k.rare || k.neg)) signs(k, W);
                         second_product(t % NBUF, W);
                     }
                 }
@@ -421,7 +492,6 @@ __global__ void __launch_bounds__(256, 1) rg_softmax_wide_kernel(PassArgs A) {
                 }
             }
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // no load may write to LDS that is no longer ours
     }
     finish<DT, MODE, OB, NX>(A, x0, n, g, slice, split, M, TWO ? Ml : M, l, O);
 }
