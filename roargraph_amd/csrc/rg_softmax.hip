@@ -101,16 +101,25 @@ __global__ void __launch_bounds__(256) rg_softmax_merge_kernel(const float *rest
     loss[i] = v;
 }
 
+// what a pass needs of a streamed row, 32 rows at a time: factors, biases, signs, targets (PassArgs::yinfo)
+__device__ __forceinline__ void put_info(float *info, uint64_t y, float factor, float bias, float sign, uint32_t target) {
+    float *at = info + (y / 32 * 128 + y % 32);
+    at[0] = factor;
+    at[32] = bias;
+    at[64] = sign;
+    at[96] = __uint_as_float(target);
+}
+
 // per query: what the pass over the rows needs of it (info and ytarget, padded to whole tiles), and dq.  One wave per query.
 template <int DT>
 __global__ void __launch_bounds__(64) rg_softmax_dq_kernel(const void *base, uint64_t bstride, uint32_t nb, uint32_t id_base, uint32_t nq, uint32_t dim, float scale,
                                                            const uint32_t *targets, const float *lse, const float *loss, const float *rest, const float *mean,
-                                                           const float *weights, void *dq, uint64_t dqstride, float4 *info, float *ytarget) {
+                                                           const float *weights, void *dq, uint64_t dqstride, float *info, float *ytarget) {
     typedef typename Elem<DT>::T T;
     const uint32_t i = blockIdx.x;
     if (i >= nq) {
         if (threadIdx.x == 0) {
-            info[i] = make_float4(1.0f, -INFINITY, 1.0f, __uint_as_float(kNoTarget));
+            put_info(info, i, 1.0f, -INFINITY, 1.0f, kNoTarget);
             ytarget[i] = -INFINITY;
         }
         return;
@@ -120,7 +129,7 @@ __global__ void __launch_bounds__(64) rg_softmax_dq_kernel(const void *base, uin
     const float w = t == kNoTarget ? 0.0f : weights[i], miss = here ? -expm1f(-loss[i]) : 0.0f;      // 1 - p_target
     if (info && threadIdx.x == 0) {
         const float lw = log2f(fabsf(w));
-        info[i] = make_float4(1.0f, t == kNoTarget ? -INFINITY : lw - lse[i] * kLog2e, w < 0.0f ? -1.0f : 1.0f, __uint_as_float(here ? row : kNoTarget));
+        put_info(info, i, 1.0f, t == kNoTarget ? -INFINITY : lw - lse[i] * kLog2e, w < 0.0f ? -1.0f : 1.0f, here ? row : kNoTarget);
         ytarget[i] = lw + log2f(miss);
     }
     if (!dq) return;
@@ -140,7 +149,7 @@ __global__ void __launch_bounds__(64) rg_softmax_dq_kernel(const void *base, uin
 // row's power of two, whose factor and exponent go to `info` (`more`: the exponent is added to what the queries' parameters already hold).
 // 16 lanes per row, CI chunks of 8 elements a lane.
 template <int DT, int CI>
-__global__ void __launch_bounds__(256) rg_softmax_planes_kernel(const void *rows, uint64_t stride, uint32_t n, uint32_t npad, uint32_t dim, uint32_t ks, uint16_t *planes, float4 *info, float *ytarget,
+__global__ void __launch_bounds__(256) rg_softmax_planes_kernel(const void *rows, uint64_t stride, uint32_t n, uint32_t npad, uint32_t dim, uint32_t ks, uint16_t *planes, float *info, float *ytarget,
                                                                 int more) {
     typedef typename Elem<DT>::T T;
     constexpr int NP = DT == RG_DTYPE_F32 ? 2 : 1;
@@ -169,11 +178,14 @@ __global__ void __launch_bounds__(256) rg_softmax_planes_kernel(const void *rows
                 *reinterpret_cast<half8 *>(out + ks * 32 + 8 * (lc + 16 * i)) = lo;
             }
             if (lc == 0) {
-                float4 v = more ? info[r] : make_float4(1.0f, 0.0f, 1.0f, __uint_as_float(kNoTarget));
-                v.x = row_factor(top, e);
-                v.y += (float)e;
-                info[r] = v;
-                if (more) ytarget[r] += (float)e;
+                if (more) {
+                    float *at = info + (r / 32 * 128 + r % 32);
+                    at[0] = row_factor(top, e);
+                    at[32] += (float)e;
+                    ytarget[r] += (float)e;
+                } else {
+                    put_info(info, r, row_factor(top, e), (float)e, 1.0f, kNoTarget);
+                }
             }
         } else {
 #pragma unroll
@@ -301,7 +313,7 @@ bool direct_rows(const void *rows, uint64_t stride, uint32_t dim, int dtype) {
 float k_of(float scale) { return scale == 0.0f ? 1e-30f : scale * kLog2e; }
 
 template <int DT>
-rg_status make_planes(const void *rows, uint64_t stride, uint32_t n, uint32_t dim, int ks, void *planes, float4 *info, float *ytarget, hipStream_t s) {
+rg_status make_planes(const void *rows, uint64_t stride, uint32_t n, uint32_t dim, int ks, void *planes, float *info, float *ytarget, hipStream_t s) {
     auto kern = ks <= 4 ? rg_softmax_planes_kernel<DT, 1> : ks <= 8 ? rg_softmax_planes_kernel<DT, 2> : ks <= 16 ? rg_softmax_planes_kernel<DT, 4> : rg_softmax_planes_kernel<DT, 8>;
     const uint32_t npad = up32(n);
     hipLaunchKernelGGL(kern, dim3(std::min(npad / 16, 1u << 16)), dim3(256), 0, s, rows, stride, n, npad, dim, (uint32_t)ks, static_cast<uint16_t *>(planes), info, ytarget, ytarget ? 1 : 0);
@@ -383,7 +395,7 @@ rg_status shard(const Call &c, float *rest, float *own, float *lse, float *loss,
         A.ml = ml + (size_t)slot * c.nq;
         A.o = o + (size_t)slot * c.nq * A.opitch;
         if (p.planes && n) {
-            float4 *info = reinterpret_cast<float4 *>(c.work + L.info);
+            float *info = reinterpret_cast<float *>(c.work + L.info);
             rg_status st = make_planes<DT>(A.y, c.bstride, n, c.dim, p.ks, c.work + L.planes, info, nullptr, c.s);
             if (st != RG_OK) return st;
             A.y = c.work + L.planes; A.ystride = p.row_bytes / 2; A.ydim = 32 * p.ks; A.yinfo = info;
@@ -402,7 +414,7 @@ rg_status grad(const Call &c, const float *lse, const float *loss, const float *
     const uint32_t rows = db ? c.nb : 0;
     const Plan p = plan_of(DT, kRows, c.dim, rows, c.nq, direct_rows(c.queries, c.qstride, c.dim, DT));
     const Layout L = layout_of(p, kRows, DT, c.dim);
-    float4 *info = rows ? reinterpret_cast<float4 *>(c.work + L.info) : nullptr;
+    float *info = rows ? reinterpret_cast<float *>(c.work + L.info) : nullptr;
     float *ytarget = rows ? reinterpret_cast<float *>(c.work + L.aux) : nullptr;
     if (c.nq) {
         hipLaunchKernelGGL((rg_softmax_dq_kernel<DT>), dim3(rows ? up32(c.nq) : c.nq), dim3(64), 0, c.s, c.base, c.bstride, c.nb, c.id_base, c.nq, c.dim, c.scale, c.targets, lse, loss, rest, mean, weights,

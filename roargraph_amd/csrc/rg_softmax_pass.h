@@ -16,9 +16,10 @@
 // M is a reference, not the running maximum: it moves only when a weight would pass 2^15 (a branch no wave takes on most tiles), so sums
 // are rescaled a few times per pass instead of once per tile.
 //
-// LDS: a row of a plane is KS * 64 bytes in 16-byte chunks, pitch a multiple of 256 bytes, chunk c of row y at slot
-// c ^ (2 (y % 8) + y / 8 % 2) within its 256 bytes: 16 rows read at one chunk (first product) and 8 rows read 32 bytes wide (second)
-// both touch every bank once.
+// LDS: a row of a plane is KS * 64 bytes in 16-byte chunks, pitch a multiple of 256 bytes, chunk c of row y at slot c ^ swizzle(y) within its 256
+// bytes.  The second product's reads touch 8 rows 32 bytes wide: those need distinct pairs of slots.  The first product's touch 16 rows at one
+// chunk and are served 16 lanes at a time as lanes 0-3, 12-15, 20-23, 24-27 (and so on), that is rows 0-3, 12-15 at chunk c and rows 4-11 at
+// chunk c + 1: rows r and r ^ 12 share a pair.  (With 2 (y % 8) + y / 8 instead every such read took twice its time: 34 % of the LDS cycles.)
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -42,7 +43,7 @@ struct PassArgs {
     const uint32_t *targets;           // kStats, kMean: per x (global ids)
     uint32_t id_base;
     float *own2;                       // kStats, kMean: z2 of the target, written where it is met
-    const float4 *yinfo;               // fp32 rows and kRows, per y (padded to 32): factor and bias of a logit, sign of the weight, target row (bits)
+    const float *yinfo;                // fp32 rows and kRows, per 32 rows y: 32 factors and biases of a logit, signs of the weight, target rows (bits)
     const float *ytarget;              // kRows, per y: the biased logit of its own row, log2(|w| (1 - p_target)) (+ the exponent of the row)
     void *out;                         // kRows in one piece: the gradient itself
     uint64_t ostride;
@@ -80,6 +81,8 @@ template <> struct Frag<RG_DTYPE_BF16> { typedef bf8 V; };
 
 __device__ __forceinline__ f32x4 mma(half8 a, half8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 mma(bf8 a, bf8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ uint32_t swizzle(uint32_t y) { return (((y & 7) ^ (y >> 1 & 4)) << 1) | (y >> 3 & 1); }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 

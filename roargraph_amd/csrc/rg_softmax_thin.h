@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
         float *yv = reinterpret_cast<float *>(lds + C::NBUF * C::BUF) + buf * C::TY * 2;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint32_t r = lr + 16 * h, sw = ((r & 7) << 1) | ((r >> 3) & 1);
+            const uint32_t r = lr + 16 * h, sw = swizzle(r);
             int e = 0;
             float top = 0.0f;
             if constexpr (F32) {
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
 #pragma unroll
             for (int j = 0; j < NX; ++j) S[h][j] = f32x4{0, 0, 0, 0};
         {
-            const uint32_t sw = ((n & 7) << 1) | (n >> 3);      // (row + 16: the same swizzle)
+            const uint32_t sw = swizzle(n);                     // (row + 16: the same swizzle)
             const char *row = tile + n * PITCH;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
         if constexpr (MODE != kStats) {
             // lane (n, g) reads 8 bytes of row 4 g + n / 4 (and + 16) at dims 4 (n % 4) of the block, and receives dim n of rows 4 g .. + 3
             typedef __attribute__((address_space(3))) s16x4 *tr_ptr;
-            const uint32_t r = 4 * g + (n >> 2), sw = ((r & 7) << 1) | ((r >> 3) & 1);     // (row + 16: the same swizzle)
+            const uint32_t r = 4 * g + (n >> 2), sw = swizzle(r);     // (row + 16: the same swizzle)
             const char *row = tile + r * PITCH + (n & 1) * 8;
 #pragma unroll
             for (int ob = 0; ob < OB; ++ob) {

@@ -94,7 +94,7 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
     const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
     auto offset = [&](int i, uint32_t rows) {
         const uint32_t q = i * C::NT + tid, r = q / SR, slot = q % SR;
-        const uint32_t c = (slot & ~15u) | ((slot & 15) ^ (((r & 7) << 1) | (r >> 3 & 1)));
+        const uint32_t c = (slot & ~15u) | ((slot & 15) ^ swizzle(r));
         return c < nchunks ? min(r, rows - 1) * ystep + c * 16 : c < 4 * KS ? 0xffffffffu : min(r, rows - 1) * ystep;
     };
     uint32_t off[PER];
@@ -116,8 +116,8 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
                 const uint32_t o = rows < 32 ? offset(i, rows) : off[i];
                 if (!holes || o != 0xffffffffu) load_lds16(first + p * (KS * 64), o, to + (p * PER + i) * (16 * C::NT));
             }
-        constexpr uint32_t each = 32 / C::WAVES;
-        if (INFO && lane < each) load_lds16(A.yinfo + y0 + wave * each, lane * 16, __builtin_amdgcn_readfirstlane(ring + NBUF * C::BUF + buf * 512 + wave * each * 16));
+        constexpr uint32_t each = 32 / C::WAVES;    // lanes of a wave that load the tile's 512 bytes of info
+        if (INFO && lane < each) load_lds16(A.yinfo + (size_t)y0 * 4 + wave * each * 4, lane * 16, __builtin_amdgcn_readfirstlane(ring + NBUF * C::BUF + buf * 512 + wave * each * 16));
     };
     // tile t has landed, for all waves; `newer` tiles may still be on their way (loads land in the order they were issued; near the end,
     // where fewer are, all are waited for)
@@ -163,14 +163,18 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
     // LDS operands are asked for AHEAD steps before the products that take them, and the compiler is kept from moving the reads back
     // (vector and scalar instructions may still move between the products)
     auto keep_order = [] { __builtin_amdgcn_sched_barrier(0x6); };
+    const uint32_t sw = swizzle(n);
+    uint32_t first_at[4], second_at[8];             // what a lane reads of a tile: chunks 4 ks + g, and dims 4 (n % 4) of rows 4 g + n / 4 (they repeat every 256 bytes)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) first_at[i] = n * PITCH + (((4 * i + g) ^ sw) << 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) second_at[i] = (4 * g + (n >> 2)) * PITCH + (((2 * i + (n >> 1 & 1)) ^ swizzle(4 * g + (n >> 2))) << 4) + (n & 1) * 8;
     auto first_product = [&](uint32_t buf, f32x4 (&S)[NX][2]) {
         constexpr int AHEAD = C::WPS == 1 ? 2 : 1;
-        const char *row = lds + buf * C::BUF + n * PITCH;
-        const uint32_t sw = ((n & 7) << 1) | (n >> 3);
+        const char *tile = lds + buf * C::BUF;
         V a[AHEAD + 1][2][NP];
         auto read = [&](int ks) {
-            const uint32_t c = 4 * ks + g;
-            const char *at = row + (c & ~15u) * 16 + (((c & 15) ^ sw) << 4);
+            const char *at = tile + first_at[ks % 4] + ks / 4 * 256;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -206,12 +210,10 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
         if constexpr (MODE != kStats) {
             typedef __attribute__((address_space(3))) s16x4 *tr_ptr;
             constexpr int AHEAD = C::WPS == 1 && !F32 ? 3 : 2;
-            const uint32_t r = 4 * g + (n >> 2), sw = ((r & 7) << 1) | ((r >> 3) & 1);
-            const char *row = lds + buf * C::BUF + r * PITCH + (n & 1) * 8;
+            const char *tile = lds + buf * C::BUF + slice * (OB / 8 * 256);         // (more than one slice: OB is a multiple of 8)
             s16x4 a[AHEAD + 1][NP][2];
             auto read = [&](int ob) {
-                const uint32_t c = 2 * (slice * OB + ob) + ((n >> 1) & 1);
-                const char *at = row + (c & ~15u) * 16 + (((c & 15) ^ sw) << 4);
+                const char *at = tile + second_at[ob % 8] + ob / 8 * 256;
 #pragma unroll
                 for (int p = 0; p < NP; ++p)
 #pragma unroll
@@ -244,7 +246,9 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
         uint32_t y0, slot;          // first row; where its info lies
         bool rare, neg;             // a target of these rows, or rows behind the last, lie in the tile; a weight is negative
     };
-    auto info = [&](const Tile &t, uint32_t r) { return *reinterpret_cast<const f32x4 *>(lds + NBUF * C::BUF + t.slot * 512 + r * 16); };
+    enum { kFactor, kBias, kSign, kTarget };
+    auto info = [&](const Tile &t, int what, uint32_t r) { return *reinterpret_cast<const float *>(lds + NBUF * C::BUF + t.slot * 512 + what * 128 + r * 4); };
+    auto info4 = [&](const Tile &t, int what, int h) { return *reinterpret_cast<const f32x4 *>(lds + NBUF * C::BUF + t.slot * 512 + what * 128 + (16 * h + 4 * g) * 4); };
     auto look = [&](uint32_t t) {
         Tile k{ybeg + 32 * t, t % NBUF, false, false};
         bool met = false;
@@ -252,9 +256,8 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
 #pragma unroll
             for (int j = 0; j < NX; ++j) met |= target[j] - k.y0 < 32;
         } else {
-            const f32x4 v = info(k, lane & 31);
-            met = __float_as_uint(v[3]) - x0 < 16 * NX;
-            k.neg = __any(v[2] < 0.0f);
+            met = __float_as_uint(info(k, kTarget, lane & 31)) - x0 < 16 * NX;
+            k.neg = __any(info(k, kSign, lane & 31) < 0.0f);
         }
         k.rare = __any(met) || k.y0 + 32 > yend;
         return k;
@@ -272,16 +275,15 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t r = 16 * h + 4 * g + i;
-                    f32x4 v{1.0f, 0.0f, 1.0f, 0.0f};
-                    if (INFO) v = info(k, r);
-                    const float f = kx[j] * v[0];
+                    const float f = INFO ? kx[j] * info(k, kFactor, r) : kx[j];
                     bool dead = k.y0 + r >= yend;
                     if (MODE != kRows && k.y0 + r == target[j]) {
-                        if (slice == 0) A.own2[x] = S[j][h][i] * v[0] * kx[j];
+                        if (slice == 0) A.own2[x] = S[j][h][i] * f;
                         dead = true;
                     }
-                    if (MODE == kRows && __float_as_uint(v[3]) == x) {
-                        if (v[1] > -INFINITY) S[j][h][i] = (A.ytarget[k.y0 + r] - v[1]) / f;
+                    if (MODE == kRows && __float_as_uint(info(k, kTarget, r)) == x) {
+                        const float bias = info(k, kBias, r);
+                        if (bias > -INFINITY) S[j][h][i] = (A.ytarget[k.y0 + r] - bias) / f;
                         flip[j] |= 1u << (4 * h + i);
                     }
                     if (dead) S[j][h][i] = copysignf(INFINITY, -f);
@@ -290,14 +292,15 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
     };
     auto logits = [&](const Tile &k, const f32x4 (&S)[NX][2], bool biased, const float (&ref)[NX], float (&p)[NX][2][4]) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
+            f32x4 factor{1.0f, 1.0f, 1.0f, 1.0f}, bias{0.0f, 0.0f, 0.0f, 0.0f};
+            if (F32) factor = info4(k, kFactor, h);
+            if (BIAS) bias = info4(k, kBias, h);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                f32x4 v{1.0f, 0.0f, 0.0f, 0.0f};
-                if (INFO) v = info(k, 16 * h + 4 * g + i);
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < NX; ++j) p[j][h][i] = fmaf(F32 ? S[j][h][i] * v[0] : S[j][h][i], kx[j], biased ? v[1] - ref[j] : -ref[j]);
-            }
+                for (int j = 0; j < NX; ++j) p[j][h][i] = fmaf(F32 ? S[j][h][i] * factor[i] : S[j][h][i], kx[j], biased ? bias[i] - ref[j] : -ref[j]);
+        }
     };
     auto over = [&](const float (&p)[NX][2][4]) {
         float top = kNothing;
@@ -360,7 +363,7 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
     auto signs = [&](const Tile &k, V (&W)[NX][NP]) {           // rare, kRows
         uint32_t minus[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) minus[e / 2] |= (__float_as_uint(info(k, 16 * (e / 4) + 4 * g + e % 4)[2]) & 0x80000000u) >> (e % 2 ? 0 : 16);
+        for (int e = 0; e < 8; ++e) minus[e / 2] |= (__float_as_uint(info(k, kSign, 16 * (e / 4) + 4 * g + e % 4)) & 0x80000000u) >> (e % 2 ? 0 : 16);
 #pragma unroll
         for (int j = 0; j < NX; ++j) {
             const uint32_t f = k.rare ? flip[j] : 0;
