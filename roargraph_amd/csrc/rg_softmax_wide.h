@@ -30,8 +30,8 @@ constexpr WideChoice softmax_wide_cfg(int dt, int ks, int mode) {
         if (f32) return ks <= 4 ? WideChoice{3, 8, 2, false} : ks <= 7 ? WideChoice{2, 8, 2, false} : ks <= 16 ? WideChoice{1, 8, 2, false} : WideChoice{1, 4, 1, false};
         return ks <= 7 ? WideChoice{4, 8, 2, false} : ks <= 8 ? WideChoice{3, 8, 2, false} : ks <= 16 ? WideChoice{2, 8, 2, false} : WideChoice{1, 8, 2, false};
     }
-    if (f32) return ks <= 4 ? WideChoice{2, 8, 2, false} : ks <= 8 ? WideChoice{1, 8, 2, false} : ks <= 12 ? WideChoice{2, 4, 1, false} : WideChoice{1, 4, 1, false};
-    return ks <= 4 ? WideChoice{3, 8, 2, false} : ks <= 7 ? WideChoice{2, 8, 2, false} : ks <= 16 ? WideChoice{1, 8, 2, false} : WideChoice{1, 4, 1, false};
+    if (f32) return ks <= 4 ? WideChoice{2, 8, 2, false} : ks <= 8 ? WideChoice{1, 8, 2, false} : WideChoice{1, 4, 1, false};
+    return ks <= 2 ? WideChoice{4, 8, 2, false} : ks <= 4 ? WideChoice{3, 8, 2, false} : ks <= 7 || (ks == 8 && mode == kMean) ? WideChoice{2, 8, 2, false} : ks <= 16 ? WideChoice{1, 8, 2, false} : WideChoice{1, 4, 1, false};
 #endif
 }
 
@@ -163,22 +163,29 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
     // LDS operands are asked for AHEAD steps before the products that take them, and the compiler is kept from moving the reads back
     // (vector and scalar instructions may still move between the products)
     auto keep_order = [] { __builtin_amdgcn_sched_barrier(0x6); };
+    typedef __attribute__((address_space(3))) const V LdsV;
+    // an LDS address the compiler takes as it is: left to itself it splits these sums over the loop and folds no constant into the reads
+    auto lds_at = [](uint32_t a) {
+        asm("" : "+v"(a));
+        return a;
+    };
     const uint32_t sw = swizzle(n);
     uint32_t first_at[4], second_at[8];             // what a lane reads of a tile: chunks 4 ks + g, and dims 4 (n % 4) of rows 4 g + n / 4 (they repeat every 256 bytes)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) first_at[i] = n * PITCH + (((4 * i + g) ^ sw) << 4);
+    for (int i = 0; i < 4; ++i) first_at[i] = ring + n * PITCH + (((4 * i + g) ^ sw) << 4);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) second_at[i] = (4 * g + (n >> 2)) * PITCH + (((2 * i + (n >> 1 & 1)) ^ swizzle(4 * g + (n >> 2))) << 4) + (n & 1) * 8;
+    for (int i = 0; i < 8; ++i) second_at[i] = ring + (4 * g + (n >> 2)) * PITCH + (((2 * i + (n >> 1 & 1)) ^ swizzle(4 * g + (n >> 2))) << 4) + (n & 1) * 8;
     auto first_product = [&](uint32_t buf, f32x4 (&S)[NX][2]) {
         constexpr int AHEAD = C::WPS == 1 ? 2 : 1;
-        const char *tile = lds + buf * C::BUF;
+        uint32_t at[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) at[i] = lds_at(first_at[i] + buf * C::BUF);
         V a[AHEAD + 1][2][NP];
         auto read = [&](int ks) {
-            const char *at = tile + first_at[ks % 4] + ks / 4 * 256;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int p = 0; p < NP; ++p) a[ks % (AHEAD + 1)][h][p] = *reinterpret_cast<const V *>(at + h * 16 * PITCH + p * C::PLANE);
+                for (int p = 0; p < NP; ++p) a[ks % (AHEAD + 1)][h][p] = *(LdsV *)(at[ks % 4] + (uint32_t)(ks / 4 * 256 + h * 16 * PITCH + p * C::PLANE));
         };
 #pragma unroll
         for (int j = 0; j < NX; ++j) S[j][0] = S[j][1] = f32x4{0, 0, 0, 0};
@@ -210,14 +217,15 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
         if constexpr (MODE != kStats) {
             typedef __attribute__((address_space(3))) s16x4 *tr_ptr;
             constexpr int AHEAD = C::WPS == 1 && !F32 ? 3 : 2;
-            const char *tile = lds + buf * C::BUF + slice * (OB / 8 * 256);         // (more than one slice: OB is a multiple of 8)
+            uint32_t at[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) at[i] = lds_at(second_at[i] + buf * C::BUF + slice * (OB / 8 * 256));    // (more than one slice: OB is a multiple of 8)
             s16x4 a[AHEAD + 1][NP][2];
             auto read = [&](int ob) {
-                const char *at = tile + second_at[ob % 8] + ob / 8 * 256;
 #pragma unroll
                 for (int p = 0; p < NP; ++p)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) a[ob % (AHEAD + 1)][p][h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(const_cast<char *>(at) + p * C::PLANE + h * 16 * PITCH));
+                    for (int h = 0; h < 2; ++h) a[ob % (AHEAD + 1)][p][h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at[ob % 8] + (uint32_t)(ob / 8 * 256 + p * C::PLANE + h * 16 * PITCH)));
             };
 #pragma unroll
             for (int ob = 0; ob < AHEAD && ob < OB; ++ob) read(ob);
