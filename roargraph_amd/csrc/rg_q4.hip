@@ -64,24 +64,254 @@ __global__ void __launch_bounds__(256) rg_q4_unpack_kernel(const uint8_t *codes,
     }
 }
 
-// one wave per row and query
-template <int DT>
-__global__ void __launch_bounds__(256) rg_q4_score_kernel(const uint8_t *codes, uint64_t cstride, const uint16_t *scales, const uint16_t *mins, uint64_t sstride, uint32_t nb, uint32_t dim,
-                                                          uint32_t group, const void *queries, uint32_t nq, uint64_t qstride, float *out, uint64_t ostride) {
+// ---------------------------------------------------------------- scores
+//
+// Bound by reading the codes; the arithmetic has to stay out of the way.  Rows are the A operand of v_mfma_f32_16x16x32_f16 (16 rows x 32
+// elements), queries its B operand: column n < 8 holds the upper half of query n, column n + 8 the lower (x = 2^e (hi + lo), 22 bits relative
+// to the query's largest element), so eight fp32 queries cost what one costs.
+//
+//   a code becomes s (c - 8) in fp16 exactly, as two halves: s has 11 bits and c - 8 four, hi = fl(s (c - 8)), lo = s (c - 8) - hi, and no multiple
+//   of 2^-24 is lost; products and sums are the matrix core's, in fp32, over the whole row -- no scale is applied to partial sums
+//   minima: s c + m = s (c - 8) + (m + 8 s), and sum_k (m + 8 s) x_k over 32 elements is one slot of one more product per 128 elements
+//
+// A wave takes 32 rows at a time; lane (n, g) reads 16 bytes = 32 codes of row n, chunk 4 j + g of the row, with their scale.  (A row's last chunk is
+// moved back to end with the row; what the chunk before it holds already meets zeros in the query.)  DEPTH such steps are on their way
+// while one is multiplied.  The dword's codes come out in the order 0 4 1 5 2 6 3 7, and the queries lie in LDS in that order.
+typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+struct ScoreArgs {
+    const uint8_t *codes;
+    const uint16_t *scales, *mins;
+    const void *queries;
+    float *out;
+    uint64_t cstride, sstride, qstride, ostride;
+    uint32_t nb, nq, dim, chunks_per_group, groups;     // chunks of 32 elements
+};
+
+constexpr int kScoreThreads = 512, kScoreRows = 32, kScoreDepth = 4;
+
+__device__ __forceinline__ void dequant(uint32_t w, half2 s, half8 &hi, half8 &lo) {
+    const uint32_t w8 = w >> 8;
+    const half2 c8 = {-1032.0f, -1032.0f}, sixteenth = {0.0625f, 0.0625f}, c72 = {-72.0f, -72.0f};
+    half2 v[4];
+    v[0] = __builtin_bit_cast(half2, (w & 0x000f000fu) | 0x64006400u) + c8;                                          // 1024 + c
+    v[1] = __builtin_elementwise_fma(__builtin_bit_cast(half2, (w & 0x00f000f0u) | 0x64006400u), sixteenth, c72);     // 1024 + 16 c
+    v[2] = __builtin_bit_cast(half2, (w8 & 0x000f000fu) | 0x64006400u) + c8;
+    v[3] = __builtin_elementwise_fma(__builtin_bit_cast(half2, (w8 & 0x00f000f0u) | 0x64006400u), sixteenth, c72);
+    half2 h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        h[i] = v[i] * s;
+        l[i] = __builtin_elementwise_fma(v[i], s, -h[i]);
+    }
+    hi = __builtin_bit_cast(half8, h);
+    lo = __builtin_bit_cast(half8, l);
+}
+
+// element i of the B operand's eight holds element order(i) of the dword
+__device__ __forceinline__ constexpr int code_order(int i) { return i % 2 * 4 + i / 2; }
+
+// NQB blocks of eight queries at a time
+template <int DT, int NQB, bool MINS>
+__global__ void __launch_bounds__(kScoreThreads) rg_q4_score_kernel(ScoreArgs A) {
     typedef typename Elem<DT>::T T;
-    const uint32_t lane = threadIdx.x % 64;
-    for (uint64_t j = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64; j < nb; j += (uint64_t)gridDim.x * 4)
-        for (uint32_t i = 0; i < nq; ++i) {
-            float acc = 0.0f;
-            for (uint32_t k = lane; k < dim; k += 64) {
-                const uint32_t c = codes[j * cstride + k / 2] >> (4 * (k & 1)) & 15u, g = k / group;
-                const float s = half_bits(scales[j * sstride + g]);
-                const float v = mins ? (float)c * s + half_bits(mins[j * sstride + g]) : (float)((int)c - 8) * s;
-                acc = fmaf(v, (float)static_cast<const T *>(queries)[(size_t)i * qstride + k], acc);
+    extern __shared__ char lds[];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
+    const uint32_t dim = A.dim, D = (dim + 7) / 8, chunks = (D + 3) / 4, steps = (chunks + 3) / 4;       // dwords, chunks, steps of four chunks of a row
+    half8 *X = reinterpret_cast<half8 *>(lds);                                        // [block][step][t][lane]
+    uint32_t *XG = reinterpret_cast<uint32_t *>(lds + (size_t)NQB * steps * 4096);    // [block][step][lane]: the chunk's sum, twice
+    float *factor = reinterpret_cast<float *>(XG + (MINS ? NQB * steps * 64 : 0));    // [query]
+
+    struct Stage {
+        u32x4 c[2];
+        uint32_t s[2], m[2];
+    };
+    Stage ring[kScoreDepth];
+    const uint32_t waves = kScoreThreads / 64, tiles = (A.nb + kScoreRows - 1) / kScoreRows;
+    const uint32_t stride = gridDim.x * waves, first = wave * gridDim.x + blockIdx.x;
+    const uint32_t mine = first < tiles ? (tiles - first - 1) / stride + 1 : 0;
+    const uint64_t total = (uint64_t)mine * steps;
+    uint32_t ptile = first, pstep = 0;                                                // what is fetched next
+    uint64_t asked = 0;
+    auto fetch = [&](Stage &st) {
+        if (asked++ >= total) return;
+        const uint32_t q = 4 * pstep + g, group = min(q / A.chunks_per_group, A.groups - 1);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const uint64_t row = min(ptile * kScoreRows + 16 * r + n, A.nb - 1);
+            const uint32_t *at = reinterpret_cast<const uint32_t *>(A.codes + row * A.cstride);
+            if (D >= 4) {
+                typedef u32x4 u32x4_dw __attribute__((aligned(4)));
+                st.c[r] = *reinterpret_cast<const u32x4_dw *>(at + min(4 * q, D - 4));
+            } else {
+#pragma unroll
+                for (int t = 0; t < 4; ++t) st.c[r][t] = at[min((uint32_t)t, D - 1)];
             }
-            for (int d = 1; d < 64; d <<= 1) acc += __shfl_xor(acc, d);
-            if (lane == 0) out[(size_t)i * ostride + j] = acc;
+            st.s[r] = A.scales[row * A.sstride + group];
+            if (MINS) st.m[r] = A.mins[row * A.sstride + group];
         }
+        if (++pstep == steps) {
+            pstep = 0;
+            ptile += stride;
+        }
+    };
+#pragma unroll
+    for (int d = 0; d < kScoreDepth; ++d) fetch(ring[d]);
+
+    for (uint32_t q0 = 0; q0 < A.nq; q0 += 8 * NQB) {
+        // queries: the largest element of each, then halves in operand order (zeros behind dim and behind the last query)
+        for (uint32_t q = wave; q < 8 * NQB; q += waves) {
+            uint32_t m = 0;
+            if (q0 + q < A.nq)
+                for (uint32_t k = lane; k < dim; k += 64) m = max(m, __float_as_uint((float)static_cast<const T *>(A.queries)[(size_t)(q0 + q) * A.qstride + k]) & 0x7fffffffu);
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
+            if (lane == 0) factor[q] = __uint_as_float(m);
+        }
+        __syncthreads();
+        auto element = [&](uint32_t q, uint32_t k, float top, float down) {      // a query's element, scaled; of one that is not finite the signs of its infinities
+            if (q0 + q >= A.nq || k >= dim) return 0.0f;
+            const float v = (float)static_cast<const T *>(A.queries)[(size_t)(q0 + q) * A.qstride + k];
+            if (top < INFINITY) return v * down;
+            return fabsf(v) < INFINITY ? 0.0f : fabsf(v) == INFINITY ? copysignf(1.0f, v) : v;
+        };
+        for (uint32_t i = tid; i < NQB * steps * 4 * 4 * 8; i += kScoreThreads) {
+            const uint32_t q = i % 8, gg = i / 8 % 4, t = i / 32 % 4, j = i / 128 % steps, qb = i / 128 / steps;
+            const float top = factor[qb * 8 + q], down = pow2(-row_exponent(top));
+            const uint32_t c = 4 * j + gg, d = D >= 4 ? min(4 * c, D - 4) + t : t;
+            half8 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float v = d >= 4 * c && d < D ? element(qb * 8 + q, 8 * d + code_order(e), top, down) : 0.0f;
+                hi[e] = (_Float16)v;
+                lo[e] = (_Float16)(v - (float)hi[e]);
+            }
+            half8 *at = X + ((size_t)(qb * steps + j) * 4 + t) * 64 + gg * 16 + q;
+            at[0] = hi;
+            at[8] = lo;
+        }
+        if (MINS)
+            for (uint32_t i = tid; i < NQB * steps * 4 * 8; i += kScoreThreads) {
+                const uint32_t q = i % 8, gg = i / 8 % 4, j = i / 32 % steps, qb = i / 32 / steps;
+                const float top = factor[qb * 8 + q], down = pow2(-row_exponent(top));
+                float v = 0.0f;
+                for (uint32_t k = 32 * (4 * j + gg); k < min(32 * (4 * j + gg) + 32, dim); ++k) v += element(qb * 8 + q, k, top, down);
+                const _Float16 h = (_Float16)v, l = (_Float16)(v - (float)h);
+                uint32_t *at = XG + (qb * steps + j) * 64 + gg * 16 + q;
+                at[0] = 0x10001u * __builtin_bit_cast(uint16_t, h);
+                at[8] = 0x10001u * __builtin_bit_cast(uint16_t, l);
+            }
+        __syncthreads();
+
+        if (q0) {                                    // the base once more for the next queries
+            ptile = first;
+            pstep = 0;
+            asked = 0;
+#pragma unroll
+            for (int d = 0; d < kScoreDepth; ++d) fetch(ring[d]);
+        }
+        f32x4 acc[2][NQB];
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int b = 0; b < NQB; ++b) acc[r][b] = f32x4{0, 0, 0, 0};
+        uint32_t tile = first, step = 0;
+        for (uint64_t it = 0; it < total; it += kScoreDepth) {
+#pragma unroll
+            for (int d = 0; d < kScoreDepth; ++d) {
+                if (it + d >= total) break;
+                const Stage st = ring[d];
+                fetch(ring[d]);
+                half2 s[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) s[r] = __builtin_bit_cast(half2, st.s[r] * 0x10001u);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    half8 x[NQB];
+#pragma unroll
+                    for (int b = 0; b < NQB; ++b) x[b] = X[((size_t)(b * steps + step) * 4 + t) * 64 + lane];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        half8 hi, lo;
+                        dequant(st.c[r][t], s[r], hi, lo);
+#pragma unroll
+                        for (int b = 0; b < NQB; ++b) {
+                            acc[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, x[b], acc[r][b], 0, 0, 0);
+                            acc[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, x[b], acc[r][b], 0, 0, 0);
+                        }
+                    }
+                }
+                if (MINS) {
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float off = fmaf(half_bits((uint16_t)st.s[r]), 8.0f, half_bits((uint16_t)st.m[r]));
+                        half8 o = {0, 0, 0, 0, 0, 0, 0, 0};
+                        o[0] = (_Float16)off;
+                        o[1] = (_Float16)(off - (float)o[0]);
+#pragma unroll
+                        for (int b = 0; b < NQB; ++b) {
+                            const u32x4 v = {XG[(b * steps + step) * 64 + lane], 0, 0, 0};
+                            acc[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(o, __builtin_bit_cast(half8, v), acc[r][b], 0, 0, 0);
+                        }
+                    }
+                }
+                if (++step == steps) {
+                    step = 0;
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+#pragma unroll
+                        for (int b = 0; b < NQB; ++b) {
+                            f32x4 v = acc[r][b];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[i] += __shfl_xor(v[i], 8);
+                            const uint32_t q = q0 + b * 8 + n, row = tile * kScoreRows + 16 * r + 4 * g;
+                            if (n < 8 && q < A.nq && row < A.nb) {
+                                const float top = factor[b * 8 + n], up = row_factor(top, row_exponent(top));
+                                float *to = A.out + q * A.ostride + row;
+                                if (row + 4 <= A.nb) {
+                                    typedef f32x4 f32x4_dw __attribute__((aligned(4)));
+                                    *reinterpret_cast<f32x4_dw *>(to) = v * up;
+                                } else {
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i)
+                                        if (row + i < A.nb) to[i] = v[i] * up;
+                                }
+                            }
+                            acc[r][b] = f32x4{0, 0, 0, 0};
+                        }
+                    tile += stride;
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+size_t score_lds(uint32_t dim, int nqb, bool mins) {
+    const size_t steps = (((dim + 7) / 8 + 3) / 4 + 3) / 4;
+    return nqb * steps * (4096 + (mins ? 256 : 0)) + nqb * 32;
+}
+
+template <int DT, int NQB>
+rg_status launch_score(const ScoreArgs &A, hipStream_t s) {
+    auto kern = A.mins ? rg_q4_score_kernel<DT, NQB, true> : rg_q4_score_kernel<DT, NQB, false>;
+    const size_t lds = score_lds(A.dim, NQB, A.mins != nullptr);
+    RG_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    const uint32_t tiles = (A.nb + kScoreRows - 1) / kScoreRows, per_cu = std::max<uint32_t>(1, std::min<uint32_t>(2, (uint32_t)(160 * 1024 / lds)));
+    hipLaunchKernelGGL(kern, dim3(std::min(tiles, 256u * per_cu)), dim3(kScoreThreads), lds, s, A);
+    RG_HIP(hipGetLastError());
+    return RG_OK;
+}
+template <int DT>
+rg_status launch_score_dt(const ScoreArgs &A, hipStream_t s) {
+    // as many queries per reading of the base as there are, and as LDS holds
+    const bool mins = A.mins != nullptr;
+    if (A.nq > 16 && score_lds(A.dim, 4, mins) <= 160 * 1024) return launch_score<DT, 4>(A, s);
+    if (A.nq > 8 && score_lds(A.dim, 2, mins) <= 160 * 1024) return launch_score<DT, 2>(A, s);
+    return launch_score<DT, 1>(A, s);
 }
 
 rg_status check_form(const void *codes, uint64_t cstride, const void *scales, const void *mins, uint64_t sstride, uint32_t nb, uint32_t dim, uint32_t group) {
@@ -150,11 +380,12 @@ rg_status rg_q4_score_dev(const uint8_t *d_codes, uint64_t cstride, const uint16
     if (ostride < nb || (uintptr_t)d_out % 4) return set_error(RG_ERR_ARG, "scores: stride smaller than the number of rows, or not aligned to their elements");
     OnDevice on(device);
     if (on.st != RG_OK) return on.st;
-    auto kern = dtype == RG_DTYPE_F32 ? rg_q4_score_kernel<RG_DTYPE_F32> : dtype == RG_DTYPE_F16 ? rg_q4_score_kernel<RG_DTYPE_F16> : rg_q4_score_kernel<RG_DTYPE_BF16>;
-    hipLaunchKernelGGL(kern, dim3(std::min<uint32_t>((nb + 3) / 4, 65536u)), dim3(256), 0, (hipStream_t)stream, d_codes, cstride, d_scales, d_mins, sstride, nb, dim, group, d_queries, nq, qstride,
-                       d_out, ostride);
-    RG_HIP(hipGetLastError());
-    return RG_OK;
+    ScoreArgs A;
+    A.codes = d_codes; A.scales = d_scales; A.mins = d_mins; A.queries = d_queries; A.out = d_out;
+    A.cstride = cstride; A.sstride = sstride; A.qstride = qstride; A.ostride = ostride;
+    A.nb = nb; A.nq = nq; A.dim = dim; A.chunks_per_group = group / 32; A.groups = (dim + group - 1) / group;
+    hipStream_t s = (hipStream_t)stream;
+    return dtype == RG_DTYPE_F32 ? launch_score_dt<RG_DTYPE_F32>(A, s) : dtype == RG_DTYPE_F16 ? launch_score_dt<RG_DTYPE_F16>(A, s) : launch_score_dt<RG_DTYPE_BF16>(A, s);
 }
 
 }  // extern "C"

@@ -24,6 +24,17 @@ template <> struct Elem<RG_DTYPE_BF16> { typedef __bf16 T; };
 inline bool known_dtype(int dtype) { return dtype == RG_DTYPE_F32 || dtype == RG_DTYPE_F16 || dtype == RG_DTYPE_BF16; }
 inline uint32_t elem_bytes(int dtype) { return dtype == RG_DTYPE_F32 ? 4 : 2; }
 
+// ---- fp32 rows as two fp16 halves, scaled by a power of two of their own
+// exponent e of a row's largest value: 2^-e brings the row to [1, 2)
+__device__ __forceinline__ int row_exponent(float top) {
+    const uint32_t u = __float_as_uint(top) >> 23;
+    return u >= 255 ? 0 : u ? (int)u - 127 : top == 0.0f ? 0 : -126;       // (subnormal rows: 2^126 is the largest factor)
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127
+
+// a row that is not finite keeps the signs of its infinities (and its NaN) and nothing else; its logits are multiplied by infinity
+__device__ __forceinline__ float row_factor(float top, int e) { return top < INFINITY ? pow2(e) : INFINITY; }
+
 // makes `device` current for a call, and the caller's device current again afterwards
 struct OnDevice {
     int before = -1;

@@ -129,16 +129,6 @@ __device__ __forceinline__ float absmax(const Chunk<RG_DTYPE_F32> &c) {
     for (int i = 0; i < 4; ++i) m = max(max(m, __float_as_uint(c.a[i]) & 0x7fffffffu), __float_as_uint(c.b[i]) & 0x7fffffffu);
     return __uint_as_float(m);
 }
-// exponent e of a row's largest value: 2^-e brings the row to [1, 2)
-__device__ __forceinline__ int row_exponent(float top) {
-    const uint32_t u = __float_as_uint(top) >> 23;
-    return u >= 255 ? 0 : u ? (int)u - 127 : top == 0.0f ? 0 : -126;       // (subnormal rows: 2^126 is the largest factor)
-}
-__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127
-
-// a row that is not finite keeps the signs of its infinities (and its NaN) and nothing else; its logits are multiplied by infinity
-__device__ __forceinline__ float row_factor(float top, int e) { return top < INFINITY ? pow2(e) : INFINITY; }
-
 __device__ __forceinline__ void split8(Chunk<RG_DTYPE_F32> c, float top, float s, half8 &hi, half8 &lo) {
     if (!(top < INFINITY)) {
 #pragma unroll
