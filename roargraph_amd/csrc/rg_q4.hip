@@ -88,7 +88,7 @@ struct ScoreArgs {
     const void *queries;
     float *out;
     uint64_t cstride, sstride, qstride, ostride;
-    uint32_t nb, nq, dim, chunks_per_group, groups;     // chunks of 32 elements
+    uint32_t nb, nq, dim, chunk_shift, groups;          // chunks of 32 elements, 2^chunk_shift to a group
 };
 
 constexpr int kScoreThreads = 512, kScoreRows = 32, kScoreDepth = 4;
@@ -133,29 +133,42 @@ __global__ void __launch_bounds__(kScoreThreads) rg_q4_score_kernel(ScoreArgs A)
     const uint32_t waves = kScoreThreads / 64, tiles = (A.nb + kScoreRows - 1) / kScoreRows;
     const uint32_t stride = gridDim.x * waves, first = wave * gridDim.x + blockIdx.x;
     const uint32_t mine = first < tiles ? (tiles - first - 1) / stride + 1 : 0;
-    const uint64_t total = (uint64_t)mine * steps;
-    uint32_t ptile = first, pstep = 0;                                                // what is fetched next
-    uint64_t asked = 0;
-    auto fetch = [&](Stage &st) {
-        if (asked++ >= total) return;
-        const uint32_t q = 4 * pstep + g, group = min(q / A.chunks_per_group, A.groups - 1);
+    const uint32_t total = mine * steps;             // (the host's rule: below 2^32)
+    // What is fetched next: a uniform address of the tile and 32-bit offsets of the lanes, so that a step's loads cost a few vector
+    // instructions.  In the last tile rows behind the last one are read as the last.
+    uint32_t ptile = first, pstep = 0, asked = 0;
+    uint32_t code_at[2], scale_at[2];
+    auto rows_of = [&](uint32_t tile) {
+        const uint32_t last = min((uint32_t)kScoreRows, A.nb - tile * kScoreRows) - 1;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const uint64_t row = min(ptile * kScoreRows + 16 * r + n, A.nb - 1);
-            const uint32_t *at = reinterpret_cast<const uint32_t *>(A.codes + row * A.cstride);
+            code_at[r] = min(16 * r + n, last) * (uint32_t)A.cstride;
+            scale_at[r] = min(16 * r + n, last) * (uint32_t)A.sstride * 2;
+        }
+    };
+    if (mine) rows_of(first);
+    auto fetch = [&](Stage &st) {
+        if (asked == total) return;
+        ++asked;
+        const char *codes = reinterpret_cast<const char *>(A.codes + (size_t)ptile * kScoreRows * A.cstride);
+        const char *scales = reinterpret_cast<const char *>(A.scales + (size_t)ptile * kScoreRows * A.sstride), *mins = reinterpret_cast<const char *>(A.mins + (size_t)ptile * kScoreRows * A.sstride);
+        const uint32_t q = 4 * pstep + g, group2 = min(q >> A.chunk_shift, A.groups - 1) * 2;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
             if (D >= 4) {
                 typedef u32x4 u32x4_dw __attribute__((aligned(4)));
-                st.c[r] = *reinterpret_cast<const u32x4_dw *>(at + min(4 * q, D - 4));
+                st.c[r] = *reinterpret_cast<const u32x4_dw *>(codes + (code_at[r] + min(16 * q, 4 * D - 16)));
             } else {
 #pragma unroll
-                for (int t = 0; t < 4; ++t) st.c[r][t] = at[min((uint32_t)t, D - 1)];
+                for (int t = 0; t < 4; ++t) st.c[r][t] = *reinterpret_cast<const uint32_t *>(codes + (code_at[r] + 4 * min((uint32_t)t, D - 1)));
             }
-            st.s[r] = A.scales[row * A.sstride + group];
-            if (MINS) st.m[r] = A.mins[row * A.sstride + group];
+            st.s[r] = *reinterpret_cast<const uint16_t *>(scales + (scale_at[r] + group2));
+            if (MINS) st.m[r] = *reinterpret_cast<const uint16_t *>(mins + (scale_at[r] + group2));
         }
         if (++pstep == steps) {
             pstep = 0;
             ptile += stride;
+            if (ptile == tiles - 1) rows_of(ptile);
         }
     };
 #pragma unroll
@@ -208,8 +221,8 @@ __global__ void __launch_bounds__(kScoreThreads) rg_q4_score_kernel(ScoreArgs A)
 
         if (q0) {                                    // the base once more for the next queries
             ptile = first;
-            pstep = 0;
-            asked = 0;
+            pstep = asked = 0;
+            if (mine) rows_of(first);
 #pragma unroll
             for (int d = 0; d < kScoreDepth; ++d) fetch(ring[d]);
         }
@@ -219,7 +232,7 @@ __global__ void __launch_bounds__(kScoreThreads) rg_q4_score_kernel(ScoreArgs A)
 #pragma unroll
             for (int b = 0; b < NQB; ++b) acc[r][b] = f32x4{0, 0, 0, 0};
         uint32_t tile = first, step = 0;
-        for (uint64_t it = 0; it < total; it += kScoreDepth) {
+        for (uint32_t it = 0; it < total; it += kScoreDepth) {
 #pragma unroll
             for (int d = 0; d < kScoreDepth; ++d) {
                 if (it + d >= total) break;
@@ -318,6 +331,7 @@ rg_status check_form(const void *codes, uint64_t cstride, const void *scales, co
     if (group != 32 && group != 64 && group != 128) return set_error(RG_ERR_ARG, "4-bit base: groups of 32, 64 or 128 elements");
     if (dim == 0 || dim > kMaxDim) return set_error(RG_ERR_ARG, "4-bit base: dim must be in [1, 4096]");
     if (nb > 0x7fffffffu) return set_error(RG_ERR_ARG, "4-bit base: at most 2^31 - 1 rows");
+    if (cstride > 1u << 26 || sstride > 1u << 25) return set_error(RG_ERR_ARG, "4-bit base: row strides of at most 64 MB");
     if (nb == 0) return RG_OK;
     if (!codes || !scales) return set_error(RG_ERR_ARG, "null argument");
     if (cstride % 4 || cstride < (uint64_t)aligned_dim(dim) / 2 || (uintptr_t)codes % 4) return set_error(RG_ERR_ARG, "4-bit base: code rows are 4-byte aligned and hold dim rounded up to 8 elements");
@@ -383,7 +397,7 @@ rg_status rg_q4_score_dev(const uint8_t *d_codes, uint64_t cstride, const uint16
     ScoreArgs A;
     A.codes = d_codes; A.scales = d_scales; A.mins = d_mins; A.queries = d_queries; A.out = d_out;
     A.cstride = cstride; A.sstride = sstride; A.qstride = qstride; A.ostride = ostride;
-    A.nb = nb; A.nq = nq; A.dim = dim; A.chunks_per_group = group / 32; A.groups = (dim + group - 1) / group;
+    A.nb = nb; A.nq = nq; A.dim = dim; A.chunk_shift = group == 32 ? 0 : group == 64 ? 1 : 2; A.groups = (dim + group - 1) / group;
     hipStream_t s = (hipStream_t)stream;
     return dtype == RG_DTYPE_F32 ? launch_score_dt<RG_DTYPE_F32>(A, s) : dtype == RG_DTYPE_F16 ? launch_score_dt<RG_DTYPE_F16>(A, s) : launch_score_dt<RG_DTYPE_BF16>(A, s);
 }
