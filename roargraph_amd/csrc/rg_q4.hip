@@ -66,21 +66,26 @@ __global__ void __launch_bounds__(256) rg_q4_unpack_kernel(const uint8_t *codes,
 
 // ---------------------------------------------------------------- scores
 //
-// Bound by reading the codes; the arithmetic has to stay out of the way.  Rows are the A operand of v_mfma_f32_16x16x32_f16 (16 rows x 32
-// elements), queries its B operand: column n < 8 holds the upper half of query n, column n + 8 the lower (x = 2^e (hi + lo), 22 bits relative
-// to the query's largest element), so eight fp32 queries cost what one costs.
+// Bound by reading the codes; the arithmetic has to stay out of the way.  v_mfma_f32_16x16x32_f16 with queries as the A operand -- rows 2 q and
+// 2 q + 1 are the halves of query q, x = 2^e (hi + lo), 22 bits relative to its largest element, so that eight fp32 queries cost what one
+// costs -- and 16 rows of the base as the B operand.
 //
-//   a code becomes s (c - 8) in fp16 exactly, as two halves: s has 11 bits and c - 8 four, hi = fl(s (c - 8)), lo = s (c - 8) - hi, and no multiple
-//   of 2^-24 is lost; products and sums are the matrix core's, in fp32, over the whole row -- no scale is applied to partial sums
-//   minima: s c + m = s (c - 8) + (m + 8 s), and sum_k (m + 8 s) x_k over 32 elements is one slot of one more product per 128 elements
+//   a code needs no conversion: its four bits where they lie in the dword are an fp16 subnormal, c 2^-24 (or 16 c 2^-24), which the matrix core
+//   takes exactly; the queries' elements carry the factors.  Five instructions make eight operands of a dword.
+//   the partial sum of a group starts at -8 times the queries' sum over it, so that it is that of c - 8, and is then multiplied by the
+//   row's scale in fp32: lane (n, g) holds it for row n and queries 2 g, 2 g + 1
+//   minima: s c + m = s (c - 8) + (m + 8 s), and the queries' sum is at hand
 //
-// A wave takes 32 rows at a time; lane (n, g) reads 16 bytes = 32 codes of row n, chunk 4 j + g of the row, with their scale.  (A row's last chunk is
-// moved back to end with the row; what the chunk before it holds already meets zeros in the query.)  DEPTH such steps are on their way
-// while one is multiplied.  The dword's codes come out in the order 0 4 1 5 2 6 3 7, and the queries lie in LDS in that order.
-typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+// A wave takes 32 rows at a time; lane (n, g) reads 16 bytes = 32 codes of row n, chunk 4 j + g of the row.  (A row's last chunk is moved back
+// to end with the row; what the chunk before it holds already meets zeros in the query.)  One product must see one group only: for
+// groups of 128 the chunks of a step are that, for 32 and 64 the dwords change lanes first (permlane swaps).  kScoreDepth steps are
+// on their way while one is multiplied.  A dword's codes come out in the order 0 4 1 5 2 6 3 7, and the queries lie in LDS in that order.
+//
+// (A first form made s (c - 8) of every code, exactly, as a pair of halves: 21 vector instructions a dword, 72 % of the vector units' time and 3.3 TB/s.)
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
 
 struct ScoreArgs {
     const uint8_t *codes;
@@ -88,46 +93,71 @@ struct ScoreArgs {
     const void *queries;
     float *out;
     uint64_t cstride, sstride, qstride, ostride;
-    uint32_t nb, nq, dim, chunk_shift, groups;          // chunks of 32 elements, 2^chunk_shift to a group
+    uint32_t nb, nq, dim, groups;
+    int dtype;
 };
 
 constexpr int kScoreThreads = 512, kScoreRows = 32, kScoreDepth = 4;
 
-__device__ __forceinline__ void dequant(uint32_t w, half2 s, half8 &hi, half8 &lo) {
-    const uint32_t w8 = w >> 8;
-    const half2 c8 = {-1032.0f, -1032.0f}, sixteenth = {0.0625f, 0.0625f}, c72 = {-72.0f, -72.0f};
-    half2 v[4];
-    v[0] = __builtin_bit_cast(half2, (w & 0x000f000fu) | 0x64006400u) + c8;                                          // 1024 + c
-    v[1] = __builtin_elementwise_fma(__builtin_bit_cast(half2, (w & 0x00f000f0u) | 0x64006400u), sixteenth, c72);     // 1024 + 16 c
-    v[2] = __builtin_bit_cast(half2, (w8 & 0x000f000fu) | 0x64006400u) + c8;
-    v[3] = __builtin_elementwise_fma(__builtin_bit_cast(half2, (w8 & 0x00f000f0u) | 0x64006400u), sixteenth, c72);
-    half2 h[4], l[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        h[i] = v[i] * s;
-        l[i] = __builtin_elementwise_fma(v[i], s, -h[i]);
+// where product u of a step finds its dword in lane group g: (lane group it was read by, dword of the 16 bytes)
+template <int GS> __device__ __forceinline__ constexpr uint32_t from_group(uint32_t u, uint32_t g) { return GS == 0 ? u : GS == 1 ? (u & 1) * 2 + (g & 1) : g; }
+template <int GS> __device__ __forceinline__ constexpr uint32_t from_dword(uint32_t u, uint32_t g) { return GS == 0 ? g : GS == 1 ? (u & 2) + (g >> 1) : u; }
+template <int GS>
+__device__ __forceinline__ void exchange(u32x4 &c) {
+    if constexpr (GS < 2) {
+        auto p = __builtin_amdgcn_permlane32_swap(c[0], c[1], false, false), q = __builtin_amdgcn_permlane32_swap(c[2], c[3], false, false);
+        if constexpr (GS == 1) {
+            c = u32x4{p[0], p[1], q[0], q[1]};
+        } else {                                     // lane groups (0 1 | 2 3) -> a 4 x 4 transpose
+            p = __builtin_amdgcn_permlane32_swap(c[0], c[2], false, false);
+            q = __builtin_amdgcn_permlane32_swap(c[1], c[3], false, false);
+            const auto a = __builtin_amdgcn_permlane16_swap(p[0], q[0], false, false), b = __builtin_amdgcn_permlane16_swap(p[1], q[1], false, false);
+            c = u32x4{a[0], a[1], b[0], b[1]};
+        }
     }
-    hi = __builtin_bit_cast(half8, h);
-    lo = __builtin_bit_cast(half8, l);
 }
 
-// element i of the B operand's eight holds element order(i) of the dword
-__device__ __forceinline__ constexpr int code_order(int i) { return i % 2 * 4 + i / 2; }
+// a row's values of the groups of a step, from the lane groups that read them to every lane
+template <int GS>
+__device__ __forceinline__ void spread(uint32_t v, uint32_t (&out)[4 >> GS]) {
+    if constexpr (GS == 2) {
+        out[0] = v;
+    } else {
+        const auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        if constexpr (GS == 1) {
+            out[0] = p[0];
+            out[1] = p[1];
+        } else {
+            const auto a = __builtin_amdgcn_permlane16_swap(p[0], p[0], false, false), b = __builtin_amdgcn_permlane16_swap(p[1], p[1], false, false);
+            out[0] = a[0];
+            out[1] = a[1];
+            out[2] = b[0];
+            out[3] = b[1];
+        }
+    }
+}
 
-// NQB blocks of eight queries at a time
-template <int DT, int NQB, bool MINS>
-__global__ void __launch_bounds__(kScoreThreads) rg_q4_score_kernel(ScoreArgs A) {
-    typedef typename Elem<DT>::T T;
+// element i of the eight holds element order(i) of the dword, times 16 where i & 2
+__device__ __forceinline__ constexpr int code_order(int i) { return i % 2 * 4 + i / 2; }
+__device__ __forceinline__ half8 codes8(uint32_t w) {
+    const uint32_t h = w >> 8;
+    return __builtin_bit_cast(half8, u32x4{w & 0x000f000fu, w & 0x00f000f0u, h & 0x000f000fu, h & 0x00f000f0u});
+}
+
+// NQB blocks of eight queries at a time; groups of 32 << GS elements
+template <int NQB, int GS, bool MINS>
+__global__ void __launch_bounds__(kScoreThreads, NQB == 1 ? 4 : 2) rg_q4_score_kernel(ScoreArgs A) {
+    constexpr uint32_t NS = 4 >> GS;                  // groups of a step
     extern __shared__ char lds[];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
     const uint32_t dim = A.dim, D = (dim + 7) / 8, chunks = (D + 3) / 4, steps = (chunks + 3) / 4;       // dwords, chunks, steps of four chunks of a row
-    half8 *X = reinterpret_cast<half8 *>(lds);                                        // [block][step][t][lane]
-    uint32_t *XG = reinterpret_cast<uint32_t *>(lds + (size_t)NQB * steps * 4096);    // [block][step][lane]: the chunk's sum, twice
-    float *factor = reinterpret_cast<float *>(XG + (MINS ? NQB * steps * 64 : 0));    // [query]
+    half8 *X = reinterpret_cast<half8 *>(lds);                                        // [block][step][product][lane]
+    f32x4 *seed = reinterpret_cast<f32x4 *>(lds + (size_t)NQB * steps * 4096);        // [block][step][group][lane group]: what a partial sum starts at
+    float *factor = reinterpret_cast<float *>(seed + NQB * steps * NS * 4);           // [query]
 
     struct Stage {
         u32x4 c[2];
-        uint32_t s[2], m[2];
+        uint32_t s[2], m[2];                         // of the group lane group g reads: 4 j + g, 2 j + g / 2 or j
     };
     Stage ring[kScoreDepth];
     const uint32_t waves = kScoreThreads / 64, tiles = (A.nb + kScoreRows - 1) / kScoreRows;
@@ -152,12 +182,11 @@ __global__ void __launch_bounds__(kScoreThreads) rg_q4_score_kernel(ScoreArgs A)
         ++asked;
         const char *codes = reinterpret_cast<const char *>(A.codes + (size_t)ptile * kScoreRows * A.cstride);
         const char *scales = reinterpret_cast<const char *>(A.scales + (size_t)ptile * kScoreRows * A.sstride), *mins = reinterpret_cast<const char *>(A.mins + (size_t)ptile * kScoreRows * A.sstride);
-        const uint32_t q = 4 * pstep + g, group2 = min(q >> A.chunk_shift, A.groups - 1) * 2;
+        const uint32_t chunk = 4 * pstep + g, group2 = min(chunk >> GS, A.groups - 1) * 2;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             if (D >= 4) {
-                typedef u32x4 u32x4_dw __attribute__((aligned(4)));
-                st.c[r] = *reinterpret_cast<const u32x4_dw *>(codes + (code_at[r] + min(16 * q, 4 * D - 16)));
+                st.c[r] = *reinterpret_cast<const u32x4_a4 *>(codes + (code_at[r] + min(16 * chunk, 4 * D - 16)));
             } else {
 #pragma unroll
                 for (int t = 0; t < 4; ++t) st.c[r][t] = *reinterpret_cast<const uint32_t *>(codes + (code_at[r] + 4 * min((uint32_t)t, D - 1)));
@@ -174,49 +203,57 @@ __global__ void __launch_bounds__(kScoreThreads) rg_q4_score_kernel(ScoreArgs A)
 #pragma unroll
     for (int d = 0; d < kScoreDepth; ++d) fetch(ring[d]);
 
+    auto value = [&](uint32_t q, uint32_t k) {       // an element of the queries
+        const size_t at = (size_t)q * A.qstride + k;
+        return A.dtype == RG_DTYPE_F32 ? static_cast<const float *>(A.queries)[at] : A.dtype == RG_DTYPE_F16 ? (float)static_cast<const _Float16 *>(A.queries)[at]
+                                                                                                      : (float)static_cast<const __bf16 *>(A.queries)[at];
+    };
     for (uint32_t q0 = 0; q0 < A.nq; q0 += 8 * NQB) {
-        // queries: the largest element of each, then halves in operand order (zeros behind dim and behind the last query)
+        // queries: the largest element of each, then halves in operand order (zeros behind dim and behind the last query) and sums of groups
         for (uint32_t q = wave; q < 8 * NQB; q += waves) {
             uint32_t m = 0;
             if (q0 + q < A.nq)
-                for (uint32_t k = lane; k < dim; k += 64) m = max(m, __float_as_uint((float)static_cast<const T *>(A.queries)[(size_t)(q0 + q) * A.qstride + k]) & 0x7fffffffu);
+                for (uint32_t k = lane; k < dim; k += 64) m = max(m, __float_as_uint(value(q0 + q, k)) & 0x7fffffffu);
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
             if (lane == 0) factor[q] = __uint_as_float(m);
         }
         __syncthreads();
-        auto element = [&](uint32_t q, uint32_t k, float top, float down) {      // a query's element, scaled; of one that is not finite the signs of its infinities
+        auto element = [&](uint32_t q, uint32_t k, float top, float down) {      // scaled; of a query that is not finite the signs of its infinities
             if (q0 + q >= A.nq || k >= dim) return 0.0f;
-            const float v = (float)static_cast<const T *>(A.queries)[(size_t)(q0 + q) * A.qstride + k];
+            const float v = value(q0 + q, k);
             if (top < INFINITY) return v * down;
             return fabsf(v) < INFINITY ? 0.0f : fabsf(v) == INFINITY ? copysignf(1.0f, v) : v;
         };
         for (uint32_t i = tid; i < NQB * steps * 4 * 4 * 8; i += kScoreThreads) {
-            const uint32_t q = i % 8, gg = i / 8 % 4, t = i / 32 % 4, j = i / 128 % steps, qb = i / 128 / steps;
+            const uint32_t q = i % 8, gg = i / 8 % 4, u = i / 32 % 4, j = i / 128 % steps, qb = i / 128 / steps;
             const float top = factor[qb * 8 + q], down = pow2(-row_exponent(top));
-            const uint32_t c = 4 * j + gg, d = D >= 4 ? min(4 * c, D - 4) + t : t;
+            const uint32_t c = 4 * j + from_group<GS>(u, gg), d = (D >= 4 ? min(4 * c, D - 4) : 0) + from_dword<GS>(u, gg);
             half8 hi, lo;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float v = d >= 4 * c && d < D ? element(qb * 8 + q, 8 * d + code_order(e), top, down) : 0.0f;
+                const float v = d >= 4 * c && d < D ? element(qb * 8 + q, 8 * d + code_order(e), top, down) * (e & 2 ? 1.0f : 16.0f) : 0.0f;
                 hi[e] = (_Float16)v;
                 lo[e] = (_Float16)(v - (float)hi[e]);
             }
-            half8 *at = X + ((size_t)(qb * steps + j) * 4 + t) * 64 + gg * 16 + q;
+            half8 *at = X + ((size_t)(qb * steps + j) * 4 + u) * 64 + gg * 16 + 2 * q;
             at[0] = hi;
-            at[8] = lo;
+            at[1] = lo;
         }
-        if (MINS)
-            for (uint32_t i = tid; i < NQB * steps * 4 * 8; i += kScoreThreads) {
-                const uint32_t q = i % 8, gg = i / 8 % 4, j = i / 32 % steps, qb = i / 32 / steps;
-                const float top = factor[qb * 8 + q], down = pow2(-row_exponent(top));
-                float v = 0.0f;
-                for (uint32_t k = 32 * (4 * j + gg); k < min(32 * (4 * j + gg) + 32, dim); ++k) v += element(qb * 8 + q, k, top, down);
-                const _Float16 h = (_Float16)v, l = (_Float16)(v - (float)h);
-                uint32_t *at = XG + (qb * steps + j) * 64 + gg * 16 + q;
-                at[0] = 0x10001u * __builtin_bit_cast(uint16_t, h);
-                at[8] = 0x10001u * __builtin_bit_cast(uint16_t, l);
+        for (uint32_t i = tid; i < NQB * steps * NS * 8; i += kScoreThreads) {
+            const uint32_t q = i % 8, u = i / 8 % NS, j = i / 8 / NS % steps, qb = i / 8 / NS / steps;
+            const float top = factor[qb * 8 + q], down = pow2(-row_exponent(top));
+            const uint32_t k0 = (j * NS + u) * (32 << GS);
+            float hi = 0.0f, lo = 0.0f;              // of the halves as they are multiplied
+            for (uint32_t k = k0; k < min(k0 + (32 << GS), dim); ++k) {
+                const float v = element(qb * 8 + q, k, top, down) * (k & 1 ? 1.0f : 16.0f), h = (float)(_Float16)v, l = (float)(_Float16)(v - h), f = k & 1 ? 1.0f : 0.0625f;
+                hi = fmaf(f, h, hi);
+                lo = fmaf(f, l, lo);
             }
+            float *at = reinterpret_cast<float *>(seed + ((size_t)(qb * steps + j) * NS + u) * 4 + q / 2) + q % 2 * 2;
+            at[0] = hi * -0x1p-17f;                  // -8 x 2^-20
+            at[1] = lo * -0x1p-17f;
+        }
         __syncthreads();
 
         if (q0) {                                    // the base once more for the next queries
@@ -236,65 +273,62 @@ __global__ void __launch_bounds__(kScoreThreads) rg_q4_score_kernel(ScoreArgs A)
 #pragma unroll
             for (int d = 0; d < kScoreDepth; ++d) {
                 if (it + d >= total) break;
-                const Stage st = ring[d];
+                Stage st = ring[d];
                 fetch(ring[d]);
-                half2 s[2];
+                uint32_t scale[2][NS], low[2][NS];
 #pragma unroll
-                for (int r = 0; r < 2; ++r) s[r] = __builtin_bit_cast(half2, st.s[r] * 0x10001u);
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    half8 x[NQB];
-#pragma unroll
-                    for (int b = 0; b < NQB; ++b) x[b] = X[((size_t)(b * steps + step) * 4 + t) * 64 + lane];
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        half8 hi, lo;
-                        dequant(st.c[r][t], s[r], hi, lo);
-#pragma unroll
-                        for (int b = 0; b < NQB; ++b) {
-                            acc[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, x[b], acc[r][b], 0, 0, 0);
-                            acc[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, x[b], acc[r][b], 0, 0, 0);
-                        }
-                    }
+                for (int r = 0; r < 2; ++r) {
+                    exchange<GS>(st.c[r]);
+                    spread<GS>(st.s[r], scale[r]);
+                    if (MINS) spread<GS>(st.m[r], low[r]);
                 }
-                if (MINS) {
+#pragma unroll
+                for (int b = 0; b < NQB; ++b) {
+                    half8 x[4];
+                    f32x4 start[NS];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) x[u] = X[((size_t)(b * steps + step) * 4 + u) * 64 + lane];
+#pragma unroll
+                    for (uint32_t u = 0; u < NS; ++u) start[u] = seed[((size_t)(b * steps + step) * NS + u) * 4 + g];
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const float off = fmaf(half_bits((uint16_t)st.s[r]), 8.0f, half_bits((uint16_t)st.m[r]));
-                        half8 o = {0, 0, 0, 0, 0, 0, 0, 0};
-                        o[0] = (_Float16)off;
-                        o[1] = (_Float16)(off - (float)o[0]);
+                        f32x4 sum[NS];
 #pragma unroll
-                        for (int b = 0; b < NQB; ++b) {
-                            const u32x4 v = {XG[(b * steps + step) * 64 + lane], 0, 0, 0};
-                            acc[r][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(o, __builtin_bit_cast(half8, v), acc[r][b], 0, 0, 0);
+                        for (int u = 0; u < 4; ++u) {
+                            const int v = GS == 0 ? u : GS == 1 ? u & 1 : 0;
+                            sum[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[u], codes8(st.c[r][u]), u == v ? start[v] : sum[v], 0, 0, 0);
+                        }
+#pragma unroll
+                        for (uint32_t u = 0; u < NS; ++u) {
+                            const float s = half_bits((uint16_t)scale[r][u]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[r][b][i] = fmaf(s, sum[u][i], acc[r][b][i]);
+                            if (MINS) {
+                                const float off = fmaf(half_bits((uint16_t)low[r][u]), -0.125f, -s);      // -(m + 8 s) / 8
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) acc[r][b][i] = fmaf(off, start[u][i], acc[r][b][i]);
+                            }
                         }
                     }
                 }
                 if (++step == steps) {
                     step = 0;
 #pragma unroll
+                    for (int b = 0; b < NQB; ++b)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t q = b * 8 + 2 * g + h;
+                            const float top = factor[q], up = row_factor(top, row_exponent(top));
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                const uint32_t row = tile * kScoreRows + 16 * r + n;
+                                if (q0 + q < A.nq && row < A.nb) A.out[(size_t)(q0 + q) * A.ostride + row] = (acc[r][b][2 * h] + acc[r][b][2 * h + 1]) * 0x1p20f * up;
+                            }
+                        }
+#pragma unroll
                     for (int r = 0; r < 2; ++r)
 #pragma unroll
-                        for (int b = 0; b < NQB; ++b) {
-                            f32x4 v = acc[r][b];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) v[i] += __shfl_xor(v[i], 8);
-                            const uint32_t q = q0 + b * 8 + n, row = tile * kScoreRows + 16 * r + 4 * g;
-                            if (n < 8 && q < A.nq && row < A.nb) {
-                                const float top = factor[b * 8 + n], up = row_factor(top, row_exponent(top));
-                                float *to = A.out + q * A.ostride + row;
-                                if (row + 4 <= A.nb) {
-                                    typedef f32x4 f32x4_dw __attribute__((aligned(4)));
-                                    *reinterpret_cast<f32x4_dw *>(to) = v * up;
-                                } else {
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i)
-                                        if (row + i < A.nb) to[i] = v[i] * up;
-                                }
-                            }
-                            acc[r][b] = f32x4{0, 0, 0, 0};
-                        }
+                        for (int b = 0; b < NQB; ++b) acc[r][b] = f32x4{0, 0, 0, 0};
                     tile += stride;
                 }
             }
@@ -303,28 +337,28 @@ __global__ void __launch_bounds__(kScoreThreads) rg_q4_score_kernel(ScoreArgs A)
     }
 }
 
-size_t score_lds(uint32_t dim, int nqb, bool mins) {
+size_t score_lds(uint32_t dim, int nqb, uint32_t group) {
     const size_t steps = (((dim + 7) / 8 + 3) / 4 + 3) / 4;
-    return nqb * steps * (4096 + (mins ? 256 : 0)) + nqb * 32;
+    return nqb * (steps * (4096 + 128 / group * 64) + 32);
 }
 
-template <int DT, int NQB>
-rg_status launch_score(const ScoreArgs &A, hipStream_t s) {
-    auto kern = A.mins ? rg_q4_score_kernel<DT, NQB, true> : rg_q4_score_kernel<DT, NQB, false>;
-    const size_t lds = score_lds(A.dim, NQB, A.mins != nullptr);
+template <int NQB, int GS>
+rg_status launch_score(const ScoreArgs &A, size_t lds, hipStream_t s) {
+    auto kern = A.mins ? rg_q4_score_kernel<NQB, GS, true> : rg_q4_score_kernel<NQB, GS, false>;
     RG_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     const uint32_t tiles = (A.nb + kScoreRows - 1) / kScoreRows, per_cu = std::max<uint32_t>(1, std::min<uint32_t>(2, (uint32_t)(160 * 1024 / lds)));
     hipLaunchKernelGGL(kern, dim3(std::min(tiles, 256u * per_cu)), dim3(kScoreThreads), lds, s, A);
     RG_HIP(hipGetLastError());
     return RG_OK;
 }
-template <int DT>
-rg_status launch_score_dt(const ScoreArgs &A, hipStream_t s) {
+template <int GS>
+rg_status launch_score_gs(const ScoreArgs &A, hipStream_t s) {
     // as many queries per reading of the base as there are, and as LDS holds
-    const bool mins = A.mins != nullptr;
-    if (A.nq > 16 && score_lds(A.dim, 4, mins) <= 160 * 1024) return launch_score<DT, 4>(A, s);
-    if (A.nq > 8 && score_lds(A.dim, 2, mins) <= 160 * 1024) return launch_score<DT, 2>(A, s);
-    return launch_score<DT, 1>(A, s);
+    const uint32_t group = 32 << GS;
+    int nqb = A.nq > 16 ? 4 : A.nq > 8 ? 2 : 1;
+    while (score_lds(A.dim, nqb, group) > 160 * 1024) nqb /= 2;
+    const size_t lds = score_lds(A.dim, nqb, group);
+    return nqb == 4 ? launch_score<4, GS>(A, lds, s) : nqb == 2 ? launch_score<2, GS>(A, lds, s) : launch_score<1, GS>(A, lds, s);
 }
 
 rg_status check_form(const void *codes, uint64_t cstride, const void *scales, const void *mins, uint64_t sstride, uint32_t nb, uint32_t dim, uint32_t group) {
@@ -397,9 +431,9 @@ rg_status rg_q4_score_dev(const uint8_t *d_codes, uint64_t cstride, const uint16
     ScoreArgs A;
     A.codes = d_codes; A.scales = d_scales; A.mins = d_mins; A.queries = d_queries; A.out = d_out;
     A.cstride = cstride; A.sstride = sstride; A.qstride = qstride; A.ostride = ostride;
-    A.nb = nb; A.nq = nq; A.dim = dim; A.chunk_shift = group == 32 ? 0 : group == 64 ? 1 : 2; A.groups = (dim + group - 1) / group;
+    A.nb = nb; A.nq = nq; A.dim = dim; A.groups = (dim + group - 1) / group; A.dtype = dtype;
     hipStream_t s = (hipStream_t)stream;
-    return dtype == RG_DTYPE_F32 ? launch_score_dt<RG_DTYPE_F32>(A, s) : dtype == RG_DTYPE_F16 ? launch_score_dt<RG_DTYPE_F16>(A, s) : launch_score_dt<RG_DTYPE_BF16>(A, s);
+    return group == 32 ? launch_score_gs<0>(A, s) : group == 64 ? launch_score_gs<1>(A, s) : launch_score_gs<2>(A, s);
 }
 
 }  // extern "C"
