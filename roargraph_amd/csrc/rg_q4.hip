@@ -97,7 +97,7 @@ struct ScoreArgs {
     int dtype;
 };
 
-constexpr int kScoreThreads = 512, kScoreRows = 32, kScoreDepth = 4;
+constexpr int kScoreThreads = 512, kScoreRows = 32, kScoreDepth = 2;
 
 // where product u of a step finds its dword in lane group g: (lane group it was read by, dword of the 16 bytes)
 template <int GS> __device__ __forceinline__ constexpr uint32_t from_group(uint32_t u, uint32_t g) { return GS == 0 ? u : GS == 1 ? (u & 1) * 2 + (g & 1) : g; }
@@ -203,56 +203,70 @@ __global__ void __launch_bounds__(kScoreThreads, NQB == 1 ? 4 : 2) rg_q4_score_k
 #pragma unroll
     for (int d = 0; d < kScoreDepth; ++d) fetch(ring[d]);
 
-    auto value = [&](uint32_t q, uint32_t k) {       // an element of the queries
-        const size_t at = (size_t)q * A.qstride + k;
-        return A.dtype == RG_DTYPE_F32 ? static_cast<const float *>(A.queries)[at] : A.dtype == RG_DTYPE_F16 ? (float)static_cast<const _Float16 *>(A.queries)[at]
-                                                                                                      : (float)static_cast<const __bf16 *>(A.queries)[at];
+    // N elements of a query from element k on, behind dim the last one again (nothing waits between the loads)
+    auto values = [&](uint32_t q, uint32_t k, uint32_t apart, auto &v) {
+        constexpr int N = sizeof(v) / sizeof(v[0]);
+        const char *row = static_cast<const char *>(A.queries) + (size_t)q * A.qstride * (A.dtype == RG_DTYPE_F32 ? 4 : 2);
+        if (A.dtype == RG_DTYPE_F32) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = reinterpret_cast<const float *>(row)[min(k + i * apart, dim - 1)];
+        } else if (A.dtype == RG_DTYPE_F16) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = (float)reinterpret_cast<const _Float16 *>(row)[min(k + i * apart, dim - 1)];
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = (float)reinterpret_cast<const __bf16 *>(row)[min(k + i * apart, dim - 1)];
+        }
     };
     for (uint32_t q0 = 0; q0 < A.nq; q0 += 8 * NQB) {
         // queries: the largest element of each, then halves in operand order (zeros behind dim and behind the last query) and sums of groups
         for (uint32_t q = wave; q < 8 * NQB; q += waves) {
             uint32_t m = 0;
             if (q0 + q < A.nq)
-                for (uint32_t k = lane; k < dim; k += 64) m = max(m, __float_as_uint(value(q0 + q, k)) & 0x7fffffffu);
+                for (uint32_t k = lane; k < dim; k += 256) {
+                    float v[4];
+                    values(q0 + q, k, 64, v);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+                }
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
             if (lane == 0) factor[q] = __uint_as_float(m);
         }
         __syncthreads();
-        auto element = [&](uint32_t q, uint32_t k, float top, float down) {      // scaled; of a query that is not finite the signs of its infinities
-            if (q0 + q >= A.nq || k >= dim) return 0.0f;
-            const float v = value(q0 + q, k);
-            if (top < INFINITY) return v * down;
-            return fabsf(v) < INFINITY ? 0.0f : fabsf(v) == INFINITY ? copysignf(1.0f, v) : v;
-        };
         for (uint32_t i = tid; i < NQB * steps * 4 * 4 * 8; i += kScoreThreads) {
             const uint32_t q = i % 8, gg = i / 8 % 4, u = i / 32 % 4, j = i / 128 % steps, qb = i / 128 / steps;
             const float top = factor[qb * 8 + q], down = pow2(-row_exponent(top));
             const uint32_t c = 4 * j + from_group<GS>(u, gg), d = (D >= 4 ? min(4 * c, D - 4) : 0) + from_dword<GS>(u, gg);
+            const bool any = q0 + qb * 8 + q < A.nq && d >= 4 * c && d < D;
+            float v[8];
+            values(any ? q0 + qb * 8 + q : q0, 8 * min(d, D - 1), 1, v);
             half8 hi, lo;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float v = d >= 4 * c && d < D ? element(qb * 8 + q, 8 * d + code_order(e), top, down) * (e & 2 ? 1.0f : 16.0f) : 0.0f;
-                hi[e] = (_Float16)v;
-                lo[e] = (_Float16)(v - (float)hi[e]);
+                float x = v[code_order(e)];          // scaled; of a query that is not finite the signs of its infinities
+                x = top < INFINITY ? x * down : fabsf(x) < INFINITY ? 0.0f : fabsf(x) == INFINITY ? copysignf(1.0f, x) : x;
+                x = any && 8 * d + code_order(e) < dim ? x * (e & 2 ? 1.0f : 16.0f) : 0.0f;
+                hi[e] = (_Float16)x;
+                lo[e] = (_Float16)(x - (float)hi[e]);
             }
             half8 *at = X + ((size_t)(qb * steps + j) * 4 + u) * 64 + gg * 16 + 2 * q;
             at[0] = hi;
             at[1] = lo;
         }
-        for (uint32_t i = tid; i < NQB * steps * NS * 8; i += kScoreThreads) {
-            const uint32_t q = i % 8, u = i / 8 % NS, j = i / 8 / NS % steps, qb = i / 8 / NS / steps;
-            const float top = factor[qb * 8 + q], down = pow2(-row_exponent(top));
-            const uint32_t k0 = (j * NS + u) * (32 << GS);
-            float hi = 0.0f, lo = 0.0f;              // of the halves as they are multiplied
-            for (uint32_t k = k0; k < min(k0 + (32 << GS), dim); ++k) {
-                const float v = element(qb * 8 + q, k, top, down) * (k & 1 ? 1.0f : 16.0f), h = (float)(_Float16)v, l = (float)(_Float16)(v - h), f = k & 1 ? 1.0f : 0.0625f;
-                hi = fmaf(f, h, hi);
-                lo = fmaf(f, l, lo);
-            }
-            float *at = reinterpret_cast<float *>(seed + ((size_t)(qb * steps + j) * NS + u) * 4 + q / 2) + q % 2 * 2;
-            at[0] = hi * -0x1p-17f;                  // -8 x 2^-20
-            at[1] = lo * -0x1p-17f;
+        __syncthreads();
+        for (uint32_t i = tid; i < NQB * steps * NS * 16; i += kScoreThreads) {
+            const uint32_t h = i % 16, u = i / 16 % NS, j = i / 16 / NS % steps, qb = i / 16 / NS / steps;
+            float sum = 0.0f;                        // of the halves as they are multiplied
+#pragma unroll
+            for (uint32_t p = 0; p < (1u << GS); ++p)
+#pragma unroll
+                for (uint32_t gg = 0; gg < 4; ++gg) {
+                    const half8 x = X[((size_t)(qb * steps + j) * 4 + u + p * NS) * 64 + gg * 16 + h];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sum = fmaf((float)x[e], e & 2 ? 1.0f : 0.0625f, sum);
+                }
+            reinterpret_cast<float *>(seed + ((size_t)(qb * steps + j) * NS + u) * 4)[h] = sum * -0x1p-17f;      // -8 x 2^-20
         }
         __syncthreads();
 
