@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "rg.h"
 #include "rg_internal.h"
@@ -17,50 +18,133 @@ constexpr uint32_t kMaxDim = 4096;
 
 __device__ __forceinline__ float half_bits(uint16_t b) { return (float)__builtin_bit_cast(_Float16, b); }
 
-// one thread per group of a row.  The nearest level is decided exactly: x, minimum, scale and code have few enough bits that
-// x - min - code * scale is exact in 64 bits, and its distance to half a scale decides (ties to the even code).
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// eight elements of a row from k on (n of them exist)
+template <int DT>
+__device__ __forceinline__ void load8(const typename Elem<DT>::T *row, uint32_t k, uint32_t n, bool vec, float (&v)[8]) {
+    if (n == 8 && vec) {
+        if constexpr (DT == RG_DTYPE_F32) {
+            const f32x4 a = *reinterpret_cast<const f32x4 *>(row + k), b = *reinterpret_cast<const f32x4 *>(row + k + 4);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = i < 4 ? a[i % 4] : b[i % 4];
+        } else {
+            typedef typename std::conditional<DT == RG_DTYPE_F16, half8, bf8>::type V;
+            const V a = *reinterpret_cast<const V *>(row + k);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)row[k + min((uint32_t)i, n - 1)];      // (behind the row: its last element, which changes no extremum)
+    }
+}
+
+// Packing: bound by reading the rows.  A lane holds eight elements, a group is 4, 8 or 16 neighbouring lanes.  The nearest level comes from an
+// fp32 quotient wherever that is not close to the border of two; there (one wave in a hundred) 64 bits decide, in which x, minimum and
+// code * scale are exact; ties go to the even code.
 template <int DT>
 __global__ void __launch_bounds__(256) rg_q4_pack_kernel(const void *rows, uint32_t nb, uint64_t stride, uint32_t dim, uint32_t group, uint8_t *codes, uint64_t cstride,
                                                          uint16_t *scales, uint16_t *mins, uint64_t sstride) {
     typedef typename Elem<DT>::T T;
-    const uint32_t ng = (dim + group - 1) / group;
-    for (uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x; at < (uint64_t)nb * ng; at += (uint64_t)gridDim.x * 256) {
-    const uint32_t j = (uint32_t)(at / ng), g = (uint32_t)(at % ng), k0 = g * group, n = min(group, dim - k0);
-    const T *x = static_cast<const T *>(rows) + (size_t)j * stride + k0;
-    float lo = INFINITY, hi = -INFINITY, top = 0.0f;
-    for (uint32_t k = 0; k < n; ++k) { const float v = (float)x[k]; lo = fminf(lo, v); hi = fmaxf(hi, v); top = fmaxf(top, fabsf(v)); }
-    const _Float16 s16 = (_Float16)(mins ? (hi - lo) * (1.0f / 15.0f) : top * (1.0f / 7.0f)), m16 = (_Float16)(mins ? lo : 0.0f);
-    const double s = (double)(float)s16, m = (double)(float)m16;
+    const uint32_t lanes = group / 8, D = (dim + 7) / 8, per_row = (D + lanes - 1) / lanes * lanes;
+    const bool vec = ((uintptr_t)rows | stride * sizeof(T)) % 16 == 0;
     const int first = mins ? 0 : -8;
-    scales[(size_t)j * sstride + g] = __builtin_bit_cast(uint16_t, s16);
-    if (mins) mins[(size_t)j * sstride + g] = __builtin_bit_cast(uint16_t, m16);
-    uint8_t *out = codes + (size_t)j * cstride + k0 / 2;
-    for (uint32_t k = 0; k < n; k += 2) {
-        uint32_t b = 0;
-        for (uint32_t e = 0; e < 2; ++e) {
-            if (k + e >= n) continue;
-            int c = 0;
-            if (s > 0) c = max(first, min(first + 15, (int)rint(((double)(float)x[k + e] - m) / s)));
-            b |= (uint32_t)(c - first) << (4 * e);
+    // (whole waves turn together: per_row * nb rounded up to them)
+    const uint64_t total = (uint64_t)nb * per_row;
+    uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    uint32_t j = (uint32_t)(at / per_row), l = (uint32_t)(at % per_row);
+    const uint64_t hop = (uint64_t)gridDim.x * 256;
+    const uint32_t hop_rows = (uint32_t)(hop / per_row), hop_lanes = (uint32_t)(hop % per_row);
+    for (; at - threadIdx.x % 64 < total; at += hop) {
+        const bool here = at < total && l < D;
+        const uint32_t row = min(j, nb - 1), k = min(l, D - 1) * 8, n = min(8u, dim - k);
+        float v[8];
+        load8<DT>(static_cast<const T *>(rows) + (size_t)row * stride, k, n, vec, v);
+        float lo = v[0], hi = v[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) { lo = fminf(lo, v[i]); hi = fmaxf(hi, v[i]); }
+        // (a lane behind the row holds the row's last eight again: of the same group as the lanes before it, or alone in a group that is none)
+        for (uint32_t d = 1; d < lanes; d <<= 1) { lo = fminf(lo, __shfl_xor(lo, d)); hi = fmaxf(hi, __shfl_xor(hi, d)); }
+        const _Float16 s16 = (_Float16)(mins ? (hi - lo) * (1.0f / 15.0f) : fmaxf(fabsf(lo), fabsf(hi)) * (1.0f / 7.0f)), m16 = (_Float16)(mins ? lo : 0.0f);
+        const float s = (float)s16, m = (float)m16, inv = s > 0.0f ? 1.0f / s : 0.0f;
+        // how far the fp32 quotient can be off: half a step of x - m and a few of the quotient
+        const float off = (fabsf(m) * inv + 32.0f) * 0x1p-22f;
+        float c[8];
+        bool close = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float t = (v[i] - m) * inv;
+            c[i] = rintf(t);
+            close |= fabsf(fabsf(t - c[i]) - 0.5f) <= off;
         }
-        out[k / 2] = (uint8_t)b;
-    }
-    if (g == ng - 1)
-        for (uint32_t b = (dim + 1) / 2; b < (dim + 7) / 8 * 4; ++b) codes[(size_t)j * cstride + b] = 0;
+        if (__any(close)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const double r = fma(-(double)c[i], (double)s, (double)v[i] - (double)m), half = 0.5 * (double)s;
+                const bool odd = ((int)c[i] & 1) != 0;
+                if (r > half || (r == half && odd)) c[i] += 1.0f;
+                else if (r < -half || (r == -half && odd)) c[i] -= 1.0f;
+            }
+        }
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int code = s > 0.0f ? (int)fminf(fmaxf(c[i], (float)first), (float)(first + 15)) - first : -first;
+            if ((uint32_t)i < n) w |= (uint32_t)code << (4 * i);
+        }
+        if (here) {
+            *reinterpret_cast<uint32_t *>(codes + (size_t)j * cstride + l * 4) = w;
+            if (l % lanes == 0) {
+                scales[(size_t)j * sstride + l / lanes] = __builtin_bit_cast(uint16_t, s16);
+                if (mins) mins[(size_t)j * sstride + l / lanes] = __builtin_bit_cast(uint16_t, m16);
+            }
+        }
+        l += hop_lanes;
+        j += hop_rows;
+        if (l >= per_row) { l -= per_row; ++j; }
     }
 }
 
+// Unpacking: bound by writing the values, eight a lane.
 __global__ void __launch_bounds__(256) rg_q4_unpack_kernel(const uint8_t *codes, uint64_t cstride, const uint16_t *scales, const uint16_t *mins, uint64_t sstride, uint32_t nb, uint32_t dim,
                                                            uint32_t group, const uint32_t *ids, uint32_t n, float *out, uint64_t ostride) {
-    for (uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x; at < (uint64_t)n * dim; at += (uint64_t)gridDim.x * 256) {
-    const uint32_t i = (uint32_t)(at / dim), k = (uint32_t)(at % dim), j = ids ? ids[i] : i;
-    float v = NAN;                              // no such row
-    if (j < nb) {
-        const uint32_t c = codes[(size_t)j * cstride + k / 2] >> (4 * (k & 1)) & 15u, g = k / group;
-        const float s = half_bits(scales[(size_t)j * sstride + g]);
-        v = mins ? (float)c * s + half_bits(mins[(size_t)j * sstride + g]) : (float)((int)c - 8) * s;
-    }
-    out[(size_t)i * ostride + k] = v;
+    const uint32_t D = (dim + 7) / 8;
+    const bool vec = ((uintptr_t)out | ostride * 4) % 16 == 0;
+    uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    uint32_t i = (uint32_t)(at / D), l = (uint32_t)(at % D);
+    const uint64_t hop = (uint64_t)gridDim.x * 256;
+    const uint32_t hop_rows = (uint32_t)(hop / D), hop_lanes = (uint32_t)(hop % D);
+    for (; at < (uint64_t)n * D; at += hop) {
+        const uint32_t j = ids ? ids[i] : i, k = 8 * l;
+        float v[8];
+        if (j < nb) {
+            const uint32_t w = *reinterpret_cast<const uint32_t *>(codes + (size_t)j * cstride + 4 * l);
+            const float s = half_bits(scales[(size_t)j * sstride + k / group]), m = mins ? half_bits(mins[(size_t)j * sstride + k / group]) : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t c = w >> (4 * e) & 15u;
+                v[e] = mins ? (float)c * s + m : (float)((int)c - 8) * s;
+            }
+        } else {                                     // no such row
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = NAN;
+        }
+        float *to = out + (size_t)i * ostride + k;
+        if (vec && k + 8 <= dim) {
+            *reinterpret_cast<f32x4 *>(to) = f32x4{v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<f32x4 *>(to + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (k + e < dim) to[e] = v[e];
+        }
+        l += hop_lanes;
+        i += hop_rows;
+        if (l >= D) { l -= D; ++i; }
     }
 }
 
@@ -82,9 +166,6 @@ __global__ void __launch_bounds__(256) rg_q4_unpack_kernel(const uint8_t *codes,
 // on their way while one is multiplied.  A dword's codes come out in the order 0 4 1 5 2 6 3 7, and the queries lie in LDS in that order.
 //
 // (A first form made s (c - 8) of every code, exactly, as a pair of halves: 21 vector instructions a dword, 72 % of the vector units' time and 3.3 TB/s.)
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
 
 struct ScoreArgs {
@@ -404,9 +485,9 @@ rg_status rg_q4_pack_dev(const void *d_rows, uint32_t nb, uint64_t stride, uint3
     if (stride < dim || (uintptr_t)d_rows % elem_bytes(dtype)) return set_error(RG_ERR_ARG, "rows: stride smaller than dim, or not aligned to their elements");
     OnDevice on(device);
     if (on.st != RG_OK) return on.st;
-    const uint64_t n = (uint64_t)nb * ((dim + group - 1) / group);
+    const uint64_t n = (uint64_t)nb * ((dim + group - 1) / group) * (group / 8);
     auto kern = dtype == RG_DTYPE_F32 ? rg_q4_pack_kernel<RG_DTYPE_F32> : dtype == RG_DTYPE_F16 ? rg_q4_pack_kernel<RG_DTYPE_F16> : rg_q4_pack_kernel<RG_DTYPE_BF16>;
-    hipLaunchKernelGGL(kern, dim3((uint32_t)std::min<uint64_t>((n + 255) / 256, 1u << 20)), dim3(256), 0, (hipStream_t)stream, d_rows, nb, stride, dim, group, d_codes, cstride, d_scales, d_mins, sstride);
+    hipLaunchKernelGGL(kern, dim3((uint32_t)std::min<uint64_t>((n + 255) / 256, 256u * 32u)), dim3(256), 0, (hipStream_t)stream, d_rows, nb, stride, dim, group, d_codes, cstride, d_scales, d_mins, sstride);
     RG_HIP(hipGetLastError());
     return RG_OK;
 }
@@ -423,7 +504,7 @@ rg_status rg_q4_unpack_dev(const uint8_t *d_codes, uint64_t cstride, const uint1
     if (ostride < dim || (uintptr_t)d_out % 4) return set_error(RG_ERR_ARG, "output rows: stride smaller than dim, or not aligned to their elements");
     OnDevice on(device);
     if (on.st != RG_OK) return on.st;
-    hipLaunchKernelGGL(rg_q4_unpack_kernel, dim3((uint32_t)std::min<uint64_t>(((uint64_t)n * dim + 255) / 256, 1u << 20)), dim3(256), 0, (hipStream_t)stream, d_codes, cstride, d_scales, d_mins, sstride, nb, dim, group, d_ids,
+    hipLaunchKernelGGL(rg_q4_unpack_kernel, dim3((uint32_t)std::min<uint64_t>(((uint64_t)n * ((dim + 7) / 8) + 255) / 256, 256u * 32u)), dim3(256), 0, (hipStream_t)stream, d_codes, cstride, d_scales, d_mins, sstride, nb, dim, group, d_ids,
                        n, d_out, ostride);
     RG_HIP(hipGetLastError());
     return RG_OK;
