@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(256) rg_q4_pack_kernel(const void *rows, uint3
         bool close = false;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float t = (v[i] - m) * inv;
+            const float t = (v[i] - m) * inv;        // (a scale of zero: all are level 0)
             c[i] = rintf(t);
             close |= fabsf(fabsf(t - c[i]) - 0.5f) <= off;
         }
@@ -90,12 +90,13 @@ __global__ void __launch_bounds__(256) rg_q4_pack_kernel(const void *rows, uint3
                 else if (r < -half || (r == -half && odd)) c[i] -= 1.0f;
             }
         }
-        uint32_t w = 0;
+        float half[2] = {0.0f, 0.0f};                // four codes each (codes and their sums are whole numbers)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int code = s > 0.0f ? (int)fminf(fmaxf(c[i], (float)first), (float)(first + 15)) - first : -first;
-            if ((uint32_t)i < n) w |= (uint32_t)code << (4 * i);
+        for (int i = 7; i >= 0; --i) {
+            const float code = __builtin_amdgcn_fmed3f(c[i], (float)first, (float)(first + 15)) - (float)first;
+            half[i / 4] = fmaf(half[i / 4], 16.0f, (uint32_t)i < n ? code : 0.0f);
         }
+        const uint32_t w = (uint32_t)half[0] | (uint32_t)half[1] << 16;
         if (here) {
             *reinterpret_cast<uint32_t *>(codes + (size_t)j * cstride + l * 4) = w;
             if (l % lanes == 0) {
@@ -135,8 +136,8 @@ __global__ void __launch_bounds__(256) rg_q4_unpack_kernel(const uint8_t *codes,
         }
         float *to = out + (size_t)i * ostride + k;
         if (vec && k + 8 <= dim) {
-            *reinterpret_cast<f32x4 *>(to) = f32x4{v[0], v[1], v[2], v[3]};
-            *reinterpret_cast<f32x4 *>(to + 4) = f32x4{v[4], v[5], v[6], v[7]};
+            __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4 *>(to));
+            __builtin_nontemporal_store(f32x4{v[4], v[5], v[6], v[7]}, reinterpret_cast<f32x4 *>(to + 4));
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
