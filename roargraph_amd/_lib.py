@@ -59,6 +59,15 @@ def lib():
         L.rg_index_close.argtypes = [C.c_void_p]
         L.rg_comm_destroy.argtypes = [C.c_void_p]
         L.rg_comm_uses_rccl.argtypes = [C.c_void_p]
+        # the operators that training loops and servers call most: plain ints, converted by ctypes itself
+        p, u32, u64, i32, f32 = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int, C.c_float
+        L.rg_softmax_workspace.argtypes = [i32, u32, u32, u32, i32, p]
+        L.rg_softmax_shard_dev.argtypes = [p, u32, u64, p, u32, u64, u32, i32, f32, p, u32, p, p, p, p, p, p, u64, i32, p]
+        L.rg_softmax_merge_dev.argtypes = [p, p, u32, u32, p, p, p, i32, p]
+        L.rg_softmax_grad_dev.argtypes = [p, u32, u64, p, u32, u64, u32, i32, f32, p, u32, p, p, p, p, p, p, u64, p, u64, p, u64, i32, p]
+        L.rg_q4_pack_dev.argtypes = [p, u32, u64, u32, i32, u32, p, u64, p, p, u64, i32, p]
+        L.rg_q4_unpack_dev.argtypes = [p, u64, p, p, u64, u32, u32, u32, p, u32, p, u64, i32, p]
+        L.rg_q4_score_dev.argtypes = [p, u64, p, p, u64, u32, u32, u32, p, u32, u64, i32, p, u64, i32, p]
         _lib = L
     return _lib
 

@@ -110,42 +110,42 @@ __global__ void __launch_bounds__(256) rg_q4_pack_kernel(const void *rows, uint3
     }
 }
 
-// Unpacking: bound by writing the values, eight a lane.
+// Unpacking: bound by writing the values.  VEC: eight a lane, written past the caches (nobody reads them soon); otherwise -- output rows that are
+// not 16-byte aligned, or of no whole dwords -- one a lane, so that neighbours write neighbours.
+template <bool VEC>
 __global__ void __launch_bounds__(256) rg_q4_unpack_kernel(const uint8_t *codes, uint64_t cstride, const uint16_t *scales, const uint16_t *mins, uint64_t sstride, uint32_t nb, uint32_t dim,
                                                            uint32_t group, const uint32_t *ids, uint32_t n, float *out, uint64_t ostride) {
-    const uint32_t D = (dim + 7) / 8;
-    const bool vec = ((uintptr_t)out | ostride * 4) % 16 == 0;
+    constexpr uint32_t E = VEC ? 8 : 1;              // elements a lane
+    const uint32_t per_row = dim / E;
     uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    uint32_t i = (uint32_t)(at / D), l = (uint32_t)(at % D);
+    uint32_t i = (uint32_t)(at / per_row), l = (uint32_t)(at % per_row);
     const uint64_t hop = (uint64_t)gridDim.x * 256;
-    const uint32_t hop_rows = (uint32_t)(hop / D), hop_lanes = (uint32_t)(hop % D);
-    for (; at < (uint64_t)n * D; at += hop) {
-        const uint32_t j = ids ? ids[i] : i, k = 8 * l;
-        float v[8];
+    const uint32_t hop_rows = (uint32_t)(hop / per_row), hop_lanes = (uint32_t)(hop % per_row);
+    for (; at < (uint64_t)n * per_row; at += hop) {
+        const uint32_t j = ids ? ids[i] : i, k = E * l;
+        float v[E];
         if (j < nb) {
-            const uint32_t w = *reinterpret_cast<const uint32_t *>(codes + (size_t)j * cstride + 4 * l);
+            const uint32_t w = *reinterpret_cast<const uint32_t *>(codes + (size_t)j * cstride + k / 8 * 4) >> 4 * (k % 8);
             const float s = half_bits(scales[(size_t)j * sstride + k / group]), m = mins ? half_bits(mins[(size_t)j * sstride + k / group]) : 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (uint32_t e = 0; e < E; ++e) {
                 const uint32_t c = w >> (4 * e) & 15u;
                 v[e] = mins ? (float)c * s + m : (float)((int)c - 8) * s;
             }
         } else {                                     // no such row
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = NAN;
+            for (uint32_t e = 0; e < E; ++e) v[e] = NAN;
         }
         float *to = out + (size_t)i * ostride + k;
-        if (vec && k + 8 <= dim) {
+        if constexpr (VEC) {
             __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4 *>(to));
             __builtin_nontemporal_store(f32x4{v[4], v[5], v[6], v[7]}, reinterpret_cast<f32x4 *>(to + 4));
         } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (k + e < dim) to[e] = v[e];
+            *to = v[0];
         }
         l += hop_lanes;
         i += hop_rows;
-        if (l >= D) { l -= D; ++i; }
+        if (l >= per_row) { l -= per_row; ++i; }
     }
 }
 
@@ -441,7 +441,7 @@ size_t score_lds(uint32_t dim, int nqb, uint32_t group) {
 template <int NQB, int GS>
 rg_status launch_score(const ScoreArgs &A, size_t lds, hipStream_t s) {
     auto kern = A.mins ? rg_q4_score_kernel<NQB, GS, true> : rg_q4_score_kernel<NQB, GS, false>;
-    RG_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    if (lds > 64 * 1024) RG_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     const uint32_t tiles = (A.nb + kScoreRows - 1) / kScoreRows, per_cu = std::max<uint32_t>(1, std::min<uint32_t>(2, (uint32_t)(160 * 1024 / lds)));
     hipLaunchKernelGGL(kern, dim3(std::min(tiles, 256u * per_cu)), dim3(kScoreThreads), lds, s, A);
     RG_HIP(hipGetLastError());
@@ -505,8 +505,10 @@ rg_status rg_q4_unpack_dev(const uint8_t *d_codes, uint64_t cstride, const uint1
     if (ostride < dim || (uintptr_t)d_out % 4) return set_error(RG_ERR_ARG, "output rows: stride smaller than dim, or not aligned to their elements");
     OnDevice on(device);
     if (on.st != RG_OK) return on.st;
-    hipLaunchKernelGGL(rg_q4_unpack_kernel, dim3((uint32_t)std::min<uint64_t>(((uint64_t)n * ((dim + 7) / 8) + 255) / 256, 256u * 32u)), dim3(256), 0, (hipStream_t)stream, d_codes, cstride, d_scales, d_mins, sstride, nb, dim, group, d_ids,
-                       n, d_out, ostride);
+    const bool vec = dim % 8 == 0 && ostride % 4 == 0 && (uintptr_t)d_out % 16 == 0;
+    const uint64_t items = (uint64_t)n * (vec ? dim / 8 : dim);
+    hipLaunchKernelGGL(vec ? rg_q4_unpack_kernel<true> : rg_q4_unpack_kernel<false>, dim3((uint32_t)std::min<uint64_t>((items + 255) / 256, 256u * 32u)), dim3(256), 0, (hipStream_t)stream, d_codes, cstride,
+                       d_scales, d_mins, sstride, nb, dim, group, d_ids, n, d_out, ostride);
     RG_HIP(hipGetLastError());
     return RG_OK;
 }

@@ -324,7 +324,7 @@ rg_status make_planes(const void *rows, uint64_t stride, uint32_t n, uint32_t di
 rg_status launch_pass(const Plan &p, const PassArgs &A, hipStream_t s) {
     const uint64_t grid = (uint64_t)p.ntx * p.nslices * A.nsplit;
     if (grid > 0xffffffull) return set_error(RG_ERR_ARG, "softmax over a base: too many rows for one launch");
-    RG_HIP(hipFuncSetAttribute(p.k.kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.k.lds));
+    if (p.k.lds > 64 * 1024) RG_HIP(hipFuncSetAttribute(p.k.kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.k.lds));
     void *args[] = {const_cast<PassArgs *>(&A)};
     RG_HIP(hipLaunchKernel(p.k.kern, dim3((uint32_t)grid), dim3(p.k.threads), args, p.k.lds, s));
     return RG_OK;

@@ -6,7 +6,6 @@
 
 Thin host layer over the C ABI (rg_q4_*, include/rg.h); everything is torch CUDA tensors, enqueued on the current stream.
 """
-import ctypes as C
 from collections import namedtuple
 
 from ._lib import check, lib
@@ -45,8 +44,8 @@ def q4_pack(base_t, group=32, mins=False):
     codes = torch.empty((nb, -(-dim // 8) * 4), dtype=torch.uint8, device=base_t.device)
     both = torch.empty((2 if mins else 1, nb, groups), dtype=torch.float16, device=base_t.device)
     low = both[1] if mins else None
-    check(lib().rg_q4_pack_dev(_ptr(base_t), C.c_uint32(nb), _stride(base_t), C.c_uint32(dim), C.c_int(code), C.c_uint32(group), _ptr(codes),
-                               C.c_uint64(codes.shape[1]), _ptr(both[0]), _ptr(low), C.c_uint64(groups), C.c_int(_device(base_t)), _stream(base_t)))
+    check(lib().rg_q4_pack_dev(_ptr(base_t), nb, _stride(base_t), dim, code, group, _ptr(codes),
+                               codes.shape[1], _ptr(both[0]), _ptr(low), groups, _device(base_t), _stream(base_t)))
     return Q4Base(codes, both[0], low, dim, group)
 
 
@@ -61,9 +60,9 @@ def q4_unpack(packed, ids=None):
         ids = ids.to(torch.int32).contiguous()
     n = nb if ids is None else ids.shape[0]
     out = torch.empty((n, packed.dim), dtype=torch.float32, device=packed.codes.device)
-    check(lib().rg_q4_unpack_dev(_ptr(packed.codes), _stride(packed.codes), _ptr(packed.scales), _ptr(packed.mins), _stride(packed.scales), C.c_uint32(nb),
-                                 C.c_uint32(packed.dim), C.c_uint32(packed.group), _ptr(ids), C.c_uint32(n), _ptr(out), C.c_uint64(packed.dim),
-                                 C.c_int(_device(out)), _stream(out)))
+    check(lib().rg_q4_unpack_dev(_ptr(packed.codes), _stride(packed.codes), _ptr(packed.scales), _ptr(packed.mins), _stride(packed.scales), nb,
+                                 packed.dim, packed.group, _ptr(ids), n, _ptr(out), packed.dim,
+                                 _device(out), _stream(out)))
     return out
 
 
@@ -80,7 +79,7 @@ def q4_score(queries_t, packed, out=None):
         out = torch.empty((nq, nb), dtype=torch.float32, device=queries_t.device)
     elif out.shape != (nq, nb) or out.dtype != torch.float32 or out.device != queries_t.device or (nb > 1 and out.stride(1) != 1) or (nq > 1 and out.stride(0) < nb):
         raise ValueError("out: fp32 rows [%d, %d] on %s are wanted" % (nq, nb, queries_t.device))
-    check(lib().rg_q4_score_dev(_ptr(packed.codes), _stride(packed.codes), _ptr(packed.scales), _ptr(packed.mins), _stride(packed.scales), C.c_uint32(nb),
-                                C.c_uint32(packed.dim), C.c_uint32(packed.group), _ptr(queries_t), C.c_uint32(nq), _stride(queries_t), C.c_int(code),
-                                _ptr(out), _stride(out), C.c_int(_device(out)), _stream(out)))
+    check(lib().rg_q4_score_dev(_ptr(packed.codes), _stride(packed.codes), _ptr(packed.scales), _ptr(packed.mins), _stride(packed.scales), nb,
+                                packed.dim, packed.group, _ptr(queries_t), nq, _stride(queries_t), code,
+                                _ptr(out), _stride(out), _device(out), _stream(out)))
     return out

@@ -33,16 +33,16 @@ def _rows(t, name):
 
 
 def _stride(t):
-    return C.c_uint64(max(t.stride(0), t.shape[1]))     # (a single row's stride may be anything)
+    return max(t.stride(0), t.shape[1])     # (a single row's stride may be anything)
 
 
 def _ptr(t):
-    return C.c_void_p(t.data_ptr() if t is not None else None)
+    return t.data_ptr() if t is not None else None
 
 
 def _stream(t):
     import torch
-    return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+    return torch.cuda.current_stream(t.device).cuda_stream
 
 
 def _device(t):
@@ -65,17 +65,17 @@ def _check_vector(t, n, dtype, like, name):
 
 
 def _targets(targets, n, like):
-    """ids as 32 bits (int64 ids are narrowed: -1 and ids up to 2^32 - 2 keep their meaning)"""
+    """ids as 32 bits (of int64: -1 and ids up to 2^32 - 2 keep their meaning, what 32 bits cannot say becomes 2^32 - 2, which no base has)"""
     import torch
     if targets.dtype == torch.int64:
-        targets = targets.to(torch.int32)
+        targets = targets.clamp(-2, 0xfffffffe).to(torch.int32)
     return _check_vector(targets, n, torch.int32, like, "targets")
 
 
 def workspace(what, nb, nq, dim, dtype_code):
     """rg_softmax_workspace: bytes of scratch of one call"""
     n = C.c_uint64()
-    check(lib().rg_softmax_workspace(C.c_int(what), C.c_uint32(nb), C.c_uint32(nq), C.c_uint32(dim), C.c_int(dtype_code), C.byref(n)))
+    check(lib().rg_softmax_workspace(what, nb, nq, dim, dtype_code, C.byref(n)))
     return n.value
 
 
@@ -96,9 +96,9 @@ def softmax_shard_dev(base_t, queries_t, targets_t, scale, id_base=0, want_mean=
     rest, own, lse, loss = torch.empty((4, nq), dtype=torch.float32, device=base_t.device).unbind(0)
     mean = torch.empty((nq, dim), dtype=torch.float32, device=base_t.device) if want_mean else None
     work, n = _scratch(MEAN if want_mean else STATS, nb, nq, dim, base_t)
-    check(lib().rg_softmax_shard_dev(_ptr(base_t), C.c_uint32(nb), _stride(base_t), _ptr(queries_t), C.c_uint32(nq), _stride(queries_t),
-                                     C.c_uint32(dim), C.c_int(_dtype_code(base_t)), C.c_float(scale), _ptr(targets_t), C.c_uint32(id_base),
-                                     _ptr(rest), _ptr(own), _ptr(lse), _ptr(loss), _ptr(mean), _ptr(work), C.c_uint64(n), C.c_int(_device(base_t)),
+    check(lib().rg_softmax_shard_dev(_ptr(base_t), nb, _stride(base_t), _ptr(queries_t), nq, _stride(queries_t),
+                                     dim, _dtype_code(base_t), scale, _ptr(targets_t), id_base,
+                                     _ptr(rest), _ptr(own), _ptr(lse), _ptr(loss), _ptr(mean), _ptr(work), n, _device(base_t),
                                      _stream(base_t)))
     return rest, own, lse, loss, mean
 
@@ -111,8 +111,8 @@ def softmax_merge_dev(rest_in, own_in, targets_t):
     rest_in, own_in = rest_in.contiguous(), own_in.contiguous()
     targets_t = _targets(targets_t, rest_in.shape[1], rest_in)
     lse, loss = torch.empty((2, rest_in.shape[1]), dtype=torch.float32, device=rest_in.device).unbind(0)
-    check(lib().rg_softmax_merge_dev(_ptr(rest_in), _ptr(own_in), C.c_uint32(rest_in.shape[0]), C.c_uint32(rest_in.shape[1]), _ptr(targets_t),
-                                     _ptr(lse), _ptr(loss), C.c_int(_device(rest_in)), _stream(rest_in)))
+    check(lib().rg_softmax_merge_dev(_ptr(rest_in), _ptr(own_in), rest_in.shape[0], rest_in.shape[1], _ptr(targets_t),
+                                     _ptr(lse), _ptr(loss), _device(rest_in), _stream(rest_in)))
     return lse, loss
 
 
@@ -132,10 +132,10 @@ def softmax_grad_dev(base_t, queries_t, targets_t, scale, lse, loss, weights, re
     dq = torch.empty((nq, dim), dtype=base_t.dtype, device=base_t.device) if want_dq else None
     db = torch.empty((nb, dim), dtype=base_t.dtype, device=base_t.device) if want_db else None
     work, n = _scratch(GRAD, nb if want_db else 0, nq, dim, base_t)
-    check(lib().rg_softmax_grad_dev(_ptr(base_t), C.c_uint32(nb), _stride(base_t), _ptr(queries_t), C.c_uint32(nq), _stride(queries_t),
-                                    C.c_uint32(dim), C.c_int(_dtype_code(base_t)), C.c_float(scale), _ptr(targets_t), C.c_uint32(id_base),
-                                    _ptr(lse), _ptr(loss), _ptr(rest), _ptr(mean), _ptr(weights), _ptr(dq), C.c_uint64(dim), _ptr(db), C.c_uint64(dim),
-                                    _ptr(work), C.c_uint64(n), C.c_int(_device(base_t)), _stream(base_t)))
+    check(lib().rg_softmax_grad_dev(_ptr(base_t), nb, _stride(base_t), _ptr(queries_t), nq, _stride(queries_t),
+                                    dim, _dtype_code(base_t), scale, _ptr(targets_t), id_base,
+                                    _ptr(lse), _ptr(loss), _ptr(rest), _ptr(mean), _ptr(weights), _ptr(dq), dim, _ptr(db), dim,
+                                    _ptr(work), n, _device(base_t), _stream(base_t)))
     return dq, db
 
 
