@@ -33,11 +33,13 @@ __device__ __forceinline__ bool target_here(uint32_t t, uint32_t id_base, uint32
 // log(1 + e^d) without overflow: loss of a target d below the others' log sum
 __device__ __forceinline__ float softplus(float d) { return d > 15.0f ? d + log1pf(expf(-d)) : log1pf(expf(d)); }
 
-// joins the slots of a query: rest, target logit, lse, loss, mean of the others.  One workgroup per query.
+// joins the slots of a query: rest, target logit, lse, loss, mean of the others.  One workgroup per query, or, where queries are few, per query
+// and kJoinDims of the mean's elements; with many slots, four groups of lanes share them.
+constexpr uint32_t kJoinDims = 64, kJoinSlots = 16;
 __global__ void __launch_bounds__(256) rg_softmax_join_kernel(const float4 *ml, const float *o, uint32_t opitch, uint32_t nslots, uint32_t nq, uint32_t dim, uint32_t nb, uint32_t id_base, const float *own2,
                                                               const uint32_t *targets, float *rest, float *own, float *lse, float *loss, float *mean) {
     const uint32_t i = blockIdx.x, tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
-    __shared__ float red[8];
+    __shared__ float red[8], weight[256], part[256];
     float M = kNothing, Mo = kNothing;
     for (uint32_t s = tid; s < nslots; s += 256) {
         const float4 v = ml[(size_t)s * nq + i];
@@ -63,7 +65,7 @@ __global__ void __launch_bounds__(256) rg_softmax_join_kernel(const float4 *ml, 
     if (lane == 0) red[wave] = l;
     __syncthreads();
     l = red[0] + red[1] + red[2] + red[3];
-    if (tid == 0) {
+    if (tid == 0 && blockIdx.y == 0) {
         const uint32_t t = targets[i];
         const bool here = target_here(t, id_base, nb);
         const float r = none ? -INFINITY : (M + log2f(l)) * kLn2;
@@ -76,10 +78,25 @@ __global__ void __launch_bounds__(256) rg_softmax_join_kernel(const float4 *ml, 
     }
     if (mean) {
         const float f = none ? 0.0f : exp2f(Mo - M) / l;
-        for (uint32_t k = tid; k < dim; k += 256) {
+        const uint32_t groups = nslots < kJoinSlots ? 1 : 4, width = 256 / groups, group = tid / width;
+        for (uint32_t k0 = blockIdx.y * width; k0 < dim; k0 += gridDim.y * width) {
+            const uint32_t k = k0 + tid % width;
             float s = 0.0f;
-            for (uint32_t e = 0; e < nslots; ++e) s = fmaf(exp2f(ml[(size_t)e * nq + i].z - Mo), o[((size_t)e * nq + i) * opitch + k], s);
-            mean[(size_t)i * dim + k] = s * f;
+            for (uint32_t e0 = 0; e0 < nslots; e0 += 256) {
+                __syncthreads();
+                if (e0 + tid < nslots) weight[tid] = exp2f(ml[(size_t)(e0 + tid) * nq + i].z - Mo);
+                __syncthreads();
+                const uint32_t n = min(256u, nslots - e0);
+                if (k < dim)
+#pragma unroll 8
+                    for (uint32_t e = group; e < n; e += groups) s = fmaf(weight[e], o[((size_t)(e0 + e) * nq + i) * opitch + k], s);
+            }
+            if (groups > 1) {
+                part[tid] = s;
+                __syncthreads();
+                if (group == 0) s = (part[tid] + part[width + tid]) + (part[2 * width + tid] + part[3 * width + tid]);
+            }
+            if (group == 0 && k < dim) mean[(size_t)i * dim + k] = s * f;
         }
     }
 }
@@ -225,34 +242,6 @@ int steps_of(uint32_t dim) {
 // at most this many bytes of planes at a time: a large base is streamed piece by piece
 constexpr uint64_t kPieceBytes = 1ull << 30;
 
-// how a pass is cut: into pieces of y that are made into planes one after another (planes), each split into slots whose partial results are
-// joined at the end -- as many as give every workgroup place of the device the same work, of at least four tiles
-struct Plan {
-    SoftmaxKernel k;
-    int ks;
-    bool thin, planes;
-    uint32_t nx, ny, ntx, nslices, piece, nslots;
-    uint64_t row_bytes;               // of a row of planes
-    struct Cut {
-        uint32_t nsplit, rows;
-    };
-    Cut cut(uint32_t rows) const {
-        const uint64_t nt = (uint64_t)ntx * nslices, places = 256ull * std::min<uint32_t>(k.wps * 256 / k.threads, 160 * 1024 / k.lds);     // (256 CUs)
-        const uint32_t most = std::max(1u, rows / 128);
-        uint32_t best = 1;
-        double best_use = 0;
-        for (uint32_t n = 1; n <= most && n * nt <= 2 * places + nt; ++n) {
-            const uint64_t rounds = (n * nt + places - 1) / places;
-            const double use = (double)(n * nt) / (double)(rounds * places) - 0.01 * (double)(rounds - 1);
-            if (use > best_use * 1.02) { best_use = use; best = n; }
-        }
-        Cut c;
-        c.rows = up32((std::max(rows, 1u) + best - 1) / best);
-        c.nsplit = std::max(1u, (rows + c.rows - 1) / c.rows);
-        return c;
-    }
-};
-
 SoftmaxKernel kernel_of(int dtype, int mode, bool thin, int ks) {
     typedef SoftmaxKernel (*Pick)(int);
     static const Pick wide[3][3] = {{softmax_wide_f32_stats, softmax_wide_f32_mean, softmax_wide_f32_rows},
@@ -261,6 +250,57 @@ SoftmaxKernel kernel_of(int dtype, int mode, bool thin, int ks) {
     static const Pick few[3][2] = {{softmax_thin_f32_stats, softmax_thin_f32_mean}, {softmax_thin_f16_stats, softmax_thin_f16_mean}, {softmax_thin_bf16_stats, softmax_thin_bf16_mean}};
     return thin ? few[dtype][mode](ks) : wide[dtype][mode](ks);
 }
+
+// how a pass is cut: into pieces of y that are made into planes one after another (planes), each split into slots whose partial results are
+// joined at the end.  More slots fill the workgroup places of the device, and each costs the writing and reading of its results: the cheapest
+// number is taken, in bytes of the device's traffic, one of which it moves while its matrix cores do kOpsPerByte operations of a pass (measured:
+// 600 Top/s of the 16-bit passes, 4 TB/s).  333 fp16 queries on 70001 rows of 93 dims: 3 slots, which leave fewer places empty, took
+// 80 us + 29 us to join for the gradient of the rows, 1 slot 58 us.
+// With and without the mean, a call is cut alike (for the sum of both costs), so that both give the same loss.
+constexpr double kOpsPerByte = 150;
+struct Use {                          // of the device by a kernel
+    uint64_t nt, places;              // workgroups of a slot; workgroups that run at once
+    double row_cost;                  // bytes of a row y, were all places used
+    double busy(uint32_t rows, uint32_t n) const {
+        const uint64_t rounds = (n * nt + places - 1) / places;
+        return row_cost * rows * (double)(rounds * places) / ((double)nt * n);
+    }
+};
+struct Plan {
+    SoftmaxKernel k;
+    int ks;
+    bool thin, planes;
+    uint32_t nx, ny, ntx, nslices, piece, nslots;
+    uint64_t row_bytes;               // of a row of planes
+    Use use[2];
+    int nuse;
+    double slot_cost;                 // bytes of a slot
+    bool free_slot;                   // a single slot needs no joining
+    struct Cut {
+        uint32_t nsplit, rows;
+    };
+    Cut cut(uint32_t rows) const {
+        const uint32_t most = std::max(1u, rows / 32);
+        uint32_t best = 1;
+        double least = HUGE_VAL;
+        auto look = [&](uint64_t n_) {
+            const uint32_t n = (uint32_t)std::clamp<uint64_t>(n_, 1, most);
+            double cost = n == 1 && free_slot ? 0.0 : nuse * n * slot_cost;
+            for (int u = 0; u < nuse; ++u) cost += use[u].busy(rows, n);
+            if (cost < least || (cost == least && n < best)) { least = cost; best = n; }
+        };
+        look(1);
+        for (int u = 0; u < nuse; ++u) {
+            const Use &U = use[u];
+            look((uint64_t)std::sqrt(U.row_cost * rows * (double)U.places / ((double)U.nt * slot_cost)));     // where one round does: the least of busy / n + n slot_cost
+            for (uint64_t first = (U.nt + U.places - 1) / U.places, rounds = first; rounds <= first + 3; ++rounds) look(rounds * U.places / U.nt);     // the most slots of so many rounds
+        }
+        Cut c;
+        c.rows = up32((std::max(rows, 1u) + best - 1) / best);
+        c.nsplit = std::max(1u, (rows + c.rows - 1) / c.rows);
+        return c;
+    }
+};
 
 // direct: the streamed rows can be read where they lie (16-bit rows of whole 16-byte chunks, 16-byte aligned)
 Plan plan_of(int dtype, int mode, uint32_t dim, uint32_t nx, uint32_t ny, bool direct) {
@@ -274,6 +314,18 @@ Plan plan_of(int dtype, int mode, uint32_t dim, uint32_t nx, uint32_t ny, bool d
     p.ntx = std::max(1u, (uint32_t)(((uint64_t)nx + p.k.xt - 1) / p.k.xt));
     p.nslices = mode == kStats ? 1 : (dim + 16 * p.k.ob - 1) / (16 * p.k.ob);
     p.row_bytes = (uint64_t)(dtype == RG_DTYPE_F32 ? 2 : 1) * p.ks * 64;
+    p.nuse = 0;
+    for (int m = mode == kRows ? kRows : kStats; m <= (mode == kRows ? kRows : kMean); ++m) {
+        const SoftmaxKernel k = kernel_of(dtype, m, p.thin, p.ks);
+        const uint64_t ntx = std::max<uint64_t>(1, ((uint64_t)nx + k.xt - 1) / k.xt), nslices = m == kStats ? 1 : (dim + 16 * k.ob - 1) / (16 * k.ob);
+        Use &u = p.use[p.nuse++];
+        u.nt = ntx * nslices;
+        u.places = 256ull * std::min<uint32_t>(k.wps * 256 / k.threads, 160 * 1024 / k.lds);     // (256 CUs)
+        const double ops = 2.0 * (dtype == RG_DTYPE_F32 ? 3 : 1) * (double)(u.nt * k.xt) * (32.0 * p.ks + (m == kStats ? 0.0 : 16.0 * k.ob));     // of a row y
+        u.row_cost = p.thin ? (double)dim * elem_bytes(dtype) * (double)nslices : ops / kOpsPerByte;
+    }
+    p.slot_cost = 8.0 * opitch_of(dim) * std::max(nx, 1u);
+    p.free_slot = mode == kRows;
     p.piece = ny;
     if (p.planes && mode != kRows) p.piece = (uint32_t)std::min<uint64_t>(ny, kPieceBytes / p.row_bytes / 32 * 32);
     p.nslots = 0;
@@ -323,7 +375,7 @@ rg_status make_planes(const void *rows, uint64_t stride, uint32_t n, uint32_t di
 
 rg_status launch_pass(const Plan &p, const PassArgs &A, hipStream_t s) {
     const uint64_t grid = (uint64_t)p.ntx * p.nslices * A.nsplit;
-    if (grid > 0xffffffull) return set_error(RG_ERR_ARG, "softmax over a base: too many rows for one launch");
+    if (grid * p.k.threads > 0xffffffffull) return set_error(RG_ERR_ARG, "softmax over a base: too many rows for one launch");
     if (p.k.lds > 64 * 1024) RG_HIP(hipFuncSetAttribute(p.k.kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.k.lds));
     void *args[] = {const_cast<PassArgs *>(&A)};
     RG_HIP(hipLaunchKernel(p.k.kern, dim3((uint32_t)grid), dim3(p.k.threads), args, p.k.lds, s));
@@ -333,7 +385,7 @@ rg_status launch_pass(const Plan &p, const PassArgs &A, hipStream_t s) {
 rg_status check_shapes(uint32_t nb, uint32_t nq, uint32_t dim, int dtype) {
     if (!known_dtype(dtype)) return set_error(RG_ERR_ARG, "unknown dtype");
     if (dim == 0 || dim > kMaxDim) return set_error(RG_ERR_ARG, "softmax over a base: dim must be in [1, 1024]");
-    if (nb > 0x7fffffffu || nq > 0x7fffffffu) return set_error(RG_ERR_ARG, "softmax over a base: at most 2^31 - 1 rows and queries");
+    if (nb > 0x7fffffffu || nq > 0xffffffu) return set_error(RG_ERR_ARG, "softmax over a base: at most 2^31 - 1 rows and 2^24 - 1 queries");     // (a launch holds 2^32 - 1 threads)
     return RG_OK;
 }
 rg_status check_rows(const void *p, uint32_t n, uint64_t stride, uint32_t dim, int dtype, const char *name) {
@@ -404,7 +456,7 @@ rg_status shard(const Call &c, float *rest, float *own, float *lse, float *loss,
         if (st != RG_OK) return st;
         slot += cut.nsplit;
     }
-    hipLaunchKernelGGL(rg_softmax_join_kernel, dim3(c.nq), dim3(256), 0, c.s, ml, o, A.opitch, p.nslots, c.nq, c.dim, c.nb, c.id_base, A.own2, c.targets, rest, own, lse, loss, mean);
+    hipLaunchKernelGGL(rg_softmax_join_kernel, dim3(c.nq, mean ? std::clamp(4096u / c.nq, 1u, (c.dim + kJoinDims - 1) / kJoinDims) : 1), dim3(256), 0, c.s, ml, o, A.opitch, p.nslots, c.nq, c.dim, c.nb, c.id_base, A.own2, c.targets, rest, own, lse, loss, mean);
     RG_HIP(hipGetLastError());
     return RG_OK;
 }
