@@ -74,7 +74,6 @@ typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 template <int DT> struct Frag { typedef half8 V; };
 template <> struct Frag<RG_DTYPE_BF16> { typedef bf8 V; };
@@ -148,17 +147,21 @@ __device__ __forceinline__ void split8(Chunk<RG_DTYPE_F32> c, float top, float s
     }
 }
 
-// stationary operands of row x: lane (n, g) holds elements 32 ks + 8 g .. + 7; returns what its logits are multiplied by
+// stationary operands of row x: lane (n, g) holds elements 32 ks + 8 g .. + 7 of part kq of nkq of the row; returns what its logits are
+// multiplied by
 template <int DT, int KS, int NP>
-__device__ __forceinline__ float load_stationary(const PassArgs &A, uint32_t x, uint32_t g, bool vec, typename Frag<DT>::V (&X)[KS][NP]) {
+__device__ __forceinline__ float load_stationary(const PassArgs &A, uint32_t x, uint32_t g, bool vec, typename Frag<DT>::V (&X)[KS][NP], uint32_t kq = 0, uint32_t nkq = 1) {
     const char *row = static_cast<const char *>(A.x) + (size_t)x * A.xstride * sizeof(typename Elem<DT>::T);
-    const uint32_t dim = x < A.nx ? A.dim : 0;
+    const uint32_t dim = x < A.nx ? A.dim : 0, k0 = 32 * KS * kq + 8 * g;
     if constexpr (DT == RG_DTYPE_F32) {
         uint32_t m = 0;
         Chunk<DT> c[KS];
+        for (uint32_t q = 1; q < nkq; ++q)          // the other parts count for the largest element
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) m = max(m, __float_as_uint(absmax(load_chunk<DT>(row, 32 * KS * ((kq + q) % nkq) + 32 * ks + 8 * g, dim, vec))));
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            c[ks] = load_chunk<DT>(row, 32 * ks + 8 * g, dim, vec);
+            c[ks] = load_chunk<DT>(row, k0 + 32 * ks, dim, vec);
             m = max(m, __float_as_uint(absmax(c[ks])));
         }
         m = max(m, (uint32_t)__shfl_xor((int)m, 16));
@@ -170,7 +173,7 @@ __device__ __forceinline__ float load_stationary(const PassArgs &A, uint32_t x, 
         return A.k * row_factor(top, e);
     } else {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) X[ks][0] = __builtin_bit_cast(typename Frag<DT>::V, load_chunk<DT>(row, 32 * ks + 8 * g, dim, vec).v);
+        for (int ks = 0; ks < KS; ++ks) X[ks][0] = __builtin_bit_cast(typename Frag<DT>::V, load_chunk<DT>(row, k0 + 32 * ks, dim, vec).v);
         return A.k;
     }
 }

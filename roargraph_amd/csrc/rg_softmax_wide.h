@@ -17,21 +17,22 @@
 
 namespace rg {
 
+// A workgroup of eight waves, two per SIMD.  KQ waves share each of its 8 / KQ groups of 16 NX rows x, a KQ-th of the dimensions each.
 struct WideChoice {
-    int nx, waves, wps;
-    bool loop3;
+    int nx, kq;
 };
+// The sums of a product over the dimensions are made in this many parts, whichever waves make them: the logits of all modes have the same bits.
+constexpr int softmax_parts(int dt, int ks) { return dt == RG_DTYPE_F32 ? (ks <= 8 ? 1 : ks <= 16 ? 2 : 4) : ks <= 16 ? 1 : 4; }
 constexpr WideChoice softmax_wide_cfg(int dt, int ks, int mode) {
     const bool f32 = dt == RG_DTYPE_F32;
 #ifdef RG_WIDE_CFG
     return RG_WIDE_CFG;
 #else
-    if (mode == kStats) {
-        if (f32) return ks <= 4 ? WideChoice{3, 8, 2, false} : ks <= 7 ? WideChoice{2, 8, 2, false} : ks <= 16 ? WideChoice{1, 8, 2, false} : WideChoice{1, 4, 1, false};
-        return ks <= 7 ? WideChoice{4, 8, 2, false} : ks <= 8 ? WideChoice{3, 8, 2, false} : ks <= 16 ? WideChoice{2, 8, 2, false} : WideChoice{1, 8, 2, false};
-    }
-    if (f32) return ks <= 4 ? WideChoice{2, 8, 2, false} : ks <= 8 ? WideChoice{1, 8, 2, false} : WideChoice{1, 4, 1, false};
-    return ks <= 2 ? WideChoice{4, 8, 2, false} : ks <= 4 ? WideChoice{3, 8, 2, false} : ks <= 7 || (ks == 8 && mode == kMean) ? WideChoice{2, 8, 2, false} : ks <= 16 ? WideChoice{1, 8, 2, false} : WideChoice{1, 4, 1, false};
+    if (mode == kStats && f32) return ks <= 4 ? WideChoice{3, 1} : ks <= 7 ? WideChoice{2, 1} : ks <= 16 ? WideChoice{1, 1} : ks <= 24 ? WideChoice{2, 4} : WideChoice{1, 4};
+    if (mode == kStats) return {ks <= 7 ? 4 : ks <= 8 ? 3 : ks <= 16 ? 2 : 1, 1};
+    const int kq = softmax_parts(dt, ks);
+    if (f32) return {ks <= 4 ? 2 : 1, kq};
+    return {ks <= 2 ? 4 : ks <= 4 ? 3 : ks <= 7 || (ks == 8 && mode == kMean) ? 2 : ks <= 16 ? 1 : ks <= 24 || mode == kMean ? 2 : 1, kq};
 #endif
 }
 
@@ -39,21 +40,23 @@ template <int DT, int KS, int MODE>
 struct WideCfg {
     static constexpr bool F32 = DT == RG_DTYPE_F32;
     static constexpr int NP = F32 ? 2 : 1;
-    static constexpr int OB = KS == 7 ? 13 : F32 && KS == 32 ? 32 : 2 * KS;
-    static constexpr int NX = softmax_wide_cfg(DT, KS, MODE).nx, WAVES = softmax_wide_cfg(DT, KS, MODE).waves, WPS = softmax_wide_cfg(DT, KS, MODE).wps;
-    static constexpr bool LOOP3 = softmax_wide_cfg(DT, KS, MODE).loop3;
-    static constexpr int NT = 64 * WAVES;
-    static constexpr int XT = 16 * NX * WAVES;
+    static constexpr int NX = softmax_wide_cfg(DT, KS, MODE).nx, KQ = softmax_wide_cfg(DT, KS, MODE).kq;
+    static constexpr int WAVES = 8, WPS = 2, NT = 64 * WAVES;
+    static constexpr int KW = KS / KQ, OW = KS == 7 ? 13 : 2 * KW;   // steps of the first product and output blocks of a wave
+    static constexpr int OB = KQ * OW;
+    static constexpr int XT = 16 * NX * WAVES / KQ;
     static constexpr int TY = 32;
     static constexpr int PITCH = (KS * 64 + 255) / 256 * 256;
     static constexpr int PLANE = TY * PITCH;
     static constexpr int BUF = NP * PLANE;
     static constexpr bool INFO = F32 || MODE == kRows;
     static constexpr int NI = BUF / (16 * NT) + (INFO ? 1 : 0);      // loads of a tile, per wave
-    static constexpr int FIT = 160 * 1024 * WAVES / (4 * WPS) / (BUF + (INFO ? TY * 16 : 0));
+    static constexpr int PARTS = softmax_parts(DT, KS);
+    static constexpr int EX = KQ > 1 ? WAVES * NX * 2 * 1024 : 0;    // where the waves of a group add up their products
+    static constexpr int FIT = (160 * 1024 - EX) / (BUF + (INFO ? TY * 16 : 0));
     static constexpr int NBUF = FIT > 8 ? 8 : FIT;
-    static constexpr bool PIPE = LOOP3 && NBUF >= 6;
-    static constexpr int LDS = NBUF * (BUF + (INFO ? TY * 16 : 0));
+    static constexpr int LDS = NBUF * (BUF + (INFO ? TY * 16 : 0)) + EX;
+    static_assert((KQ == 1 || KQ == PARTS) && KS % PARTS == 0 && NBUF >= 1, "parts are whole steps, and a tile fits");
 };
 
 // 16 bytes a lane from base + off to LDS at `to` + 16 * lane.  Written as assembly because the compiler, which cannot tell the ring's buffers
@@ -68,7 +71,7 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
     typedef WideCfg<DT, KS, MODE> C;
     typedef typename Elem<DT>::T T;
     typedef typename Frag<DT>::V V;
-    constexpr int NP = C::NP, NX = C::NX, OB = C::OB, PITCH = C::PITCH, NBUF = C::NBUF;
+    constexpr int NP = C::NP, NX = C::NX, KQ = C::KQ, KW = C::KW, OW = C::OW, PITCH = C::PITCH, NBUF = C::NBUF;
     constexpr bool F32 = C::F32, INFO = C::INFO;
     constexpr bool TWO = F32 && MODE == kMean;      // weights of O carry the rows' scales: the sum l has a reference of its own
     constexpr bool BIAS = TWO || MODE == kRows;
@@ -78,13 +81,12 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
     extern __shared__ char lds[];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
     const uint32_t ntx = (A.nx + C::XT - 1) / C::XT;
-    uint32_t b = xcd_block(blockIdx.x, gridDim.x);
+    const uint32_t b = xcd_block(blockIdx.x, gridDim.x);
     const uint32_t xt = b % ntx;
-    b /= ntx;
-    const uint32_t slice = MODE == kStats ? 0 : b % A.nslices, split = MODE == kStats ? b : b / A.nslices;
+    const uint32_t split = b / ntx, kq = wave % KQ;
     const uint32_t ybeg = min(A.ny, split * A.rows_per_split), yend = min(A.ny, ybeg + A.rows_per_split);
     const uint32_t ntiles = (yend - ybeg + 31) / 32;
-    const uint32_t x0 = xt * C::XT + wave * 16 * NX;
+    const uint32_t x0 = xt * C::XT + wave / KQ * 16 * NX;
     const bool live = x0 < A.nx;
 
     // tile t of this piece into its buffer: 16-byte slot q of a plane of the tile is (row, slot of the row).  Rows behind the last one are
@@ -92,14 +94,16 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
     constexpr int SR = PITCH / 16, PER = 32 * SR / C::NT;
     const uint32_t nchunks = A.ydim / 8, ystep = (uint32_t)A.ystride * 2;           // (32 rows' bytes fit 32 bits: the host's rule)
     const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-    auto offset = [&](int i, uint32_t rows) {
-        const uint32_t q = i * C::NT + tid, r = q / SR, slot = q % SR;
+    auto offset = [&](int i, uint32_t rows, uint32_t thread) {
+        const uint32_t q = i * C::NT + thread, r = q / SR, slot = q % SR;
         const uint32_t c = (slot & ~15u) | ((slot & 15) ^ swizzle(r));
         return c < nchunks ? min(r, rows - 1) * ystep + c * 16 : c < 4 * KS ? 0xffffffffu : min(r, rows - 1) * ystep;
     };
-    uint32_t off[PER];
+    constexpr bool KEPT = PER <= 6;                 // (more offsets than that are made anew for every tile: the registers are worth more)
+    uint32_t off[KEPT ? PER : 1];
+    if (KEPT)
 #pragma unroll
-    for (int i = 0; i < PER; ++i) off[i] = offset(i, 32);
+        for (int i = 0; i < PER; ++i) off[i] = offset(i, 32, tid);
     const bool holes = nchunks < 4 * KS;
     if (holes) {                                    // what no load writes
         for (uint32_t i = tid; i < NBUF * C::BUF / 16; i += C::NT) reinterpret_cast<u32x4 *>(lds)[i] = u32x4{0, 0, 0, 0};
@@ -108,14 +112,16 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
     auto load = [&](uint32_t t) {
         const uint32_t buf = t % NBUF, y0 = ybeg + 32 * t, to = __builtin_amdgcn_readfirstlane(ring + buf * C::BUF + wave * 1024);
         const char *first = static_cast<const char *>(A.y) + (size_t)y0 * A.ystride * 2;
-        const uint32_t rows = yend - y0;
+        const uint32_t rows = min(yend - y0, 32u);
+        uint32_t thread = tid;
+        if (!KEPT) asm("" : "+v"(thread));
 #pragma unroll
-        for (int p = 0; p < NP; ++p)
+        for (int i = 0; i < PER; ++i) {
+            const uint32_t o = !KEPT || rows < 32 ? offset(i, rows, thread) : off[i];
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const uint32_t o = rows < 32 ? offset(i, rows) : off[i];
+            for (int p = 0; p < NP; ++p)
                 if (!holes || o != 0xffffffffu) load_lds16(first + p * (KS * 64), o, to + (p * PER + i) * (16 * C::NT));
-            }
+        }
         constexpr uint32_t each = 32 / C::WAVES;    // lanes of a wave that load the tile's 512 bytes of info
         if (INFO && lane < each) load_lds16(A.yinfo + (size_t)y0 * 4 + wave * each * 4, lane * 16, __builtin_amdgcn_readfirstlane(ring + NBUF * C::BUF + buf * 512 + wave * each * 16));
     };
@@ -133,14 +139,14 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
     if (ntiles)
         for (uint32_t t = 0; t + 1 < (NBUF > 1 ? NBUF : 2) && t < ntiles; ++t) load(t);
 
-    V X[NX][KS][NP];
+    V X[NX][KW][NP];
     float kx[NX];
     uint32_t target[NX];
     const bool xvec = ((uintptr_t)A.x | A.xstride * sizeof(T)) % 16 == 0;
 #pragma unroll
     for (int j = 0; j < NX; ++j) {
         const uint32_t x = x0 + j * 16 + n;
-        kx[j] = load_stationary<DT, KS>(A, x, g, xvec, X[j]);
+        kx[j] = load_stationary<DT, KW>(A, x, g, xvec, X[j], kq, KQ);
         target[j] = kNoTarget;
         if (MODE != kRows && x < A.nx) {
             const uint32_t tg = A.targets[x];
@@ -148,7 +154,7 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
         }
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);             // the compiler's own loads (vmcnt(0)): none of its waits is left for the loop
-    f32x4 O[MODE == kStats ? 1 : OB][NX];
+    f32x4 O[MODE == kStats ? 1 : OW][NX];
     float M[NX], l[NX], Ml[NX];
 #pragma unroll
     for (int j = 0; j < NX; ++j) {
@@ -157,7 +163,7 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
         l[j] = 0.0f;
         if (MODE != kStats)
 #pragma unroll
-            for (int ob = 0; ob < OB; ++ob) O[ob][j] = f32x4{0, 0, 0, 0};
+            for (int ob = 0; ob < OW; ++ob) O[ob][j] = f32x4{0, 0, 0, 0};
     }
 
     // LDS operands are asked for AHEAD steps before the products that take them, and the compiler is kept from moving the reads back
@@ -169,14 +175,15 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
         asm("" : "+v"(a));
         return a;
     };
-    const uint32_t sw = swizzle(n);
-    uint32_t first_at[4], second_at[8];             // what a lane reads of a tile: chunks 4 ks + g, and dims 4 (n % 4) of rows 4 g + n / 4 (they repeat every 256 bytes)
+    // what a lane reads of a tile: chunks 4 ks + g of row n, and dims 4 (n % 4) of each block of rows 4 g + n / 4 (they repeat every 256 bytes)
+    uint32_t first_at[4], second_at[8];
+    auto chunk_at = [&](uint32_t row, uint32_t c) { return ring + row * PITCH + (c >> 4 << 8) + (((c & 15) ^ swizzle(row)) << 4); };
 #pragma unroll
-    for (int i = 0; i < 4; ++i) first_at[i] = ring + n * PITCH + (((4 * i + g) ^ sw) << 4);
+    for (int i = 0; i < 4; ++i) first_at[i] = chunk_at(n, 4 * (kq * KW + i) + g);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) second_at[i] = ring + (4 * g + (n >> 2)) * PITCH + (((2 * i + (n >> 1 & 1)) ^ swizzle(4 * g + (n >> 2))) << 4) + (n & 1) * 8;
+    for (int i = 0; i < 8; ++i) second_at[i] = chunk_at(4 * g + (n >> 2), 2 * (kq * OW + i) + (n >> 1 & 1)) + (n & 1) * 8;
     auto first_product = [&](uint32_t buf, f32x4 (&S)[NX][2]) {
-        constexpr int AHEAD = C::WPS == 1 ? 2 : 1;
+        constexpr int AHEAD = 1;
         uint32_t at[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) at[i] = lds_at(first_at[i] + buf * C::BUF);
@@ -189,12 +196,23 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
         };
 #pragma unroll
         for (int j = 0; j < NX; ++j) S[j][0] = S[j][1] = f32x4{0, 0, 0, 0};
+        constexpr int PART = KQ == 1 ? KS / C::PARTS : KW;      // steps of a part
+        f32x4 sum[NX][2];
 #pragma unroll
-        for (int ks = 0; ks < AHEAD && ks < KS; ++ks) read(ks);
+        for (int ks = 0; ks < AHEAD && ks < KW; ++ks) read(ks);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            if (ks + AHEAD < KS) read(ks + AHEAD);
+        for (int ks = 0; ks < KW; ++ks) {
+            if (ks + AHEAD < KW) read(ks + AHEAD);
             keep_order();
+            if (ks % PART == 0 && ks) {
+#pragma unroll
+                for (int j = 0; j < NX; ++j)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        sum[j][h] = ks == PART ? S[j][h] : sum[j][h] + S[j][h];
+                        S[j][h] = f32x4{0, 0, 0, 0};
+                    }
+            }
             const V(&v)[2][NP] = a[ks % (AHEAD + 1)];
             if constexpr (F32) {
 #pragma unroll
@@ -212,14 +230,37 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
                 for (int j = 0; j < NX; ++j) S[j][h] = mma(v[h][0], X[j][ks][0], S[j][h]);
             keep_order();
         }
+        if (PART < KW)
+#pragma unroll
+            for (int j = 0; j < NX; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) S[j][h] = sum[j][h] + S[j][h];
+    };
+    // the products of the waves of a group, added up in one order by all of them
+    f32x4 *const ex = reinterpret_cast<f32x4 *>(lds + C::LDS - C::EX);
+    auto part_out = [&](const f32x4 (&S)[NX][2]) {
+#pragma unroll
+        for (int j = 0; j < NX; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) ex[((wave * NX + j) * 2 + h) * 64 + lane] = S[j][h];
+    };
+    auto parts_in = [&](f32x4 (&S)[NX][2]) {
+#pragma unroll
+        for (int j = 0; j < NX; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                S[j][h] = ex[((wave / KQ * KQ * NX + j) * 2 + h) * 64 + lane];
+#pragma unroll
+                for (int q = 1; q < KQ; ++q) S[j][h] += ex[(((wave / KQ * KQ + q) * NX + j) * 2 + h) * 64 + lane];
+            }
     };
     auto second_product = [&](uint32_t buf, const V (&W)[NX][NP]) {
         if constexpr (MODE != kStats) {
             typedef __attribute__((address_space(3))) s16x4 *tr_ptr;
-            constexpr int AHEAD = C::WPS == 1 && !F32 ? 3 : 2;
+            constexpr int AHEAD = 2;
             uint32_t at[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) at[i] = lds_at(second_at[i] + buf * C::BUF + slice * (OB / 8 * 256));    // (more than one slice: OB is a multiple of 8)
+            for (int i = 0; i < 8; ++i) at[i] = lds_at(second_at[i] + buf * C::BUF);
             s16x4 a[AHEAD + 1][NP][2];
             auto read = [&](int ob) {
 #pragma unroll
@@ -228,10 +269,10 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
                     for (int h = 0; h < 2; ++h) a[ob % (AHEAD + 1)][p][h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at[ob % 8] + (uint32_t)(ob / 8 * 256 + p * C::PLANE + h * 16 * PITCH)));
             };
 #pragma unroll
-            for (int ob = 0; ob < AHEAD && ob < OB; ++ob) read(ob);
+            for (int ob = 0; ob < AHEAD && ob < OW; ++ob) read(ob);
 #pragma unroll
-            for (int ob = 0; ob < OB; ++ob) {
-                if (ob + AHEAD < OB) read(ob + AHEAD);
+            for (int ob = 0; ob < OW; ++ob) {
+                if (ob + AHEAD < OW) read(ob + AHEAD);
                 keep_order();
                 V v[NP];
 #pragma unroll
@@ -286,7 +327,7 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
                     const float f = INFO ? kx[j] * info(k, kFactor, r) : kx[j];
                     bool dead = k.y0 + r >= yend;
                     if (MODE != kRows && k.y0 + r == target[j]) {
-                        if (slice == 0) A.own2[x] = S[j][h][i] * f;
+                        if (kq == 0) A.own2[x] = S[j][h][i] * f;
                         dead = true;
                     }
                     if (MODE == kRows && __float_as_uint(info(k, kTarget, r)) == x) {
@@ -384,7 +425,7 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
             }
         }
     };
-    // the weights of a tile, in two halves; `pending`: what has to be added to O before it is rescaled
+    // the weights of a tile, in two halves
     float pl[TWO ? NX : 1][2][4];
     auto weigh_first = [&](const Tile &k, const f32x4 (&S)[NX][2], float (&p)[NX][2][4]) {
         if constexpr (TWO) logits(k, S, false, Ml, pl);
@@ -393,21 +434,20 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
         if constexpr (TWO) o |= over(pl);
         return !NOREF && __any(o);
     };
-    auto move_all = [&](const Tile &k, const f32x4 (&S)[NX][2], auto &&pending, float (&p)[NX][2][4]) {
+    auto move_all = [&](const Tile &k, const f32x4 (&S)[NX][2], float (&p)[NX][2][4]) {
         float old[NX];
         if constexpr (TWO) {
             move(k, S, false, Ml, pl, old);
 #pragma unroll
             for (int j = 0; j < NX; ++j) l[j] *= old[j];
         }
-        pending();
         move(k, S, BIAS, M, p, old);
 #pragma unroll
         for (int j = 0; j < NX; ++j) {
             if (!TWO) l[j] *= old[j];
             if (MODE != kStats)
 #pragma unroll
-                for (int ob = 0; ob < OB; ++ob) O[ob][j] *= old[j];
+                for (int ob = 0; ob < OW; ++ob) O[ob][j] *= old[j];
         }
     };
     auto weigh_second = [&](float (&p)[NX][2][4]) {
@@ -422,7 +462,7 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
     };
 
     if (ntiles) {
-        if constexpr (MODE == kStats && NBUF >= 3) {
+        if constexpr (MODE == kStats && NBUF >= 3 && KQ == 1) {
             // first product of the next tile beside the weights of this one; tile t + NBUF - 1 takes the place of tile t - 1
             f32x4 S[NX][2], next[NX][2];
             arrived(0, std::integral_constant<int, NBUF - 2>{});
@@ -435,49 +475,12 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
                     const Tile k = look(t);
                     if (k.rare) special(k, S);
                     first_product((t + 1) % NBUF, next);                       // (behind the last tile: of old rows, for nobody)
-                    if (weigh_first(k, S, p)) move_all(k, S, [] {}, p);
+                    if (weigh_first(k, S, p)) move_all(k, S, p);
                     weigh_second(p);
 #pragma unroll
                     for (int j = 0; j < NX; ++j) { S[j][0] = next[j][0]; S[j][1] = next[j][1]; }
                 }
             }
-        } else if constexpr (C::PIPE) {
-            // tile t + NBUF - 2 takes the place of tile t - 2
-            f32x4 S[NX][2], next[NX][2];
-            V W[NX][NP];
-#pragma unroll
-            for (int j = 0; j < NX; ++j)
-#pragma unroll
-                for (int p = 0; p < NP; ++p) W[j][p] = __builtin_bit_cast(V, u32x4{0, 0, 0, 0});
-            arrived(0, std::integral_constant<int, NBUF - 2>{});
-            if (live) first_product(0, S);
-            for (uint32_t t = 0; t < ntiles; ++t) {
-                arrived(t + 1, std::integral_constant<int, NBUF - 4>{});       // (every wave is through with tile t - 2)
-                if (t && t + NBUF - 2 < ntiles) load(t + NBUF - 2);
-                if (live) {
-                    float p[NX][2][4];
-                    const Tile k = look(t);
-                    if (k.rare) special(k, S);
-                    // (the first time round the pending product is of no rows: weights of zero, and tile 0 so that no stale bits are read)
-                    const uint32_t before = t ? (t - 1) % NBUF : 0;
-                    first_product(t + 1 < ntiles ? (t + 1) % NBUF : t % NBUF, next);
-                    if (weigh_first(k, S, p))
-                        move_all(k, S, [&] {
-                            second_product(before, W);
-#pragma unroll
-                            for (int j = 0; j < NX; ++j)
-#pragma unroll
-                                for (int q = 0; q < NP; ++q) W[j][q] = __builtin_bit_cast(V, u32x4{0, 0, 0, 0});
-                        }, p);
-                    second_product(before, W);
-                    weigh_second(p);
-                    pack(p, W);
-                    if (MODE == kRows && (k.rare || k.neg)) signs(k, W);
-#pragma unroll
-                    for (int j = 0; j < NX; ++j) { S[j][0] = next[j][0]; S[j][1] = next[j][1]; }
-                }
-            }
-            if (live) second_product((ntiles - 1) % NBUF, W);
         } else {
             f32x4 S[NX][2];
             V W[NX][NP];
@@ -485,11 +488,16 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
             for (uint32_t t = 0; t < ntiles; ++t) {
                 arrived(t, std::integral_constant<int, (NBUF > 1 ? NBUF - 2 : 0)>{});     // (every wave is through with tile t - 1)
                 if (NBUF > 1 && t + NBUF - 1 < ntiles) load(t + NBUF - 1);
+                if (live) first_product(t % NBUF, S);
+                if constexpr (KQ > 1) {
+                    part_out(S);
+                    __syncthreads();
+                }
                 if (live) {
+                    if constexpr (KQ > 1) parts_in(S);
                     const Tile k = look(t);
-                    first_product(t % NBUF, S);
                     if (k.rare) special(k, S);
-                    if (weigh_first(k, S, p)) move_all(k, S, [] {}, p);
+                    if (weigh_first(k, S, p)) move_all(k, S, p);
                     weigh_second(p);
                     if (MODE != kStats) {
                         pack(p, W);
@@ -504,7 +512,7 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
             }
         }
     }
-    finish<DT, MODE, OB, NX>(A, x0, n, g, slice, split, M, TWO ? Ml : M, l, O);
+    finish<DT, MODE, OW, NX>(A, x0, n, g, kq, split, M, TWO ? Ml : M, l, O);
 }
 
 }  // namespace rg
