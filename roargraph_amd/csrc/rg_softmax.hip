@@ -302,11 +302,21 @@ struct Plan {
     }
 };
 
+// The kernel of a mode.  Few rows x: the pass is bound by reading y, and the thin kernel, which reads fp32 rows and rows of any alignment once
+// and where they lie, beats planes made first (1M x 256 fp32, 8 to 64 queries: 280 - 331 us against 649 us).  It holds a row in a wave's
+// registers: of wide rows the sums no longer fit, and the wide kernel is faster even with planes (fp32 x 768: 994 against 669 us; x 512: 519
+// against 649 us).  16-bit rows it can read where they lie are a draw up to 256 elements, and the wide kernel's beyond (x 512: 238 - 333
+// against 150 - 160 us); their statistics alone are the thin kernel's up to 512 (111 against 121 us; x 1024: 131 against 122 us).
+bool thin_of(int mode, int ks, uint32_t nx, bool direct) {
+    if (mode == kRows || nx > 64) return false;
+    return mode == kStats ? ks <= 16 || !direct : ks <= (direct ? 8 : 16);
+}
+
 // direct: the streamed rows can be read where they lie (16-bit rows of whole 16-byte chunks, 16-byte aligned)
 Plan plan_of(int dtype, int mode, uint32_t dim, uint32_t nx, uint32_t ny, bool direct) {
     Plan p;
     p.ks = steps_of(dim);
-    p.thin = mode != kRows && nx <= 64;
+    p.thin = thin_of(mode, p.ks, nx, direct);
     p.k = kernel_of(dtype, mode, p.thin, p.ks);
     p.planes = !p.thin && !direct;
     p.nx = nx;
@@ -315,19 +325,22 @@ Plan plan_of(int dtype, int mode, uint32_t dim, uint32_t nx, uint32_t ny, bool d
     p.nslices = mode == kStats ? 1 : (dim + 16 * p.k.ob - 1) / (16 * p.k.ob);
     p.row_bytes = (uint64_t)(dtype == RG_DTYPE_F32 ? 2 : 1) * p.ks * 64;
     p.nuse = 0;
+    bool any_planes = false;
     for (int m = mode == kRows ? kRows : kStats; m <= (mode == kRows ? kRows : kMean); ++m) {
-        const SoftmaxKernel k = kernel_of(dtype, m, p.thin, p.ks);
+        const bool thin = thin_of(m, p.ks, nx, direct);
+        const SoftmaxKernel k = kernel_of(dtype, m, thin, p.ks);
         const uint64_t ntx = std::max<uint64_t>(1, ((uint64_t)nx + k.xt - 1) / k.xt), nslices = m == kStats ? 1 : (dim + 16 * k.ob - 1) / (16 * k.ob);
         Use &u = p.use[p.nuse++];
         u.nt = ntx * nslices;
         u.places = 256ull * std::min<uint32_t>(k.wps * 256 / k.threads, 160 * 1024 / k.lds);     // (256 CUs)
         const double ops = 2.0 * (dtype == RG_DTYPE_F32 ? 3 : 1) * (double)(u.nt * k.xt) * (32.0 * p.ks + (m == kStats ? 0.0 : 16.0 * k.ob));     // of a row y
-        u.row_cost = p.thin ? (double)dim * elem_bytes(dtype) * (double)nslices : ops / kOpsPerByte;
+        u.row_cost = std::max(thin || direct ? (double)dim * elem_bytes(dtype) * (double)nslices : 0.0, thin ? 0.0 : ops / kOpsPerByte);
+        any_planes |= !thin && !direct;
     }
     p.slot_cost = 8.0 * opitch_of(dim) * std::max(nx, 1u);
     p.free_slot = mode == kRows;
     p.piece = ny;
-    if (p.planes && mode != kRows) p.piece = (uint32_t)std::min<uint64_t>(ny, kPieceBytes / p.row_bytes / 32 * 32);
+    if (any_planes && mode != kRows) p.piece = (uint32_t)std::min<uint64_t>(ny, kPieceBytes / p.row_bytes / 32 * 32);
     p.nslots = 0;
     for (uint64_t y = 0; y == 0 || y < ny; y += std::max(p.piece, 1u)) p.nslots += p.cut((uint32_t)std::min<uint64_t>(p.piece, ny - y)).nsplit;
     return p;

@@ -16,7 +16,7 @@ SoftmaxKernel softmax_wide_bf16_mean(int ks) {
 SoftmaxKernel softmax_thin_bf16_mean(int ks) {
     switch (ks) {
 #define RG_KS(K) case K: return {reinterpret_cast<const void *>(rg_softmax_thin_kernel<RG_DTYPE_BF16, K, kMean>), (uint32_t)ThinCfg<RG_DTYPE_BF16, K>::XT, (uint32_t)ThinCfg<RG_DTYPE_BF16, K>::OB, (uint32_t)ThinCfg<RG_DTYPE_BF16, K>::LDS, (uint32_t)ThinCfg<RG_DTYPE_BF16, K>::WPS, 256u};
-        RG_KS(2) RG_KS(4) RG_KS(7) RG_KS(8) RG_KS(12) RG_KS(16) RG_KS(24) RG_KS(32)
+        RG_KS(2) RG_KS(4) RG_KS(7) RG_KS(8) RG_KS(12) RG_KS(16)
 #undef RG_KS
         default: return {};
     }

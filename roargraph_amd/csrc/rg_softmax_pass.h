@@ -75,6 +75,10 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
+// The sums of a product over the dimensions are made in this many parts, whichever kernel and waves make them: the logits
+// of all modes have the same bits.
+constexpr int softmax_parts(int dt, int ks) { return dt == RG_DTYPE_F32 ? (ks <= 8 ? 1 : ks <= 16 ? 2 : 4) : ks <= 16 ? 1 : 4; }
+
 template <int DT> struct Frag { typedef half8 V; };
 template <> struct Frag<RG_DTYPE_BF16> { typedef bf8 V; };
 

@@ -9,7 +9,7 @@ namespace rg {
 template <int DT, int KS>
 struct ThinCfg {
     static constexpr int NP = DT == RG_DTYPE_F32 ? 2 : 1;
-    static constexpr int OB = KS == 7 ? 13 : (DT == RG_DTYPE_F32 && KS == 32) ? 32 : 2 * KS;
+    static constexpr int OB = KS == 7 ? 13 : 2 * KS;
     static constexpr int XT = 64;
     static constexpr int TY = 32;
     static constexpr int PITCH = (KS * 64 + 255) / 256 * 256;
@@ -129,8 +129,19 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
         {
             const uint32_t sw = swizzle(n);                     // (row + 16: the same swizzle)
             const char *row = tile + n * PITCH;
+            constexpr int PART = KS / softmax_parts(DT, KS);
+            f32x4 sum[2][NX];
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
+                if (ks % PART == 0 && ks) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int j = 0; j < NX; ++j) {
+                            sum[h][j] = ks == PART ? S[h][j] : sum[h][j] + S[h][j];
+                            S[h][j] = f32x4{0, 0, 0, 0};
+                        }
+                }
                 const uint32_t c = 4 * ks + g;
                 const char *at = row + (c & ~15u) * 16 + (((c & 15) ^ sw) << 4);
                 V a[2][NP];
@@ -153,6 +164,11 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
 #pragma unroll
                     for (int j = 0; j < NX; ++j) S[h][j] = mma(a[h][0], X[j][ks][0], S[h][j]);
             }
+            if (PART < KS)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < NX; ++j) S[h][j] = sum[h][j] + S[h][j];
         }
         f32x4 ky[2], bias[2];
         if (F32)

@@ -21,8 +21,6 @@ namespace rg {
 struct WideChoice {
     int nx, kq;
 };
-// The sums of a product over the dimensions are made in this many parts, whichever waves make them: the logits of all modes have the same bits.
-constexpr int softmax_parts(int dt, int ks) { return dt == RG_DTYPE_F32 ? (ks <= 8 ? 1 : ks <= 16 ? 2 : 4) : ks <= 16 ? 1 : 4; }
 constexpr WideChoice softmax_wide_cfg(int dt, int ks, int mode) {
     const bool f32 = dt == RG_DTYPE_F32;
 #ifdef RG_WIDE_CFG
