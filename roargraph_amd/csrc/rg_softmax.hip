@@ -270,7 +270,7 @@ struct Plan {
     SoftmaxKernel k;
     int ks;
     bool thin, planes;
-    uint32_t nx, ny, ntx, nslices, piece, nslots;
+    uint32_t nx, ny, ntx, piece, nslots;
     uint64_t row_bytes;               // of a row of planes
     Use use[2];
     int nuse;
@@ -322,19 +322,17 @@ Plan plan_of(int dtype, int mode, uint32_t dim, uint32_t nx, uint32_t ny, bool d
     p.nx = nx;
     p.ny = ny;
     p.ntx = std::max(1u, (uint32_t)(((uint64_t)nx + p.k.xt - 1) / p.k.xt));
-    p.nslices = mode == kStats ? 1 : (dim + 16 * p.k.ob - 1) / (16 * p.k.ob);
     p.row_bytes = (uint64_t)(dtype == RG_DTYPE_F32 ? 2 : 1) * p.ks * 64;
     p.nuse = 0;
     bool any_planes = false;
     for (int m = mode == kRows ? kRows : kStats; m <= (mode == kRows ? kRows : kMean); ++m) {
         const bool thin = thin_of(m, p.ks, nx, direct);
         const SoftmaxKernel k = kernel_of(dtype, m, thin, p.ks);
-        const uint64_t ntx = std::max<uint64_t>(1, ((uint64_t)nx + k.xt - 1) / k.xt), nslices = m == kStats ? 1 : (dim + 16 * k.ob - 1) / (16 * k.ob);
         Use &u = p.use[p.nuse++];
-        u.nt = ntx * nslices;
+        u.nt = std::max<uint64_t>(1, ((uint64_t)nx + k.xt - 1) / k.xt);
         u.places = 256ull * std::min<uint32_t>(k.wps * 256 / k.threads, 160 * 1024 / k.lds);     // (256 CUs)
         const double ops = 2.0 * (dtype == RG_DTYPE_F32 ? 3 : 1) * (double)(u.nt * k.xt) * (32.0 * p.ks + (m == kStats ? 0.0 : 16.0 * k.ob));     // of a row y
-        u.row_cost = std::max(thin || direct ? (double)dim * elem_bytes(dtype) * (double)nslices : 0.0, thin ? 0.0 : ops / kOpsPerByte);
+        u.row_cost = std::max(thin || direct ? (double)dim * elem_bytes(dtype) : 0.0, thin ? 0.0 : ops / kOpsPerByte);
         any_planes |= !thin && !direct;
     }
     p.slot_cost = 8.0 * opitch_of(dim) * std::max(nx, 1u);
@@ -387,7 +385,7 @@ rg_status make_planes(const void *rows, uint64_t stride, uint32_t n, uint32_t di
 }
 
 rg_status launch_pass(const Plan &p, const PassArgs &A, hipStream_t s) {
-    const uint64_t grid = (uint64_t)p.ntx * p.nslices * A.nsplit;
+    const uint64_t grid = (uint64_t)p.ntx * A.nsplit;
     if (grid * p.k.threads > 0xffffffffull) return set_error(RG_ERR_ARG, "softmax over a base: too many rows for one launch");
     if (p.k.lds > 64 * 1024) RG_HIP(hipFuncSetAttribute(p.k.kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.k.lds));
     void *args[] = {const_cast<PassArgs *>(&A)};
@@ -445,7 +443,7 @@ rg_status shard(const Call &c, float *rest, float *own, float *lse, float *loss,
     A.x = c.queries; A.xstride = c.qstride; A.nx = c.nq;
     A.dim = A.ydim = c.dim;
     A.k = k_of(c.scale);
-    A.nslices = p.nslices; A.opitch = opitch_of(c.dim);
+    A.opitch = opitch_of(c.dim);
     A.targets = c.targets; A.own2 = reinterpret_cast<float *>(c.work + L.aux);
     float4 *ml = reinterpret_cast<float4 *>(c.work + L.ml);
     float *o = reinterpret_cast<float *>(c.work + L.o);
@@ -493,7 +491,7 @@ rg_status grad(const Call &c, const float *lse, const float *loss, const float *
     A.y = c.queries; A.ystride = c.qstride; A.ny = c.nq;
     A.dim = A.ydim = c.dim;
     A.k = k_of(c.scale);
-    A.nsplit = cut.nsplit; A.rows_per_split = cut.rows; A.nslices = p.nslices; A.opitch = opitch_of(c.dim);
+    A.nsplit = cut.nsplit; A.rows_per_split = cut.rows; A.opitch = opitch_of(c.dim);
     A.ml = reinterpret_cast<float4 *>(c.work + L.ml);
     A.o = reinterpret_cast<float *>(c.work + L.o);
     A.yinfo = info; A.ytarget = ytarget;

@@ -36,7 +36,6 @@ struct PassArgs {
     uint32_t nx, ny, dim, ydim;        // ydim: what of a row of y may be read
     float k;                           // scale * log2 e
     uint32_t nsplit, rows_per_split;   // of y
-    uint32_t nslices;                  // of the dimensions of O
     uint32_t opitch;                   // floats of a row of o
     float4 *ml;                        // [slot][nx] reference and sum of the weights, reference of O, -- (kMean, kStats; kRows in pieces: the third)
     float *o;                          // [slot][nx][opitch] (kMean, kRows in pieces)
@@ -50,7 +49,7 @@ struct PassArgs {
     float oscale;
 };
 
-// an instantiation: rows x of a workgroup, blocks of 16 output dims per slice, bytes of LDS, waves per SIMD, threads (rg_softmax_inst_*.hip)
+// an instantiation: rows x of a workgroup, blocks of 16 output dims, bytes of LDS, waves per SIMD, threads (rg_softmax_inst_*.hip)
 struct SoftmaxKernel {
     const void *kern;
     uint32_t xt, ob, lds, wps, threads;
@@ -182,9 +181,9 @@ __device__ __forceinline__ float load_stationary(const PassArgs &A, uint32_t x, 
     }
 }
 
-// what a wave leaves behind: references and sums, and the sums of rows (partial results, or the gradient itself)
+// what a wave (with part kq of the output blocks) leaves behind: references and sums, and the sums of rows (partial results, or the gradient itself)
 template <int DT, int MODE, int OB, int NX, int NO>
-__device__ __forceinline__ void finish(const PassArgs &A, uint32_t x0, uint32_t n, uint32_t g, uint32_t slice, uint32_t split, const float (&M)[NX], const float (&Ml)[NX], const float (&l)[NX],
+__device__ __forceinline__ void finish(const PassArgs &A, uint32_t x0, uint32_t n, uint32_t g, uint32_t kq, uint32_t split, const float (&M)[NX], const float (&Ml)[NX], const float (&l)[NX],
                                        const f32x4 (&O)[NO][NX]) {
     typedef typename Elem<DT>::T T;
 #pragma unroll
@@ -196,12 +195,12 @@ __device__ __forceinline__ void finish(const PassArgs &A, uint32_t x0, uint32_t 
         if (x >= A.nx) continue;
         const size_t at = (size_t)split * A.nx + x;
         const bool direct = MODE == kRows && A.nsplit == 1;
-        if (!direct && g == 0 && slice == 0) A.ml[at] = make_float4(Ml[j], s, M[j], 0.0f);
+        if (!direct && g == 0 && kq == 0) A.ml[at] = make_float4(Ml[j], s, M[j], 0.0f);
         if constexpr (MODE != kStats) {
             const float f = direct ? exp2_hw(0.5f * M[j]) : 1.0f;      // 2^M in two steps: it may lie below the normal range
 #pragma unroll
             for (int ob = 0; ob < OB; ++ob) {
-                const uint32_t d = (slice * OB + ob) * 16 + 4 * g;
+                const uint32_t d = (kq * OB + ob) * 16 + 4 * g;
                 if (d >= A.dim) continue;
                 if (!direct) {
                     *reinterpret_cast<f32x4 *>(A.o + at * A.opitch + d) = O[ob][j];

@@ -30,8 +30,7 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
     constexpr float kTop = 15.0f, kStart = DT == RG_DTYPE_BF16 ? 0.0f : 7.0f;   // a weight is at most 2^15; the first largest one 2^0 / 2^7
     extern __shared__ char lds[];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
-    const uint32_t b = xcd_block(blockIdx.x, gridDim.x);
-    const uint32_t slice = MODE == kStats ? 0 : b % A.nslices, split = MODE == kStats ? b : b / A.nslices;
+    const uint32_t split = xcd_block(blockIdx.x, gridDim.x);
     const uint32_t ybeg = min(A.ny, split * A.rows_per_split), yend = min(A.ny, ybeg + A.rows_per_split);
     const uint32_t x0 = wave * 16;
     const bool live = x0 < A.nx;                                // waves behind the last row only help to load
@@ -192,7 +191,7 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
                         if (y0 + r == target[j]) {
                             float z = S[h][j][i];
                             if (F32) z *= ky[h][i];
-                            if (slice == 0) A.own2[x] = z * kx[j];
+                            A.own2[x] = z * kx[j];
                             dead |= 1u << (4 * h + i);
                         }
                         if (y0 + r >= yend) dead |= 1u << (4 * h + i);
@@ -279,7 +278,7 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
             const char *row = tile + r * PITCH + (n & 1) * 8;
 #pragma unroll
             for (int ob = 0; ob < OB; ++ob) {
-                const uint32_t c = 2 * (slice * OB + ob) + ((n >> 1) & 1);
+                const uint32_t c = 2 * ob + ((n >> 1) & 1);
                 const char *at = row + (c & ~15u) * 16 + (((c & 15) ^ sw) << 4);
                 V a[NP];
 #pragma unroll
@@ -324,7 +323,7 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
         }
     }
 
-    finish<DT, MODE, OB, NX>(A, x0, n, g, slice, split, M, TWO ? Ml : M, l, O);
+    finish<DT, MODE, OB, NX>(A, x0, n, g, 0, split, M, TWO ? Ml : M, l, O);
 }
 
 }  // namespace rg

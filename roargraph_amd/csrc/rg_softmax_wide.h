@@ -3,13 +3,12 @@
 //
 // Streamed rows arrive as 16-bit planes (16-bit rows where they lie, or what rg_softmax_planes_kernel wrote: rows padded to the
 // instantiation's width, fp32 as two halves) and go from memory to LDS without passing registers (global_load_lds, 16 bytes a lane) into
-// a ring of as many tile buffers as fit, so that 50 - 100 KB per CU are on their way at any time.  One wave per SIMD, as many blocks of x
-// as 512 registers hold: every LDS operand read feeds NX products.
+// a ring of as many tile buffers as fit, so that 50 - 100 KB per CU are on their way at any time.
 //
-// With a ring of six and more the loop runs three tiles at a time, so that matrix and vector units work side by side in one wave:
-//     first product of tile t + 1   while  the logits of tile t are scaled and compared with the reference
-//     second product of tile t - 1  while  the weights of tile t are taken (exp2, sums, rounding)
-// A reference that moves (rare) first lets the pending second product go, then rescales.
+// Two waves per SIMD, so that the weights of one are taken while the products of the other run.  (One wave per SIMD with 512 registers and a
+// loop over three tiles, which does the same within a wave, took 4.5 ms where this takes 3.0: half the registers can only be moved to, not used.)
+// Every LDS operand read feeds NX products.  Wide rows, of which a wave's 256 registers do not hold one, are shared by KQ waves: each has a
+// part of the dimensions, they add up their products in LDS, and each takes the weights of all rows y for its own part of the output.
 #pragma once
 #include <type_traits>
 
@@ -21,17 +20,17 @@ namespace rg {
 struct WideChoice {
     int nx, kq;
 };
+// Measured (2000 queries, 30M elements of base, training step; with spills: the form whose registers were not enough): fp32 x 512 one wave a row
+// 1.82 ms, two 1.57 ms; x 768 four waves, 16 rows each 2.31 ms, 32 rows (spills) 2.80 ms, one wave (spills) 6.07 ms; fp16 x 512 one wave, 16 rows
+// 0.62 ms, two waves, 32 rows (spills) 1.10 ms; x 1024 four waves 1.10 ms, one (spills) 5.59 ms.  Statistics alone: fp16 x 768 one wave 0.14 ms,
+// four 0.26 ms; fp32 x 768 four waves, 32 rows 0.56 ms, one 0.93 ms.
 constexpr WideChoice softmax_wide_cfg(int dt, int ks, int mode) {
     const bool f32 = dt == RG_DTYPE_F32;
-#ifdef RG_WIDE_CFG
-    return RG_WIDE_CFG;
-#else
     if (mode == kStats && f32) return ks <= 4 ? WideChoice{3, 1} : ks <= 7 ? WideChoice{2, 1} : ks <= 16 ? WideChoice{1, 1} : ks <= 24 ? WideChoice{2, 4} : WideChoice{1, 4};
     if (mode == kStats) return {ks <= 7 ? 4 : ks <= 8 ? 3 : ks <= 16 ? 2 : 1, 1};
     const int kq = softmax_parts(dt, ks);
     if (f32) return {ks <= 4 ? 2 : 1, kq};
     return {ks <= 2 ? 4 : ks <= 4 ? 3 : ks <= 7 || (ks == 8 && mode == kMean) ? 2 : ks <= 16 ? 1 : ks <= 24 || mode == kMean ? 2 : 1, kq};
-#endif
 }
 
 template <int DT, int KS, int MODE>
