@@ -170,14 +170,13 @@ __global__ void __launch_bounds__(256) rg_softmax_planes_kernel(const void *rows
                                                                 int more) {
     typedef typename Elem<DT>::T T;
     constexpr int NP = DT == RG_DTYPE_F32 ? 2 : 1;
-    const bool vec = ((uintptr_t)rows | stride * sizeof(T)) % 16 == 0;
     const uint32_t lc = threadIdx.x % 16;
     for (uint64_t r = (uint64_t)blockIdx.x * 16 + threadIdx.x / 16; r < npad; r += (uint64_t)gridDim.x * 16) {
         const char *row = static_cast<const char *>(rows) + (size_t)r * stride * sizeof(T);
         uint16_t *out = planes + (size_t)r * NP * ks * 32;
         Chunk<DT> c[CI];
 #pragma unroll
-        for (int i = 0; i < CI; ++i) c[i] = load_chunk<DT>(row, 8 * (lc + 16 * i), r < n ? dim : 0, vec);
+        for (int i = 0; i < CI; ++i) c[i] = load_chunk<DT>(row, 8 * (lc + 16 * i), r < n ? dim : 0);
         if constexpr (DT == RG_DTYPE_F32) {
             uint32_t m = 0;
 #pragma unroll

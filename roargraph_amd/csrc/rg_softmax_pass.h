@@ -88,33 +88,36 @@ __device__ __forceinline__ uint32_t swizzle(uint32_t y) { return (((y & 7) ^ (y 
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// 8 elements of a row from element k on (zeros from dim on): as they are for 16-bit types, as floats for fp32
+// 8 elements of a row from element k on (zeros from dim on): as they are for 16-bit types, as floats for fp32.  Rows need no other alignment
+// than their elements': the memory units take wide loads and stores of any address.
 template <int DT> struct Chunk { u32x4 v; };
 template <> struct Chunk<RG_DTYPE_F32> { f32x4 a, b; };
+typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+typedef f32x4 f32x4_a4 __attribute__((aligned(4)));
 
 template <int DT>
-__device__ __forceinline__ Chunk<DT> load_chunk(const void *row, uint32_t k, uint32_t dim, bool vec) {
+__device__ __forceinline__ Chunk<DT> load_chunk(const void *row, uint32_t k, uint32_t dim) {
     const uint16_t *p = static_cast<const uint16_t *>(row) + k;
     Chunk<DT> c;
     c.v = u32x4{0, 0, 0, 0};
-    if (k + 8 <= dim && vec) {
-        c.v = *reinterpret_cast<const u32x4 *>(p);
-    } else {
+    if (k + 8 <= dim) {
+        c.v = *reinterpret_cast<const u32x4_a2 *>(p);
+    } else if (k < dim) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 7; ++i)
             if (k + i < dim) c.v[i / 2] |= (uint32_t)p[i] << (16 * (i % 2));
     }
     return c;
 }
 template <>
-__device__ __forceinline__ Chunk<RG_DTYPE_F32> load_chunk<RG_DTYPE_F32>(const void *row, uint32_t k, uint32_t dim, bool vec) {
+__device__ __forceinline__ Chunk<RG_DTYPE_F32> load_chunk<RG_DTYPE_F32>(const void *row, uint32_t k, uint32_t dim) {
     const float *p = static_cast<const float *>(row) + k;
     Chunk<RG_DTYPE_F32> c;
     c.a = c.b = f32x4{0, 0, 0, 0};
-    if (k + 8 <= dim && vec) {
-        c.a = *reinterpret_cast<const f32x4 *>(p);
-        c.b = *reinterpret_cast<const f32x4 *>(p + 4);
-    } else {
+    if (k + 8 <= dim) {
+        c.a = *reinterpret_cast<const f32x4_a4 *>(p);
+        c.b = *reinterpret_cast<const f32x4_a4 *>(p + 4);
+    } else if (k < dim) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (k + i < dim) c.a[i] = p[i];
@@ -153,7 +156,7 @@ __device__ __forceinline__ void split8(Chunk<RG_DTYPE_F32> c, float top, float s
 // stationary operands of row x: lane (n, g) holds elements 32 ks + 8 g .. + 7 of part kq of nkq of the row; returns what its logits are
 // multiplied by
 template <int DT, int KS, int NP>
-__device__ __forceinline__ float load_stationary(const PassArgs &A, uint32_t x, uint32_t g, bool vec, typename Frag<DT>::V (&X)[KS][NP], uint32_t kq = 0, uint32_t nkq = 1) {
+__device__ __forceinline__ float load_stationary(const PassArgs &A, uint32_t x, uint32_t g, typename Frag<DT>::V (&X)[KS][NP], uint32_t kq = 0, uint32_t nkq = 1) {
     const char *row = static_cast<const char *>(A.x) + (size_t)x * A.xstride * sizeof(typename Elem<DT>::T);
     const uint32_t dim = x < A.nx ? A.dim : 0, k0 = 32 * KS * kq + 8 * g;
     if constexpr (DT == RG_DTYPE_F32) {
@@ -161,10 +164,10 @@ __device__ __forceinline__ float load_stationary(const PassArgs &A, uint32_t x, 
         Chunk<DT> c[KS];
         for (uint32_t q = 1; q < nkq; ++q)          // the other parts count for the largest element
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) m = max(m, __float_as_uint(absmax(load_chunk<DT>(row, 32 * KS * ((kq + q) % nkq) + 32 * ks + 8 * g, dim, vec))));
+            for (int ks = 0; ks < KS; ++ks) m = max(m, __float_as_uint(absmax(load_chunk<DT>(row, 32 * KS * ((kq + q) % nkq) + 32 * ks + 8 * g, dim))));
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            c[ks] = load_chunk<DT>(row, k0 + 32 * ks, dim, vec);
+            c[ks] = load_chunk<DT>(row, k0 + 32 * ks, dim);
             m = max(m, __float_as_uint(absmax(c[ks])));
         }
         m = max(m, (uint32_t)__shfl_xor((int)m, 16));
@@ -176,7 +179,7 @@ __device__ __forceinline__ float load_stationary(const PassArgs &A, uint32_t x, 
         return A.k * row_factor(top, e);
     } else {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) X[ks][0] = __builtin_bit_cast(typename Frag<DT>::V, load_chunk<DT>(row, k0 + 32 * ks, dim, vec).v);
+        for (int ks = 0; ks < KS; ++ks) X[ks][0] = __builtin_bit_cast(typename Frag<DT>::V, load_chunk<DT>(row, k0 + 32 * ks, dim).v);
         return A.k;
     }
 }
@@ -206,9 +209,18 @@ __device__ __forceinline__ void finish(const PassArgs &A, uint32_t x0, uint32_t 
                     *reinterpret_cast<f32x4 *>(A.o + at * A.opitch + d) = O[ob][j];
                 } else {
                     T *out = static_cast<T *>(A.out) + (size_t)x * A.ostride + d;
+                    typedef T T4 __attribute__((ext_vector_type(4)));
+                    typedef T4 T4_any __attribute__((aligned(sizeof(T))));
+                    T4 v;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (d + i < A.dim) out[i] = (T)(O[ob][j][i] * f * (f * A.oscale));
+                    for (int i = 0; i < 4; ++i) v[i] = (T)(O[ob][j][i] * f * (f * A.oscale));
+                    if (d + 4 <= A.dim) {
+                        *reinterpret_cast<T4_any *>(out) = v;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 3; ++i)
+                            if (d + i < A.dim) out[i] = v[i];
+                    }
                 }
             }
         }

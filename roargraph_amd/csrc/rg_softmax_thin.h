@@ -36,7 +36,6 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
     const bool live = x0 < A.nx;                                // waves behind the last row only help to load
     const uint32_t dim = A.dim;
     const size_t esz = sizeof(T);
-    const bool xvec = ((uintptr_t)A.x | A.xstride * esz) % 16 == 0, yvec = ((uintptr_t)A.y | A.ystride * esz) % 16 == 0;
 
     V X[NX][KS][NP];
     float kx[NX];
@@ -44,7 +43,7 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
 #pragma unroll
     for (int j = 0; j < NX; ++j) {
         const uint32_t x = x0 + j * 16 + n;
-        kx[j] = load_stationary<DT, KS>(A, x, g, xvec, X[j]);
+        kx[j] = load_stationary<DT, KS>(A, x, g, X[j]);
         target[j] = kNoTarget;
         if (x < A.nx) {
             const uint32_t t = A.targets[x];
@@ -74,7 +73,7 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
             const uint32_t y = y0 + lr + 16 * h;
             const char *row = static_cast<const char *>(A.y) + (size_t)y * A.ystride * esz;
 #pragma unroll
-            for (int i = 0; i < CI; ++i) stage[h][i] = load_chunk<DT>(row, 8 * (lc + 16 * i), y < yend ? dim : 0, yvec);
+            for (int i = 0; i < CI; ++i) stage[h][i] = load_chunk<DT>(row, 8 * (lc + 16 * i), y < yend ? dim : 0);
         }
     };
     auto commit = [&](uint32_t buf) {

@@ -139,11 +139,10 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
     V X[NX][KW][NP];
     float kx[NX];
     uint32_t target[NX];
-    const bool xvec = ((uintptr_t)A.x | A.xstride * sizeof(T)) % 16 == 0;
 #pragma unroll
     for (int j = 0; j < NX; ++j) {
         const uint32_t x = x0 + j * 16 + n;
-        kx[j] = load_stationary<DT, KW>(A, x, g, xvec, X[j], kq, KQ);
+        kx[j] = load_stationary<DT, KW>(A, x, g, X[j], kq, KQ);
         target[j] = kNoTarget;
         if (MODE != kRows && x < A.nx) {
             const uint32_t tg = A.targets[x];
