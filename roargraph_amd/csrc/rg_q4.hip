@@ -25,15 +25,17 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // eight elements of a row from k on (n of them exist)
 template <int DT>
-__device__ __forceinline__ void load8(const typename Elem<DT>::T *row, uint32_t k, uint32_t n, bool vec, float (&v)[8]) {
-    if (n == 8 && vec) {
+__device__ __forceinline__ void load8(const typename Elem<DT>::T *row, uint32_t k, uint32_t n, float (&v)[8]) {
+    if (n == 8) {                                    // (wide loads take any address)
         if constexpr (DT == RG_DTYPE_F32) {
-            const f32x4 a = *reinterpret_cast<const f32x4 *>(row + k), b = *reinterpret_cast<const f32x4 *>(row + k + 4);
+            typedef f32x4 f32x4_a4 __attribute__((aligned(4)));
+            const f32x4 a = *reinterpret_cast<const f32x4_a4 *>(row + k), b = *reinterpret_cast<const f32x4_a4 *>(row + k + 4);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = i < 4 ? a[i % 4] : b[i % 4];
         } else {
             typedef typename std::conditional<DT == RG_DTYPE_F16, half8, bf8>::type V;
-            const V a = *reinterpret_cast<const V *>(row + k);
+            typedef V V_a2 __attribute__((aligned(2)));
+            const V a = *reinterpret_cast<const V_a2 *>(row + k);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
         }
@@ -51,7 +53,6 @@ __global__ void __launch_bounds__(256) rg_q4_pack_kernel(const void *rows, uint3
                                                          uint16_t *scales, uint16_t *mins, uint64_t sstride) {
     typedef typename Elem<DT>::T T;
     const uint32_t lanes = group / 8, D = (dim + 7) / 8, per_row = (D + lanes - 1) / lanes * lanes;
-    const bool vec = ((uintptr_t)rows | stride * sizeof(T)) % 16 == 0;
     const int first = mins ? 0 : -8;
     // (whole waves turn together: per_row * nb rounded up to them)
     const uint64_t total = (uint64_t)nb * per_row;
@@ -63,7 +64,7 @@ __global__ void __launch_bounds__(256) rg_q4_pack_kernel(const void *rows, uint3
         const bool here = at < total && l < D;
         const uint32_t row = min(j, nb - 1), k = min(l, D - 1) * 8, n = min(8u, dim - k);
         float v[8];
-        load8<DT>(static_cast<const T *>(rows) + (size_t)row * stride, k, n, vec, v);
+        load8<DT>(static_cast<const T *>(rows) + (size_t)row * stride, k, n, v);
         float lo = v[0], hi = v[0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) { lo = fminf(lo, v[i]); hi = fmaxf(hi, v[i]); }

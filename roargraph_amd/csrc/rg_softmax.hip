@@ -25,7 +25,7 @@
 namespace rg {
 namespace {
 
-constexpr uint32_t kMaxDim = 1024;
+constexpr uint32_t kMaxDim = 1024, kMaxQueries = (1u << 24) - 1;     // (a workgroup of 256 each, and a launch holds less than 2^32 threads)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ bool target_here(uint32_t t, uint32_t id_base, uint32_t nb) { return t != kNoTarget && t >= id_base && t - id_base < nb; }
@@ -129,14 +129,14 @@ __device__ __forceinline__ void put_info(float *info, uint64_t y, float factor, 
 
 // per query: what the pass over the rows needs of it (info and ytarget, padded to whole tiles), and dq.  One wave per query.
 template <int DT>
-__global__ void __launch_bounds__(64) rg_softmax_dq_kernel(const void *base, uint64_t bstride, uint32_t nb, uint32_t id_base, uint32_t nq, uint32_t dim, float scale,
+__global__ void __launch_bounds__(64) rg_softmax_dq_kernel(const void *queries, uint64_t qstride, const void *base, uint64_t bstride, uint32_t nb, uint32_t id_base, uint32_t nq, uint32_t dim, float scale,
                                                            const uint32_t *targets, const float *lse, const float *loss, const float *rest, const float *mean,
                                                            const float *weights, void *dq, uint64_t dqstride, float *info, float *ytarget) {
     typedef typename Elem<DT>::T T;
     const uint32_t i = blockIdx.x;
     if (i >= nq) {
         if (threadIdx.x == 0) {
-            put_info(info, i, 1.0f, -INFINITY, 1.0f, kNoTarget);
+            put_info(info, i, 1.0f, -INFINITY, 0.0f, kNoTarget);     // (copies of the last query: they take no part, whatever that holds)
             ytarget[i] = -INFINITY;
         }
         return;
@@ -144,9 +144,14 @@ __global__ void __launch_bounds__(64) rg_softmax_dq_kernel(const void *base, uin
     const uint32_t t = targets[i], row = t - id_base;
     const bool here = target_here(t, id_base, nb);
     const float w = t == kNoTarget ? 0.0f : weights[i], miss = here ? -expm1f(-loss[i]) : 0.0f;      // 1 - p_target
+    bool whole = true;                  // a query that takes no part may hold anything: the pass over the rows is told (sign 0)
+    if (info && t == kNoTarget) {
+        for (uint32_t k = threadIdx.x; k < dim; k += 64) whole &= fabsf((float)static_cast<const T *>(queries)[(size_t)i * qstride + k]) < INFINITY;
+        whole = __all(whole);
+    }
     if (info && threadIdx.x == 0) {
         const float lw = log2f(fabsf(w));
-        put_info(info, i, 1.0f, t == kNoTarget ? -INFINITY : lw - lse[i] * kLog2e, w < 0.0f ? -1.0f : 1.0f, here ? row : kNoTarget);
+        put_info(info, i, 1.0f, t == kNoTarget ? -INFINITY : lw - lse[i] * kLog2e, w < 0.0f ? -1.0f : whole ? 1.0f : 0.0f, here ? row : kNoTarget);
         ytarget[i] = lw + log2f(miss);
     }
     if (!dq) return;
@@ -175,8 +180,9 @@ __global__ void __launch_bounds__(256) rg_softmax_planes_kernel(const void *rows
         const char *row = static_cast<const char *>(rows) + (size_t)r * stride * sizeof(T);
         uint16_t *out = planes + (size_t)r * NP * ks * 32;
         Chunk<DT> c[CI];
+        const bool take = r < n && !(more && info[r / 32 * 128 + 64 + r % 32] == 0.0f);     // (not finite, and takes no part)
 #pragma unroll
-        for (int i = 0; i < CI; ++i) c[i] = load_chunk<DT>(row, 8 * (lc + 16 * i), r < n ? dim : 0);
+        for (int i = 0; i < CI; ++i) c[i] = load_chunk<DT>(row, 8 * (lc + 16 * i), take ? dim : 0);
         if constexpr (DT == RG_DTYPE_F32) {
             uint32_t m = 0;
 #pragma unroll
@@ -251,7 +257,7 @@ SoftmaxKernel kernel_of(int dtype, int mode, bool thin, int ks) {
 }
 
 // how a pass is cut: into pieces of y that are made into planes one after another (planes), each split into slots whose partial results are
-// joined at the end.  More slots fill the workgroup places of the device, and each costs the writing and reading of its results: the cheapest
+// joined at the end (a slot goes on from piece to piece).  More slots fill the workgroup places of the device, and each costs the writing and reading of its results: the cheapest
 // number is taken, in bytes of the device's traffic, one of which it moves while its matrix cores do kOpsPerByte operations of a pass (measured:
 // 600 Top/s of the 16-bit passes, 4 TB/s).  333 fp16 queries on 70001 rows of 93 dims: 3 slots, which leave fewer places empty, took
 // 80 us + 29 us to join for the gradient of the rows, 1 slot 58 us.
@@ -338,8 +344,7 @@ Plan plan_of(int dtype, int mode, uint32_t dim, uint32_t nx, uint32_t ny, bool d
     p.free_slot = mode == kRows;
     p.piece = ny;
     if (any_planes && mode != kRows) p.piece = (uint32_t)std::min<uint64_t>(ny, kPieceBytes / p.row_bytes / 32 * 32);
-    p.nslots = 0;
-    for (uint64_t y = 0; y == 0 || y < ny; y += std::max(p.piece, 1u)) p.nslots += p.cut((uint32_t)std::min<uint64_t>(p.piece, ny - y)).nsplit;
+    p.nslots = p.cut(p.piece).nsplit;
     return p;
 }
 
@@ -395,7 +400,7 @@ rg_status launch_pass(const Plan &p, const PassArgs &A, hipStream_t s) {
 rg_status check_shapes(uint32_t nb, uint32_t nq, uint32_t dim, int dtype) {
     if (!known_dtype(dtype)) return set_error(RG_ERR_ARG, "unknown dtype");
     if (dim == 0 || dim > kMaxDim) return set_error(RG_ERR_ARG, "softmax over a base: dim must be in [1, 1024]");
-    if (nb > 0x7fffffffu || nq > 0xffffffu) return set_error(RG_ERR_ARG, "softmax over a base: at most 2^31 - 1 rows and 2^24 - 1 queries");     // (a launch holds 2^32 - 1 threads)
+    if (nb > 0x7fffffffu || nq > kMaxQueries) return set_error(RG_ERR_ARG, "softmax over a base: at most 2^31 - 1 rows and 2^24 - 1 queries");
     return RG_OK;
 }
 rg_status check_rows(const void *p, uint32_t n, uint64_t stride, uint32_t dim, int dtype, const char *name) {
@@ -446,16 +451,15 @@ rg_status shard(const Call &c, float *rest, float *own, float *lse, float *loss,
     A.targets = c.targets; A.own2 = reinterpret_cast<float *>(c.work + L.aux);
     float4 *ml = reinterpret_cast<float4 *>(c.work + L.ml);
     float *o = reinterpret_cast<float *>(c.work + L.o);
-    uint32_t slot = 0;
+    A.ml = ml; A.o = o;
+    A.nsplit = p.nslots;
     for (uint64_t y = 0; y == 0 || y < c.nb; y += std::max(p.piece, 1u)) {
         const uint32_t n = (uint32_t)std::min<uint64_t>(p.piece, c.nb - y);
-        const Plan::Cut cut = p.cut(n);
         A.y = static_cast<const char *>(c.base) + y * c.bstride * sizeof(typename Elem<DT>::T);
         A.ystride = c.bstride; A.ny = n;
         A.id_base = c.id_base + (uint32_t)y;
-        A.nsplit = cut.nsplit; A.rows_per_split = cut.rows;
-        A.ml = ml + (size_t)slot * c.nq;
-        A.o = o + (size_t)slot * c.nq * A.opitch;
+        A.rows_per_split = up32((uint32_t)(((uint64_t)n + p.nslots - 1) / p.nslots));
+        A.resume = y != 0;
         if (p.planes && n) {
             float *info = reinterpret_cast<float *>(c.work + L.info);
             rg_status st = make_planes<DT>(A.y, c.bstride, n, c.dim, p.ks, c.work + L.planes, info, nullptr, c.s);
@@ -464,7 +468,6 @@ rg_status shard(const Call &c, float *rest, float *own, float *lse, float *loss,
         }
         rg_status st = launch_pass(p, A, c.s);
         if (st != RG_OK) return st;
-        slot += cut.nsplit;
     }
     hipLaunchKernelGGL(rg_softmax_join_kernel, dim3(c.nq, mean ? std::clamp(4096u / c.nq, 1u, (c.dim + kJoinDims - 1) / kJoinDims) : 1), dim3(256), 0, c.s, ml, o, A.opitch, p.nslots, c.nq, c.dim, c.nb, c.id_base, A.own2, c.targets, rest, own, lse, loss, mean);
     RG_HIP(hipGetLastError());
@@ -479,7 +482,7 @@ rg_status grad(const Call &c, const float *lse, const float *loss, const float *
     float *info = rows ? reinterpret_cast<float *>(c.work + L.info) : nullptr;
     float *ytarget = rows ? reinterpret_cast<float *>(c.work + L.aux) : nullptr;
     if (c.nq) {
-        hipLaunchKernelGGL((rg_softmax_dq_kernel<DT>), dim3(rows ? up32(c.nq) : c.nq), dim3(64), 0, c.s, c.base, c.bstride, c.nb, c.id_base, c.nq, c.dim, c.scale, c.targets, lse, loss, rest, mean, weights,
+        hipLaunchKernelGGL((rg_softmax_dq_kernel<DT>), dim3(rows ? up32(c.nq) : c.nq), dim3(64), 0, c.s, c.queries, c.qstride, c.base, c.bstride, c.nb, c.id_base, c.nq, c.dim, c.scale, c.targets, lse, loss, rest, mean, weights,
                            dq, dqstride, info, ytarget);
         RG_HIP(hipGetLastError());
     }
@@ -543,6 +546,7 @@ rg_status rg_softmax_shard_dev(const void *d_base, uint32_t nb, uint64_t bstride
 rg_status rg_softmax_merge_dev(const float *d_rest_in, const float *d_own_in, uint32_t nlists, uint32_t nq, const uint32_t *d_targets,
                                float *d_lse, float *d_loss, int device, void *stream) {
     if (nlists == 0) return set_error(RG_ERR_ARG, "nlists must be positive");
+    if (nq > kMaxQueries) return set_error(RG_ERR_ARG, "softmax over a base: at most 2^24 - 1 queries");
     if (nq == 0) return RG_OK;
     if (!d_rest_in || !d_own_in || !d_targets || !d_lse || !d_loss) return set_error(RG_ERR_ARG, "null argument");
     OnDevice on(device);

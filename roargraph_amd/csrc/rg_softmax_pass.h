@@ -37,6 +37,7 @@ struct PassArgs {
     float k;                           // scale * log2 e
     uint32_t nsplit, rows_per_split;   // of y
     uint32_t opitch;                   // floats of a row of o
+    uint32_t resume;                   // the slots hold what earlier pieces of y left
     float4 *ml;                        // [slot][nx] reference and sum of the weights, reference of O, -- (kMean, kStats; kRows in pieces: the third)
     float *o;                          // [slot][nx][opitch] (kMean, kRows in pieces)
     const uint32_t *targets;           // kStats, kMean: per x (global ids)
@@ -153,34 +154,62 @@ __device__ __forceinline__ void split8(Chunk<RG_DTYPE_F32> c, float top, float s
     }
 }
 
-// stationary operands of row x: lane (n, g) holds elements 32 ks + 8 g .. + 7 of part kq of nkq of the row; returns what its logits are
+// stationary operands of row x: lane (n, g) holds elements 32 ks + 8 g .. + 7 of part kq of KQ of the row; returns what its logits are
 // multiplied by
-template <int DT, int KS, int NP>
-__device__ __forceinline__ float load_stationary(const PassArgs &A, uint32_t x, uint32_t g, typename Frag<DT>::V (&X)[KS][NP], uint32_t kq = 0, uint32_t nkq = 1) {
+template <int DT, int KS, int KQ, int NP>
+__device__ __forceinline__ float load_stationary(const PassArgs &A, uint32_t x, uint32_t g, typename Frag<DT>::V (&X)[KS][NP], uint32_t kq = 0) {
     const char *row = static_cast<const char *>(A.x) + (size_t)x * A.xstride * sizeof(typename Elem<DT>::T);
     const uint32_t dim = x < A.nx ? A.dim : 0, k0 = 32 * KS * kq + 8 * g;
     if constexpr (DT == RG_DTYPE_F32) {
+        // the largest element of the row, all its parts, then this part -- at once where it is all of it, else once more from the caches
+        // (with the registers of a wide row's part it would not fit)
         uint32_t m = 0;
         Chunk<DT> c[KS];
-        for (uint32_t q = 1; q < nkq; ++q)          // the other parts count for the largest element
+        if (KQ == 1) {
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) m = max(m, __float_as_uint(absmax(load_chunk<DT>(row, 32 * KS * ((kq + q) % nkq) + 32 * ks + 8 * g, dim))));
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            c[ks] = load_chunk<DT>(row, k0 + 32 * ks, dim);
-            m = max(m, __float_as_uint(absmax(c[ks])));
+            for (int ks = 0; ks < KS; ++ks) {
+                c[ks] = load_chunk<DT>(row, k0 + 32 * ks, dim);
+                m = max(m, __float_as_uint(absmax(c[ks])));
+            }
+        } else {
+#pragma unroll 4
+            for (uint32_t ks = 0; ks < KS * KQ; ++ks) m = max(m, __float_as_uint(absmax(load_chunk<DT>(row, 32 * ks + 8 * g, dim))));
         }
         m = max(m, (uint32_t)__shfl_xor((int)m, 16));
         m = max(m, (uint32_t)__shfl_xor((int)m, 32));
         const float top = __uint_as_float(m);
         const int e = row_exponent(top);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) split8(c[ks], top, pow2(-e), X[ks][0], X[ks][1]);
+        for (int ks = 0; ks < KS; ++ks) {
+            split8(KQ == 1 ? c[ks] : load_chunk<DT>(row, k0 + 32 * ks, dim), top, pow2(-e), X[ks][0], X[ks][1]);
+            if (KQ > 1) __builtin_amdgcn_sched_barrier(0);
+        }
         return A.k * row_factor(top, e);
     } else {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) X[ks][0] = __builtin_bit_cast(typename Frag<DT>::V, load_chunk<DT>(row, k0 + 32 * ks, dim).v);
         return A.k;
+    }
+}
+
+// what an earlier piece left in a wave's slot
+template <int MODE, int OB, int NX, int NO>
+__device__ __forceinline__ void take_up(const PassArgs &A, uint32_t x0, uint32_t n, uint32_t g, uint32_t kq, uint32_t split, float (&M)[NX], float (&Ml)[NX], float (&l)[NX], f32x4 (&O)[NO][NX]) {
+#pragma unroll
+    for (int j = 0; j < NX; ++j) {
+        const uint32_t x = x0 + j * 16 + n;
+        if (x >= A.nx) continue;
+        const size_t at = (size_t)split * A.nx + x;
+        const float4 v = A.ml[at];
+        Ml[j] = v.x;
+        M[j] = v.z;
+        l[j] = g == 0 ? v.y : 0.0f;                  // (finish adds the four up)
+        if constexpr (MODE != kStats)
+#pragma unroll
+            for (int ob = 0; ob < OB; ++ob) {
+                const uint32_t d = (kq * OB + ob) * 16 + 4 * g;
+                if (d < A.dim) O[ob][j] = *reinterpret_cast<const f32x4 *>(A.o + at * A.opitch + d);
+            }
     }
 }
 

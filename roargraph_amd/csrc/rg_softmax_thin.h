@@ -43,7 +43,7 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
 #pragma unroll
     for (int j = 0; j < NX; ++j) {
         const uint32_t x = x0 + j * 16 + n;
-        kx[j] = load_stationary<DT, KS>(A, x, g, X[j]);
+        kx[j] = load_stationary<DT, KS, 1>(A, x, g, X[j]);
         target[j] = kNoTarget;
         if (x < A.nx) {
             const uint32_t t = A.targets[x];
@@ -63,6 +63,8 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
 #pragma unroll
             for (int ob = 0; ob < OB; ++ob) O[ob][j] = f32x4{0, 0, 0, 0};
     }
+
+    if (A.resume) take_up<MODE, OB, NX>(A, x0, n, g, 0, split, M, Ml, l, O);
 
     // streaming: 16 lanes per row, two rows per thread (r, r + 16)
     const uint32_t lr = tid >> 4, lc = tid & 15;

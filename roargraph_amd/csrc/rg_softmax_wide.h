@@ -142,7 +142,7 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
 #pragma unroll
     for (int j = 0; j < NX; ++j) {
         const uint32_t x = x0 + j * 16 + n;
-        kx[j] = load_stationary<DT, KW>(A, x, g, X[j], kq, KQ);
+        kx[j] = load_stationary<DT, KW, KQ>(A, x, g, X[j], kq);
         target[j] = kNoTarget;
         if (MODE != kRows && x < A.nx) {
             const uint32_t tg = A.targets[x];
@@ -160,6 +160,11 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
         if (MODE != kStats)
 #pragma unroll
             for (int ob = 0; ob < OW; ++ob) O[ob][j] = f32x4{0, 0, 0, 0};
+    }
+
+    if (MODE != kRows && A.resume) {
+        take_up<MODE, OW, NX>(A, x0, n, g, kq, split, M, Ml, l, O);
+        __builtin_amdgcn_s_waitcnt(0x0f70);         // (as above)
     }
 
     // LDS operands are asked for AHEAD steps before the products that take them, and the compiler is kept from moving the reads back
@@ -306,6 +311,13 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
         }
         k.rare = __any(met) || k.y0 + 32 > yend;
         return k;
+    };
+    // Rows read where they lie that take no part and hold an infinity or NaN (rare; planes of fp32 hold zeros there) become zeros: every wave
+    // writes them before it reads the tile.
+    auto blank = [&](uint32_t buf) {
+        const float sign = *reinterpret_cast<const float *>(lds + NBUF * C::BUF + buf * 512 + kSign * 128 + (lane & 31) * 4);
+        for (uint32_t m = (uint32_t)__ballot(sign == 0.0f); m; m &= m - 1)
+            for (uint32_t c = lane; c < PITCH / 16; c += 64) reinterpret_cast<u32x4 *>(lds + buf * C::BUF + (__ffs(m) - 1) * PITCH)[c] = u32x4{0, 0, 0, 0};
     };
     // Rare: products are replaced so that the logits made of them come out as they should -- minus infinity for a target (whose logit is
     // set aside) and for rows behind the last; for a query's own row the logarithm of its weight, whose sign `flip` keeps.
@@ -484,6 +496,7 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
             for (uint32_t t = 0; t < ntiles; ++t) {
                 arrived(t, std::integral_constant<int, (NBUF > 1 ? NBUF - 2 : 0)>{});     // (every wave is through with tile t - 1)
                 if (NBUF > 1 && t + NBUF - 1 < ntiles) load(t + NBUF - 1);
+                if (MODE == kRows && !F32) blank(t % NBUF);
                 if (live) first_product(t % NBUF, S);
                 if constexpr (KQ > 1) {
                     part_out(S);

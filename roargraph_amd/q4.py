@@ -23,11 +23,15 @@ def _check_form(p):
         raise ValueError("codes: rows of uint8 on a GPU are wanted")
     if p.codes.shape[1] < -(-p.dim // 8) * 4:
         raise ValueError("codes: %d bytes a row, dim %d needs %d" % (p.codes.shape[1], p.dim, -(-p.dim // 8) * 4))
+    if nb > 1 and p.codes.stride(0) < p.codes.shape[1]:
+        raise ValueError("codes: rows that do not overlap are wanted, got strides %s" % (p.codes.stride(),))
     for t, name in ((p.scales, "scales"), (p.mins, "mins")):
         if t is None and name == "mins":
             continue
         if t.dtype != torch.float16 or t.shape != (nb, groups) or t.device != p.codes.device or (groups > 1 and t.stride(1) != 1):
             raise ValueError("%s: fp16 [%d, %d] on %s is wanted" % (name, nb, groups, p.codes.device))
+        if nb > 1 and t.stride(0) < groups:
+            raise ValueError("%s: rows that do not overlap are wanted, got strides %s" % (name, t.stride()))
     if p.mins is not None and nb > 1 and p.mins.stride(0) != p.scales.stride(0):
         raise ValueError("scales and mins have one row stride")
 
@@ -57,7 +61,9 @@ def q4_unpack(packed, ids=None):
     if ids is not None:
         if ids.dim() != 1 or ids.device != packed.codes.device or ids.dtype not in (torch.int32, torch.int64):
             raise ValueError("ids: a vector of int32 or int64 on %s is wanted" % packed.codes.device)
-        ids = ids.to(torch.int32).contiguous()
+        if ids.dtype == torch.int64:
+            ids = ids.clamp(-1, 0xffffffff).to(torch.int32)      # (what 32 bits cannot say becomes an id that is no row)
+        ids = ids.contiguous()
     n = nb if ids is None else ids.shape[0]
     out = torch.empty((n, packed.dim), dtype=torch.float32, device=packed.codes.device)
     check(lib().rg_q4_unpack_dev(_ptr(packed.codes), _stride(packed.codes), _ptr(packed.scales), _ptr(packed.mins), _stride(packed.scales), nb,

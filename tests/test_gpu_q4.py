@@ -182,6 +182,24 @@ def test_empty_and_refused():
             bad()
 
 
+def test_rows_that_overlap_are_refused():
+    """(an expanded matrix has no row stride: reading it as rows would leave the tensor)"""
+    p = q4.q4_pack(torch.randn(100, 24, device="cuda"), mins=True)
+    q = torch.zeros(1, 24, device="cuda")
+    for bad in (p._replace(scales=p.scales[:1].expand(100, 1), mins=p.mins[:1].expand(100, 1)), p._replace(codes=p.codes[:1].expand(100, 12)),
+                p._replace(mins=None, scales=p.scales[:1].expand(100, 1))):
+        for call in (lambda: q4.q4_score(q, bad), lambda: q4.q4_unpack(bad)):
+            with pytest.raises(ValueError, match="overlap"):
+                call()
+
+
+def test_ids_beyond_32_bits_are_no_rows():
+    p = q4.q4_pack(torch.randn(100, 24, device="cuda"))
+    got = q4.q4_unpack(p, torch.tensor([5, 2 ** 32 + 5, -2 ** 32, -1, 2 ** 31, 2 ** 40, 99, 100], device="cuda"))
+    want = q4.q4_unpack(p)
+    assert torch.equal(got[0], want[5]) and torch.equal(got[6], want[99]) and got[[1, 2, 3, 4, 5, 7]].isnan().all()
+
+
 def test_streams_and_graphs():
     p = q4.q4_pack(torch.randn(5000, 200, device="cuda"), mins=True)
     sets = [torch.randn(3, 200, device="cuda") for _ in range(3)]

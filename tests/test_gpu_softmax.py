@@ -91,7 +91,8 @@ def within(got, want, tol, what):
 
 SHAPES = [(1, 1, 1), (1, 17, 8), (3, 1000, 24), (64, 1000, 24), (65, 333, 33), (16, 16, 64), (17, 129, 7), (33, 31, 65), (130, 4097, 200), (64, 2048, 208), (40, 700, 209),
           (5, 513, 93), (100, 300, 128), (31, 900, 256), (70, 257, 257), (66, 1025, 384), (129, 515, 512), (20, 260, 513), (9, 400, 768), (19, 130, 1000), (35, 97, 1024),
-          (1, 30000, 200), (2000, 40, 96), (300, 20000, 16)]
+          (1, 30000, 200), (2000, 40, 96), (300, 20000, 16),
+          (70, 2000, 768), (200, 700, 700), (130, 3000, 1024), (64, 6000, 1000), (65, 500, 515), (90, 600, 385)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
@@ -287,6 +288,28 @@ def test_values_that_are_not_finite(dtype):
     tl, _, _ = tolerances(base, q, targets, w, scale, e, dtype)
     assert ((loss.double().cpu() - e["loss"]).abs() <= tl)[keep].all()
     assert not torch.isfinite(loss[~down]).any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nq,dim", [(20, 40), (70, 93), (97, 200), (33, 512), (70, 1024), (40, 771)])
+def test_queries_without_a_row_may_hold_anything(nq, dim, dtype):
+    base, q, targets, w, scale = make(nq, 300, dim, dtype, seed=nq)
+    out = torch.tensor([0, 3, 4, 19, nq - 1])
+    targets[out] = -1
+    q[out] = 0.0
+    want = step(base, q, targets, w, scale)
+    q[0], q[3, 1], q[4, dim - 1], q[19, 2], q[nq - 1, 0] = float("nan"), float("inf"), -float("inf"), float("nan"), float("nan")
+    loss, (dq, db) = step(base, q, targets, w, scale)
+    assert torch.equal(loss, want[0]) and torch.equal(dq, want[1][0]) and torch.equal(db, want[1][1])
+    assert not loss[out].any() and not dq[out].any()
+
+
+def test_targets_beyond_32_bits():
+    base, q, targets, w, scale = make(8, 100, 24, "f32", seed=3)
+    t = targets.long()
+    t[0], t[1], t[2], t[3] = 2 ** 32 + 5, -2 ** 32, 2 ** 40 - 1, -1
+    loss = softmax.softmax_loss(q.cuda(), base.cuda(), t.cuda(), scale).cpu()
+    assert (loss[:3] == np.inf).all() and loss[3] == 0 and torch.equal(loss[4:], softmax.softmax_loss(q.cuda(), base.cuda(), targets.cuda(), scale).cpu()[4:])
 
 
 def test_gradients_are_differences():

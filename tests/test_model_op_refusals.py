@@ -44,6 +44,7 @@ def unpack(codes=P, cs=16, scales=P, mins=0, ss=1, nb=100, dim=32, group=32, ids
     lambda: score(dim=4097, cs=2064, qs=4097, ss=200), lambda: score(cs=12), lambda: score(cs=18), lambda: score(codes=P + 2), lambda: score(ss=0), lambda: score(qs=31), lambda: score(os=99),
     lambda: score(dtype=9), lambda: score(out=P + 2), lambda: score(nb=1 << 31, os=1 << 31), lambda: score(mins=P + 1),
     lambda: pack(rows=0), lambda: pack(codes=0), lambda: pack(scales=0), lambda: pack(group=31), lambda: pack(stride=31), lambda: pack(cs=15), lambda: pack(dtype=5), lambda: pack(mins=P + 1),
+    lambda: shard(nq=1 << 24), lambda: grad(nq=1 << 24), lambda: score(cs=(1 << 26) + 4), lambda: score(ss=(1 << 25) + 1), lambda: score(nq=1 << 31), lambda: unpack(ids=P, n=1 << 31),
     lambda: unpack(codes=0), lambda: unpack(out=0), lambda: unpack(os=31), lambda: unpack(n=101), lambda: unpack(group=8),
 ])
 def test_refused(call):
@@ -53,7 +54,7 @@ def test_refused(call):
 
 def test_merge_refused():
     m = lib().rg_softmax_merge_dev
-    for args in ((0, P, 1, 5, P, P, P), (P, 0, 1, 5, P, P, P), (P, P, 0, 5, P, P, P), (P, P, 1, 5, 0, P, P), (P, P, 1, 5, P, 0, P), (P, P, 1, 5, P, P, 0)):
+    for args in ((0, P, 1, 5, P, P, P), (P, 0, 1, 5, P, P, P), (P, P, 0, 5, P, P, P), (P, P, 1, 5, 0, P, P), (P, P, 1, 5, P, 0, P), (P, P, 1, 5, P, P, 0), (P, P, 1, 1 << 24, P, P, P)):
         a = args
         assert m(vp(a[0]), vp(a[1]), u32(a[2]), u32(a[3]), vp(a[4]), vp(a[5]), vp(a[6]), C.c_int(0), vp(0)) == RG_ERR_ARG
 
