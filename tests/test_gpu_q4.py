@@ -200,6 +200,21 @@ def test_ids_beyond_32_bits_are_no_rows():
     assert torch.equal(got[0], want[5]) and torch.equal(got[6], want[99]) and got[[1, 2, 3, 4, 5, 7]].isnan().all()
 
 
+def test_rows_and_scores_beyond_4_gigabytes():
+    nb, dim = 5_000_000, 40
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    p = q4.q4_pack(torch.randn(nb, dim, device="cuda", generator=gen), mins=True)
+    far = p._replace(codes=torch.empty(nb, 1024, dtype=torch.uint8, device="cuda")[:, 900:900 + p.codes.shape[1]],
+                     scales=torch.empty(nb, 512, dtype=torch.float16, device="cuda")[:, 300:300 + p.scales.shape[1]], mins=torch.empty(nb, 512, dtype=torch.float16, device="cuda")[:, 7:7 + p.scales.shape[1]])
+    far.codes.copy_(p.codes), far.scales.copy_(p.scales), far.mins.copy_(p.mins)
+    q = torch.randn(3, dim, device="cuda", generator=gen)
+    out = torch.empty(3, 700_000_000, device="cuda")[:, 5:5 + nb]
+    want = q4.q4_score(q, p)
+    assert torch.equal(q4.q4_score(q, far, out=out), want) and torch.equal(out, want)
+    ids = torch.tensor([nb - 1, 0, nb // 2], device="cuda")
+    assert torch.equal(q4.q4_unpack(far, ids), q4.q4_unpack(p)[ids])
+
+
 def test_streams_and_graphs():
     p = q4.q4_pack(torch.randn(5000, 200, device="cuda"), mins=True)
     sets = [torch.randn(3, 200, device="cuda") for _ in range(3)]

@@ -312,6 +312,73 @@ def test_targets_beyond_32_bits():
     assert (loss[:3] == np.inf).all() and loss[3] == 0 and torch.equal(loss[4:], softmax.softmax_loss(q.cuda(), base.cuda(), targets.cuda(), scale).cpu()[4:])
 
 
+@pytest.mark.parametrize("dtype,nq,nb,dim", [("f32", 70, 4_300_000, 8), ("bf16", 70, 8_500_000, 5), ("f32", 5, 270_000, 1000)])
+def test_a_base_of_more_than_one_piece(dtype, nq, nb, dim):
+    """planes of fp32 and unaligned rows are made a gigabyte at a time; the sums go on from piece to piece"""
+    gen = torch.Generator(device="cuda").manual_seed(dim)
+    base = torch.randn(nb, dim, device="cuda", generator=gen).to(DT[dtype])
+    q = torch.randn(nq, dim, device="cuda", generator=gen).to(DT[dtype])
+    t = torch.randint(nb, (nq,), device="cuda", generator=gen, dtype=torch.int32)
+    t[0], t[1], t[2], t[3] = 0, nb - 1, 4194304 % nb, -1
+    w = torch.rand(nq, device="cuda", generator=gen) + 0.5
+    scale = 2.0 * dim ** -0.5
+    x = q.clone().requires_grad_()
+    loss = softmax.softmax_loss(x, base, t, scale)
+    dq, = torch.autograd.grad(loss, x, w)
+    assert torch.equal(softmax.softmax_loss(q, base, t, scale), loss)
+    e, parts = {}, [base[i:i + 200_000].double() for i in range(0, nb, 200_000)]
+    has, rows = t >= 0, torch.arange(nq, device="cuda")
+    tt = t.long().clamp(min=0)
+    own = scale * (q.double() * base[tt].double()).sum(1)
+    rest = torch.full((nq,), -np.inf, dtype=torch.float64, device="cuda")
+    for pass_ in (0, 1):
+        total, size = torch.zeros(nq, dim, dtype=torch.float64, device="cuda"), torch.zeros(nq, dim, dtype=torch.float64, device="cuda")
+        for i, b in enumerate(parts):
+            z = scale * (q.double() @ b.T.contiguous())
+            here = has & (tt >= 200_000 * i) & (tt < 200_000 * i + b.shape[0])
+            z[rows[here], tt[here] - 200_000 * i] = -np.inf
+            if pass_ == 0:
+                rest = torch.logaddexp(rest, torch.logsumexp(z, 1))
+            else:
+                p = torch.exp(z - e["lse"][:, None])
+                total += p @ b
+                size += p @ b.abs()
+        if pass_ == 0:
+            e["own"] = own.cpu()
+            e["loss"] = torch.where(has, torch.nn.functional.softplus(rest - own, threshold=1e9), 0.0).cpu()
+            e["lse"] = torch.where(has, torch.logaddexp(rest, own), rest)
+    ww = torch.where(has, w.double(), 0.0)[:, None]
+    miss = -torch.expm1(-e["loss"].cuda())[:, None]
+    mine = base[tt].double()
+    e["dq"] = (scale * ww * (total - miss * mine)).cpu()
+    e["aq"] = (scale * ww * (size + miss * mine.abs())).cpu()
+    top = float(base.double().norm(dim=1).max() * q.double().norm(dim=1).max() * scale)
+    dz = top * (dim + 8) * U + (3 * 2.0 ** -22 * dim ** 0.5 * top if dtype == "f32" else 0)
+    within(loss.detach(), e["loss"], 2 * dz + 4 * U * (e["loss"].abs() + e["own"].abs()) + 16 * U, "loss")
+    half, out = {"f32": (2.0 ** -22, U), "bf16": (2.0 ** -8, 2.0 ** -8)}[dtype]
+    largest = (ww[:, 0] * torch.maximum(miss[:, 0], torch.exp(top - e["lse"]))).cpu()[:, None]      # (no weight is larger)
+    floor = (0.0 if dtype == "bf16" else 2.0 ** -32) * largest * scale * sum(b.abs().sum(0) for b in parts).cpu()[None]
+    # sums in fp32: a few thousand terms a lane and slot, the lanes of an MFMA and the slots on top
+    within(dq, e["dq"], e["aq"] * (2 * dz + half + (nb / 64 + 4096) * U) + floor + out * e["dq"].abs() + 1e-38, "dq")
+
+
+@pytest.mark.parametrize("dtype,nq", [("bf16", 3), ("bf16", 70), ("f32", 70)])
+def test_rows_beyond_4_gigabytes(dtype, nq):
+    width = 2048 if dtype == "bf16" else 1024
+    base = torch.empty(1_200_000, width, dtype=DT[dtype], device="cuda")[:, 100 * 8 : 100 * 8 + 40]
+    gen = torch.Generator(device="cuda").manual_seed(nq)
+    base.copy_(torch.randn(base.shape, device="cuda", generator=gen))
+    q = torch.randn(nq, 40, device="cuda", generator=gen).to(DT[dtype])
+    t = torch.randint(1_200_000, (nq,), device="cuda", generator=gen, dtype=torch.int32)
+    t[-1] = 1_199_999
+    got, want = [], []
+    for b, to in ((base, got), (base.contiguous(), want)):
+        x, b = q.clone().requires_grad_(), b.detach().requires_grad_()
+        loss = softmax.softmax_loss(x, b, t, 0.2)
+        to += [loss.detach(), *torch.autograd.grad(loss.sum(), (x, b))]
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.isfinite(got[0]).all() and got[2][-1].any()
+
+
 def test_gradients_are_differences():
     """central differences of the loss the kernels give: h^2 / 6 times the third derivative, and the loss's rounding over h"""
     base, q, targets, _, _ = make(12, 90, 10, "f32", seed=13)
