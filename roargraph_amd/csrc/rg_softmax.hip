@@ -181,8 +181,7 @@ __global__ void __launch_bounds__(256) rg_softmax_planes_kernel(const void *rows
         uint16_t *out = planes + (size_t)r * NP * ks * 32;
         Chunk<DT> c[CI];
         const bool take = r < n && !(more && info[r / 32 * 128 + 64 + r % 32] == 0.0f);     // (not finite, and takes no part)
-#pragma unroll
-        for (int i = 0; i < CI; ++i) c[i] = load_chunk<DT>(row, 8 * (lc + 16 * i), take ? dim : 0);
+        load_chunks<DT, CI == 1>(c, row, 8 * lc, 128, dim, take);
         if constexpr (DT == RG_DTYPE_F32) {
             uint32_t m = 0;
 #pragma unroll

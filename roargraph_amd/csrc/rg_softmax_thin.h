@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
             const uint32_t y = y0 + lr + 16 * h;
             const char *row = static_cast<const char *>(A.y) + (size_t)y * A.ystride * esz;
 #pragma unroll
-            for (int i = 0; i < CI; ++i) stage[h][i] = load_chunk<DT>(row, 8 * (lc + 16 * i), y < yend ? dim : 0);
+            for (int i = 0; i < CI; ++i) stage[h][i] = fetch_chunk<DT, KS <= 2>(row, 8 * (lc + 16 * i), dim, y < yend);
         }
     };
     auto commit = [&](uint32_t buf) {
@@ -84,6 +84,9 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const uint32_t r = lr + 16 * h, sw = swizzle(r);
+            if (ragged<KS <= 2>(dim))
+#pragma unroll
+                for (int i = 0; i < CI; ++i) stage[h][i] = settle<DT>(stage[h][i], 8 * (lc + 16 * i), dim);
             int e = 0;
             float top = 0.0f;
             if constexpr (F32) {

@@ -481,9 +481,9 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
                 if (live) {
                     float p[NX][2][4];
                     const Tile k = look(t);
-                    if (k.rare) special(k, S);
+                    if (__builtin_expect(k.rare, 0)) special(k, S);
                     first_product((t + 1) % NBUF, next);                       // (behind the last tile: of old rows, for nobody)
-                    if (weigh_first(k, S, p)) move_all(k, S, p);
+                    if (__builtin_expect(weigh_first(k, S, p), 0)) move_all(k, S, p);
                     weigh_second(p);
 #pragma unroll
                     for (int j = 0; j < NX; ++j) { S[j][0] = next[j][0]; S[j][1] = next[j][1]; }
@@ -505,12 +505,12 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
                 if (live) {
                     if constexpr (KQ > 1) parts_in(S);
                     const Tile k = look(t);
-                    if (k.rare) special(k, S);
-                    if (weigh_first(k, S, p)) move_all(k, S, p);
+                    if (__builtin_expect(k.rare, 0)) special(k, S);
+                    if (__builtin_expect(weigh_first(k, S, p), 0)) move_all(k, S, p);
                     weigh_second(p);
                     if (MODE != kStats) {
                         pack(p, W);
-                        if (MODE == kRows && (k.rare || k.neg)) signs(k, W);
+                        if (MODE == kRows && __builtin_expect(k.rare || k.neg, 0)) signs(k, W);
                         second_product(t % NBUF, W);
                     }
                 }
