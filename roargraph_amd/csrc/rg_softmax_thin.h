@@ -15,8 +15,13 @@ struct ThinCfg {
     static constexpr int PITCH = (KS * 64 + 255) / 256 * 256;
     static constexpr int PLANE = TY * PITCH;
     static constexpr int BUF = NP * PLANE;
-    static constexpr int NBUF = 2 * BUF <= 128 * 1024 ? 2 : 1;
-    static constexpr int LDS = NBUF * (BUF + TY * 8);           // a factor and a bias per row
+    // tiles a turn: of short rows several, for the bytes that are on their way between two barriers (16 queries on 4M x 64, loss: fp16 one tile
+    // 257 us, four 124 us; fp32 one 518 us, two 309 us; on 2M x 128 fp16 one 140 us, two 115 us)
+    static constexpr int TURN = DT == RG_DTYPE_F32 ? (KS <= 4 ? 2 : 1) : KS <= 2 ? 4 : KS <= 4 ? 2 : 1;
+    static constexpr int LPR = KS < 4 ? 4 * KS : 16;            // lanes that load a row
+    static constexpr int ROWS = 256 / LPR, RPT = TURN * TY / ROWS;      // rows loaded at once, and by a thread
+    static constexpr int NBUF = 2 * TURN * BUF <= 128 * 1024 ? 2 : 1;
+    static constexpr int LDS = NBUF * TURN * (BUF + TY * 8);    // a factor and a bias per row
     static constexpr int WPS = (DT == RG_DTYPE_F32 ? KS <= 8 : KS <= 16) ? 2 : 1;
 };
 
@@ -66,24 +71,24 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
 
     if (A.resume) take_up<MODE, OB, NX>(A, x0, n, g, 0, split, M, Ml, l, O);
 
-    // streaming: 16 lanes per row, two rows per thread (r, r + 16)
-    const uint32_t lr = tid >> 4, lc = tid & 15;
-    Chunk<DT> stage[2][CI];
+    // streaming: LPR lanes per row, rows lr, lr + ROWS, .. per thread
+    const uint32_t lr = tid / C::LPR, lc = tid % C::LPR;
+    Chunk<DT> stage[C::RPT][CI];
     auto fetch = [&](uint32_t y0) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t y = y0 + lr + 16 * h;
+        for (int h = 0; h < C::RPT; ++h) {
+            const uint32_t y = y0 + lr + C::ROWS * h;
             const char *row = static_cast<const char *>(A.y) + (size_t)y * A.ystride * esz;
 #pragma unroll
             for (int i = 0; i < CI; ++i) stage[h][i] = fetch_chunk<DT, KS <= 2>(row, 8 * (lc + 16 * i), dim, y < yend);
         }
     };
     auto commit = [&](uint32_t buf) {
-        char *tile = lds + buf * C::BUF;
-        float *yv = reinterpret_cast<float *>(lds + C::NBUF * C::BUF) + buf * C::TY * 2;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t r = lr + 16 * h, sw = swizzle(r);
+        for (int h = 0; h < C::RPT; ++h) {
+            const uint32_t r = (lr + C::ROWS * h) % C::TY, t = buf * C::TURN + (lr + C::ROWS * h) / C::TY, sw = swizzle(r);
+            char *tile = lds + t * C::BUF;
+            float *yv = reinterpret_cast<float *>(lds + C::NBUF * C::TURN * C::BUF) + t * C::TY * 2;
             if (ragged<KS <= 2>(dim))
 #pragma unroll
                 for (int i = 0; i < CI; ++i) stage[h][i] = settle<DT>(stage[h][i], 8 * (lc + 16 * i), dim);
@@ -94,7 +99,7 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
 #pragma unroll
                 for (int i = 0; i < CI; ++i) m = max(m, __float_as_uint(absmax(stage[h][i])));
 #pragma unroll
-                for (int d = 1; d < 16; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
+                for (int d = 1; d < C::LPR; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
                 top = __uint_as_float(m);
                 e = row_exponent(top);
             }
@@ -121,9 +126,9 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
         }
     };
 
-    auto compute = [&](uint32_t buf, uint32_t y0) {
-        const char *tile = lds + buf * C::BUF;
-        const float *yv = reinterpret_cast<const float *>(lds + C::NBUF * C::BUF) + buf * C::TY * 2;
+    auto compute = [&](uint32_t t, uint32_t y0) {
+        const char *tile = lds + t * C::BUF;
+        const float *yv = reinterpret_cast<const float *>(lds + C::NBUF * C::TURN * C::BUF) + t * C::TY * 2;
         f32x4 S[2][NX];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -304,24 +309,30 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
     };
 
     if (ybeg < yend) {
+        constexpr uint32_t STEP = C::TURN * C::TY;
+        auto turn = [&](uint32_t buf, uint32_t y0) {
+            if (!live) return;
+#pragma unroll 1
+            for (uint32_t t = 0; t < C::TURN && y0 + t * C::TY < yend; ++t) compute(buf * C::TURN + t, y0 + t * C::TY);
+        };
         if constexpr (C::NBUF == 2) {
             fetch(ybeg);
             commit(0);
             __syncthreads();
             uint32_t buf = 0;
-            for (uint32_t y0 = ybeg; y0 < yend; y0 += 32, buf ^= 1) {
-                const bool more = y0 + 32 < yend;
-                if (more) fetch(y0 + 32);
-                if (live) compute(buf, y0);
+            for (uint32_t y0 = ybeg; y0 < yend; y0 += STEP, buf ^= 1) {
+                const bool more = y0 + STEP < yend;
+                if (more) fetch(y0 + STEP);
+                turn(buf, y0);
                 if (more) commit(buf ^ 1);
                 __syncthreads();
             }
         } else {
-            for (uint32_t y0 = ybeg; y0 < yend; y0 += 32) {
+            for (uint32_t y0 = ybeg; y0 < yend; y0 += STEP) {
                 fetch(y0);
                 commit(0);
                 __syncthreads();
-                if (live) compute(0, y0);
+                turn(0, y0);
                 __syncthreads();
             }
         }
