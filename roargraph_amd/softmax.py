@@ -147,19 +147,37 @@ def _softmax_function():
     if _function is None:
         import torch
 
+        # the calls of softmax_shard_dev and softmax_grad_dev with fewer tensors between them: rest, own, lse and the mean rows in one
         class SoftmaxLoss(torch.autograd.Function):
             @staticmethod
             def forward(ctx, queries, base, targets, scale):
-                rest, _, lse, loss, mean = softmax_shard_dev(base, queries, targets, scale, want_mean=ctx.needs_input_grad[0])
-                ctx.save_for_backward(queries, base, targets, lse, loss, rest, mean)
+                q, b = _rows(queries, "queries"), _rows(base, "base")
+                _check_pair(q, b)
+                (nq, dim), nb, code = q.shape, b.shape[0], _dtype_code(b)
+                want_mean = ctx.needs_input_grad[0]
+                loss = torch.empty(nq, dtype=torch.float32, device=b.device)
+                kept = torch.empty((3 + dim if want_mean else 3) * nq, dtype=torch.float32, device=b.device)
+                work, n = _scratch(MEAN if want_mean else STATS, nb, nq, dim, b)
+                at = kept.data_ptr()
+                check(lib().rg_softmax_shard_dev(b.data_ptr(), nb, _stride(b), q.data_ptr(), nq, _stride(q), dim, code, scale, targets.data_ptr(), 0, at, at + 4 * nq, at + 8 * nq,
+                                                 loss.data_ptr(), at + 12 * nq if want_mean else None, work.data_ptr(), n, _device(b), _stream(b)))
+                ctx.save_for_backward(queries, base, targets, loss, kept)
                 ctx.scale = scale
                 return loss
 
             @staticmethod
             @torch.autograd.function.once_differentiable
             def backward(ctx, weights):
-                queries, base, targets, lse, loss, rest, mean = ctx.saved_tensors
-                dq, db = softmax_grad_dev(base, queries, targets, ctx.scale, lse, loss, weights, rest=rest, mean=mean, want_dq=ctx.needs_input_grad[0], want_db=ctx.needs_input_grad[1])
+                queries, base, targets, loss, kept = ctx.saved_tensors
+                q, b = _rows(queries, "queries"), _rows(base, "base")
+                (nq, dim), nb, code = q.shape, b.shape[0], _dtype_code(b)
+                weights = weights.contiguous()
+                dq = torch.empty((nq, dim), dtype=b.dtype, device=b.device) if ctx.needs_input_grad[0] else None
+                db = torch.empty((nb, dim), dtype=b.dtype, device=b.device) if ctx.needs_input_grad[1] else None
+                work, n = _scratch(GRAD, nb if db is not None else 0, nq, dim, b)
+                at = kept.data_ptr()
+                check(lib().rg_softmax_grad_dev(b.data_ptr(), nb, _stride(b), q.data_ptr(), nq, _stride(q), dim, code, ctx.scale, targets.data_ptr(), 0, at + 8 * nq, loss.data_ptr(),
+                                                at, at + 12 * nq if dq is not None else None, weights.data_ptr(), _ptr(dq), dim, _ptr(db), dim, work.data_ptr(), n, _device(b), _stream(b)))
                 return dq, db, None, None
 
         _function = SoftmaxLoss
