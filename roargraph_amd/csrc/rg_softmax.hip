@@ -127,18 +127,22 @@ __device__ __forceinline__ void put_info(float *info, uint64_t y, float factor, 
     at[96] = __uint_as_float(target);
 }
 
-// per query: what the pass over the rows needs of it (info and ytarget, padded to whole tiles), and dq.  One wave per query.
+// per query: what the pass over the rows needs of it (info, ytarget and, where queries cannot be read where they lie, planes; padded to whole tiles),
+// and dq.  One wave per query.
 template <int DT>
 __global__ void __launch_bounds__(64) rg_softmax_dq_kernel(const void *queries, uint64_t qstride, const void *base, uint64_t bstride, uint32_t nb, uint32_t id_base, uint32_t nq, uint32_t dim, float scale,
                                                            const uint32_t *targets, const float *lse, const float *loss, const float *rest, const float *mean,
-                                                           const float *weights, void *dq, uint64_t dqstride, float *info, float *ytarget) {
+                                                           const float *weights, void *dq, uint64_t dqstride, float *info, float *ytarget, uint16_t *planes, uint32_t ks) {
     typedef typename Elem<DT>::T T;
+    constexpr uint32_t NP = DT == RG_DTYPE_F32 ? 2 : 1;
     const uint32_t i = blockIdx.x;
     if (i >= nq) {
         if (threadIdx.x == 0) {
             put_info(info, i, 1.0f, -INFINITY, 0.0f, kNoTarget);     // (copies of the last query: they take no part, whatever that holds)
             ytarget[i] = -INFINITY;
         }
+        if (planes)
+            for (uint32_t c = threadIdx.x; c < NP * ks * 4; c += 64) reinterpret_cast<u32x4 *>(planes + (size_t)i * NP * ks * 32)[c] = u32x4{0, 0, 0, 0};
         return;
     }
     const uint32_t t = targets[i], row = t - id_base;
@@ -149,10 +153,37 @@ __global__ void __launch_bounds__(64) rg_softmax_dq_kernel(const void *queries, 
         for (uint32_t k = threadIdx.x; k < dim; k += 64) whole &= fabsf((float)static_cast<const T *>(queries)[(size_t)i * qstride + k]) < INFINITY;
         whole = __all(whole);
     }
+    float factor = 1.0f, exponent = 0.0f;
+    if (planes) {                       // (zeros of a query that is not finite and takes no part)
+        Chunk<DT> c[2];
+        load_chunks<DT, true>(c, static_cast<const T *>(queries) + (size_t)i * qstride, 8 * threadIdx.x, 512, dim, whole);
+        uint16_t *out = planes + (size_t)i * NP * ks * 32;
+        if constexpr (DT == RG_DTYPE_F32) {
+            uint32_t m = max(__float_as_uint(absmax(c[0])), __float_as_uint(absmax(c[1])));
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
+            const float top = __uint_as_float(m);
+            const int e = row_exponent(top);
+            factor = row_factor(top, e);
+            exponent = (float)e;
+#pragma unroll
+            for (uint32_t u = 0; u < 2; ++u) {
+                if (threadIdx.x + 64 * u >= ks * 4) continue;
+                half8 hi, lo;
+                split8(c[u], top, pow2(-e), hi, lo);
+                *reinterpret_cast<half8 *>(out + 8 * (threadIdx.x + 64 * u)) = hi;
+                *reinterpret_cast<half8 *>(out + ks * 32 + 8 * (threadIdx.x + 64 * u)) = lo;
+            }
+        } else {
+#pragma unroll
+            for (uint32_t u = 0; u < 2; ++u)
+                if (threadIdx.x + 64 * u < ks * 4) *reinterpret_cast<u32x4 *>(out + 8 * (threadIdx.x + 64 * u)) = c[u].v;
+        }
+    }
     if (info && threadIdx.x == 0) {
         const float lw = log2f(fabsf(w));
-        put_info(info, i, 1.0f, t == kNoTarget ? -INFINITY : lw - lse[i] * kLog2e, w < 0.0f ? -1.0f : whole ? 1.0f : 0.0f, here ? row : kNoTarget);
-        ytarget[i] = lw + log2f(miss);
+        put_info(info, i, factor, t == kNoTarget ? -INFINITY : lw - lse[i] * kLog2e + exponent, w < 0.0f ? -1.0f : whole ? 1.0f : 0.0f, here ? row : kNoTarget);
+        ytarget[i] = lw + log2f(miss) + exponent;
     }
     if (!dq) return;
     const float part = rest[i] == -INFINITY ? 0.0f : expf(rest[i] - lse[i]);
@@ -168,11 +199,9 @@ __global__ void __launch_bounds__(64) rg_softmax_dq_kernel(const void *queries, 
 }
 
 // rows as the wide pass streams them: 16-bit planes of 32 ks elements, zeros behind dim and behind the last row; fp32 as two halves scaled by the
-// row's power of two, whose factor and exponent go to `info` (`more`: the exponent is added to what the queries' parameters already hold).
-// 16 lanes per row, CI chunks of 8 elements a lane.
+// row's power of two, whose factor and exponent go to `info`.  16 lanes per row, CI chunks of 8 elements a lane.
 template <int DT, int CI>
-__global__ void __launch_bounds__(256) rg_softmax_planes_kernel(const void *rows, uint64_t stride, uint32_t n, uint32_t npad, uint32_t dim, uint32_t ks, uint16_t *planes, float *info, float *ytarget,
-                                                                int more) {
+__global__ void __launch_bounds__(256) rg_softmax_planes_kernel(const void *rows, uint64_t stride, uint32_t n, uint32_t npad, uint32_t dim, uint32_t ks, uint16_t *planes, float *info) {
     typedef typename Elem<DT>::T T;
     constexpr int NP = DT == RG_DTYPE_F32 ? 2 : 1;
     const uint32_t lc = threadIdx.x % 16;
@@ -180,7 +209,7 @@ __global__ void __launch_bounds__(256) rg_softmax_planes_kernel(const void *rows
         const char *row = static_cast<const char *>(rows) + (size_t)r * stride * sizeof(T);
         uint16_t *out = planes + (size_t)r * NP * ks * 32;
         Chunk<DT> c[CI];
-        const bool take = r < n && !(more && info[r / 32 * 128 + 64 + r % 32] == 0.0f);     // (not finite, and takes no part)
+        const bool take = r < n;
         load_chunks<DT, CI == 1>(c, row, 8 * lc, 128, dim, take);
         if constexpr (DT == RG_DTYPE_F32) {
             uint32_t m = 0;
@@ -198,16 +227,7 @@ __global__ void __launch_bounds__(256) rg_softmax_planes_kernel(const void *rows
                 *reinterpret_cast<half8 *>(out + 8 * (lc + 16 * i)) = hi;
                 *reinterpret_cast<half8 *>(out + ks * 32 + 8 * (lc + 16 * i)) = lo;
             }
-            if (lc == 0) {
-                if (more) {
-                    float *at = info + (r / 32 * 128 + r % 32);
-                    at[0] = row_factor(top, e);
-                    at[32] += (float)e;
-                    ytarget[r] += (float)e;
-                } else {
-                    put_info(info, r, row_factor(top, e), (float)e, 1.0f, kNoTarget);
-                }
-            }
+            if (lc == 0) put_info(info, r, row_factor(top, e), (float)e, 1.0f, kNoTarget);
         } else {
 #pragma unroll
             for (int i = 0; i < CI; ++i)
@@ -261,7 +281,7 @@ SoftmaxKernel kernel_of(int dtype, int mode, bool thin, int ks) {
 // 600 Top/s of the 16-bit passes, 4 TB/s).  333 fp16 queries on 70001 rows of 93 dims: 3 slots, which leave fewer places empty, took
 // 80 us + 29 us to join for the gradient of the rows, 1 slot 58 us.
 // With and without the mean, a call is cut alike (for the sum of both costs), so that both give the same loss.
-constexpr double kOpsPerByte = 150;
+constexpr double kOpsPerByte = 150, kLaunchCost = 16e6;     // (bytes of the 4 us of a launch)
 struct Use {                          // of the device by a kernel
     uint64_t nt, places;              // workgroups of a slot; workgroups that run at once
     double row_cost;                  // bytes of a row y, were all places used
@@ -289,7 +309,7 @@ struct Plan {
         double least = HUGE_VAL;
         auto look = [&](uint64_t n_) {
             const uint32_t n = (uint32_t)std::clamp<uint64_t>(n_, 1, most);
-            double cost = n == 1 && free_slot ? 0.0 : nuse * n * slot_cost;
+            double cost = n == 1 && free_slot ? 0.0 : nuse * n * slot_cost + (free_slot ? kLaunchCost : 0.0);
             for (int u = 0; u < nuse; ++u) cost += use[u].busy(rows, n);
             if (cost < least || (cost == least && n < best)) { least = cost; best = n; }
         };
@@ -379,10 +399,10 @@ bool direct_rows(const void *rows, uint64_t stride, uint32_t dim, int dtype) {
 float k_of(float scale) { return scale == 0.0f ? 1e-30f : scale * kLog2e; }
 
 template <int DT>
-rg_status make_planes(const void *rows, uint64_t stride, uint32_t n, uint32_t dim, int ks, void *planes, float *info, float *ytarget, hipStream_t s) {
+rg_status make_planes(const void *rows, uint64_t stride, uint32_t n, uint32_t dim, int ks, void *planes, float *info, hipStream_t s) {
     auto kern = ks <= 4 ? rg_softmax_planes_kernel<DT, 1> : ks <= 8 ? rg_softmax_planes_kernel<DT, 2> : ks <= 16 ? rg_softmax_planes_kernel<DT, 4> : rg_softmax_planes_kernel<DT, 8>;
     const uint32_t npad = up32(n);
-    hipLaunchKernelGGL(kern, dim3(std::min(npad / 16, 1u << 16)), dim3(256), 0, s, rows, stride, n, npad, dim, (uint32_t)ks, static_cast<uint16_t *>(planes), info, ytarget, ytarget ? 1 : 0);
+    hipLaunchKernelGGL(kern, dim3(std::min(npad / 16, 1u << 16)), dim3(256), 0, s, rows, stride, n, npad, dim, (uint32_t)ks, static_cast<uint16_t *>(planes), info);
     RG_HIP(hipGetLastError());
     return RG_OK;
 }
@@ -461,7 +481,7 @@ rg_status shard(const Call &c, float *rest, float *own, float *lse, float *loss,
         A.resume = y != 0;
         if (p.planes && n) {
             float *info = reinterpret_cast<float *>(c.work + L.info);
-            rg_status st = make_planes<DT>(A.y, c.bstride, n, c.dim, p.ks, c.work + L.planes, info, nullptr, c.s);
+            rg_status st = make_planes<DT>(A.y, c.bstride, n, c.dim, p.ks, c.work + L.planes, info, c.s);
             if (st != RG_OK) return st;
             A.y = c.work + L.planes; A.ystride = p.row_bytes / 2; A.ydim = 32 * p.ks; A.yinfo = info;
         }
@@ -480,9 +500,10 @@ rg_status grad(const Call &c, const float *lse, const float *loss, const float *
     const Layout L = layout_of(p, kRows, DT, c.dim);
     float *info = rows ? reinterpret_cast<float *>(c.work + L.info) : nullptr;
     float *ytarget = rows ? reinterpret_cast<float *>(c.work + L.aux) : nullptr;
+    uint16_t *planes = p.planes && rows && c.nq ? reinterpret_cast<uint16_t *>(c.work + L.planes) : nullptr;
     if (c.nq) {
         hipLaunchKernelGGL((rg_softmax_dq_kernel<DT>), dim3(rows ? up32(c.nq) : c.nq), dim3(64), 0, c.s, c.queries, c.qstride, c.base, c.bstride, c.nb, c.id_base, c.nq, c.dim, c.scale, c.targets, lse, loss, rest, mean, weights,
-                           dq, dqstride, info, ytarget);
+                           dq, dqstride, info, ytarget, planes, (uint32_t)p.ks);
         RG_HIP(hipGetLastError());
     }
     if (!rows) return RG_OK;
@@ -497,9 +518,7 @@ rg_status grad(const Call &c, const float *lse, const float *loss, const float *
     A.o = reinterpret_cast<float *>(c.work + L.o);
     A.yinfo = info; A.ytarget = ytarget;
     A.out = db; A.ostride = dbstride; A.oscale = c.scale;
-    if (p.planes && c.nq) {
-        rg_status st = make_planes<DT>(c.queries, c.qstride, c.nq, c.dim, p.ks, c.work + L.planes, info, ytarget, c.s);
-        if (st != RG_OK) return st;
+    if (planes) {
         A.y = c.work + L.planes; A.ystride = p.row_bytes / 2; A.ydim = 32 * p.ks;
     }
     rg_status st = launch_pass(p, A, c.s);
