@@ -26,7 +26,8 @@ namespace rg {
 namespace {
 
 constexpr uint32_t kMaxDim = 1024, kMaxQueries = (1u << 24) - 1;     // (a workgroup of 256 each, and a launch holds less than 2^32 threads)
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLn2 = 0.6931471805599453;
 
 __device__ __forceinline__ bool target_here(uint32_t t, uint32_t id_base, uint32_t nb) { return t != kNoTarget && t >= id_base && t - id_base < nb; }
 
@@ -68,9 +69,10 @@ __global__ void __launch_bounds__(256) rg_softmax_join_kernel(const float4 *ml, 
     if (tid == 0 && blockIdx.y == 0) {
         const uint32_t t = targets[i];
         const bool here = target_here(t, id_base, nb);
-        const float r = none ? -INFINITY : (M + log2f(l)) * kLn2;
-        const float z = here ? own2[i] * kLn2 : -INFINITY;
-        const float v = here ? softplus(r - z) : t == kNoTarget ? 0.0f : INFINITY;
+        // (in 64 bits: the instruction behind log2f rounds down, which a small loss shows)
+        const double r2 = none ? -INFINITY : (double)M + log2((double)l), z2 = here ? own2[i] : -INFINITY;
+        const float r = (float)(r2 * kLn2), z = (float)(z2 * kLn2);
+        const float v = here ? softplus((float)((r2 - z2) * kLn2)) : t == kNoTarget ? 0.0f : INFINITY;
         rest[i] = r;
         own[i] = z;
         if (lse) lse[i] = here ? z + v : r;
@@ -181,9 +183,9 @@ __global__ void __launch_bounds__(64) rg_softmax_dq_kernel(const void *queries, 
         }
     }
     if (info && threadIdx.x == 0) {
-        const float lw = log2f(fabsf(w));
+        const float lw = (float)log2((double)fabsf(w));
         put_info(info, i, factor, t == kNoTarget ? -INFINITY : lw - lse[i] * kLog2e + exponent, w < 0.0f ? -1.0f : whole ? 1.0f : 0.0f, here ? row : kNoTarget);
-        ytarget[i] = lw + log2f(miss) + exponent;
+        ytarget[i] = lw + (float)log2((double)miss) + exponent;
     }
     if (!dq) return;
     const float part = rest[i] == -INFINITY ? 0.0f : expf(rest[i] - lse[i]);

@@ -226,24 +226,23 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
                         top = fmaxf(top, p[h][i]);
                     }
                 const bool move = __any(top > kTop);
-                if (move) {
+                if (move) {                                     // (of the rows that need it, whatever the others do)
                     float z = kNothing;
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            p[h][i] = logit(h, i, biased, 0.0f);
-                            z = fmaxf(z, p[h][i]);
-                        }
+                        for (int i = 0; i < 4; ++i) z = fmaxf(z, logit(h, i, biased, 0.0f));
                     z = fmaxf(z, __shfl_xor(z, 16));
                     z = fmaxf(z, __shfl_xor(z, 32));
-                    const float to = z - ref > kTop ? z - kStart : ref;
+                    top = fmaxf(top, __shfl_xor(top, 16));
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    const float to = top > kTop ? z - kStart : ref;
                     old = exp2_hw(ref - to);
                     ref = to;
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) p[h][i] -= to;
+                        for (int i = 0; i < 4; ++i) p[h][i] = logit(h, i, biased, ref);
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h)

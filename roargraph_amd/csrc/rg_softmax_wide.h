@@ -369,29 +369,32 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
                 for (int i = 0; i < 4; ++i) top = fmaxf(top, p[j][h][i]);
         return top > kTop;
     };
-    // moves the references of the rows that need it; leaves the logits minus the new ones, and what the sums so far are multiplied by
+    // moves the references of the rows that need it -- p: the logits minus the old ones --, whatever other rows of the wave do (so that results do
+    // not depend on which rows share one); leaves the logits minus the new ones, and what the sums so far are multiplied by
     auto move = [&](const Tile &k, const f32x4 (&S)[NX][2], bool biased, float (&ref)[NX], float (&p)[NX][2][4], float (&old)[NX]) {
-        float zero[NX];
-#pragma unroll
-        for (int j = 0; j < NX; ++j) zero[j] = 0.0f;
-        logits(k, S, biased, zero, p);
-#pragma unroll
-        for (int j = 0; j < NX; ++j) {
+        float zero[NX], above[NX];
+        auto largest = [&](int j) {
             float z = kNothing;
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) z = fmaxf(z, p[j][h][i]);
             z = fmaxf(z, __shfl_xor(z, 16));
-            z = fmaxf(z, __shfl_xor(z, 32));
-            const float to = z - ref[j] > kTop ? z - kStart : ref[j];
+            return fmaxf(z, __shfl_xor(z, 32));
+        };
+#pragma unroll
+        for (int j = 0; j < NX; ++j) {
+            above[j] = largest(j);
+            zero[j] = 0.0f;
+        }
+        logits(k, S, biased, zero, p);
+#pragma unroll
+        for (int j = 0; j < NX; ++j) {
+            const float z = largest(j), to = above[j] > kTop ? z - kStart : ref[j];
             old[j] = exp2_hw(ref[j] - to);
             ref[j] = to;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) p[j][h][i] -= to;
         }
+        logits(k, S, biased, ref, p);
     };
     auto sum = [&](const float (&p)[2][4]) { return ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3])); };
     auto exps = [&](float (&p)[NX][2][4]) {
