@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(64) rg_softmax_dq_kernel(const void *queries, 
         for (uint32_t k = threadIdx.x; k < dim; k += 64) whole &= fabsf((float)static_cast<const T *>(queries)[(size_t)i * qstride + k]) < INFINITY;
         whole = __all(whole);
     }
-    float factor = 1.0f, exponent = 0.0f;
+    float factor = 1.0f;
     if (planes) {                       // (zeros of a query that is not finite and takes no part)
         Chunk<DT> c[2];
         load_chunks<DT, true>(c, static_cast<const T *>(queries) + (size_t)i * qstride, 8 * threadIdx.x, 512, dim, whole);
@@ -167,7 +167,6 @@ __global__ void __launch_bounds__(64) rg_softmax_dq_kernel(const void *queries, 
             const float top = __uint_as_float(m);
             const int e = row_exponent(top);
             factor = row_factor(top, e);
-            exponent = (float)e;
 #pragma unroll
             for (uint32_t u = 0; u < 2; ++u) {
                 if (threadIdx.x + 64 * u >= ks * 4) continue;
@@ -184,8 +183,8 @@ __global__ void __launch_bounds__(64) rg_softmax_dq_kernel(const void *queries, 
     }
     if (info && threadIdx.x == 0) {
         const float lw = (float)log2((double)fabsf(w));
-        put_info(info, i, factor, t == kNoTarget ? -INFINITY : lw - lse[i] * kLog2e + exponent, w < 0.0f ? -1.0f : whole ? 1.0f : 0.0f, here ? row : kNoTarget);
-        ytarget[i] = lw + (float)log2((double)miss) + exponent;
+        put_info(info, i, factor, t == kNoTarget ? -INFINITY : lw - lse[i] * kLog2e, w < 0.0f ? -1.0f : whole ? 1.0f : 0.0f, here ? row : kNoTarget);
+        ytarget[i] = lw + (float)log2((double)miss);
     }
     if (!dq) return;
     const float part = rest[i] == -INFINITY ? 0.0f : expf(rest[i] - lse[i]);
@@ -397,9 +396,6 @@ uint64_t scratch_of(int mode, uint32_t nb, uint32_t nq, uint32_t dim, int dtype)
 bool direct_rows(const void *rows, uint64_t stride, uint32_t dim, int dtype) {
     return dtype != RG_DTYPE_F32 && dim % 8 == 0 && stride % 8 == 0 && stride < (1u << 25) && (uintptr_t)rows % 16 == 0;     // (32 rows' bytes in 32 bits)
 }
-// scale in units of log 2; a scale of zero becomes one that no product makes visible (replaced products are divided by it)
-float k_of(float scale) { return scale == 0.0f ? 1e-30f : scale * kLog2e; }
-
 template <int DT>
 rg_status make_planes(const void *rows, uint64_t stride, uint32_t n, uint32_t dim, int ks, void *planes, float *info, hipStream_t s) {
     auto kern = ks <= 4 ? rg_softmax_planes_kernel<DT, 1> : ks <= 8 ? rg_softmax_planes_kernel<DT, 2> : ks <= 16 ? rg_softmax_planes_kernel<DT, 4> : rg_softmax_planes_kernel<DT, 8>;
@@ -437,7 +433,7 @@ rg_status check_call(uint32_t nb, const void *base, uint64_t bstride, uint32_t n
     if (st == RG_OK) st = check_rows(base, nb, bstride, dim, dtype, "base");
     if (st == RG_OK) st = check_rows(queries, nq, qstride, dim, dtype, "queries");
     if (st != RG_OK) return st;
-    if (!std::isfinite(scale)) return set_error(RG_ERR_ARG, "the scale must be finite");
+    if (!std::isfinite(scale * kLog2e)) return set_error(RG_ERR_ARG, "the scale must be finite, and below 2e38");
     if ((uint64_t)id_base + nb > 0xffffffffull) return set_error(RG_ERR_ARG, "row ids beyond 2^32 - 2");
     return RG_OK;
 }
@@ -467,7 +463,7 @@ rg_status shard(const Call &c, float *rest, float *own, float *lse, float *loss,
     PassArgs A{};
     A.x = c.queries; A.xstride = c.qstride; A.nx = c.nq;
     A.dim = A.ydim = c.dim;
-    A.k = k_of(c.scale);
+    A.k = c.scale * kLog2e;
     A.opitch = opitch_of(c.dim);
     A.targets = c.targets; A.own2 = reinterpret_cast<float *>(c.work + L.aux);
     float4 *ml = reinterpret_cast<float4 *>(c.work + L.ml);
@@ -514,7 +510,7 @@ rg_status grad(const Call &c, const float *lse, const float *loss, const float *
     A.x = c.base; A.xstride = c.bstride; A.nx = rows;
     A.y = c.queries; A.ystride = c.qstride; A.ny = c.nq;
     A.dim = A.ydim = c.dim;
-    A.k = k_of(c.scale);
+    A.k = c.scale * kLog2e;
     A.nsplit = cut.nsplit; A.rows_per_split = cut.rows; A.opitch = opitch_of(c.dim);
     A.ml = reinterpret_cast<float4 *>(c.work + L.ml);
     A.o = reinterpret_cast<float *>(c.work + L.o);

@@ -44,7 +44,7 @@ struct PassArgs {
     uint32_t id_base;
     float *own2;                       // kStats, kMean: z2 of the target, written where it is met
     const float *yinfo;                // fp32 rows and kRows, per 32 rows y: 32 factors and biases of a logit, signs of the weight, target rows (bits)
-    const float *ytarget;              // kRows, per y: the biased logit of its own row, log2(|w| (1 - p_target)) (+ the exponent of the row)
+    const float *ytarget;              // kRows, per y: the biased logit of its own row, log2(|w| (1 - p_target))
     void *out;                         // kRows in one piece: the gradient itself
     uint64_t ostride;
     float oscale;

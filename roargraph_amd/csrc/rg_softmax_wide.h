@@ -309,7 +309,7 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
             met = __float_as_uint(info(k, kTarget, lane & 31)) - x0 < 16 * NX;
             k.neg = __any(info(k, kSign, lane & 31) < 0.0f);
         }
-        k.rare = __any(met) || k.y0 + 32 > yend;
+        k.rare = __any(met) || (MODE != kRows && k.y0 + 32 > yend);      // (kRows: rows behind the last have no weight as it is)
         return k;
     };
     // Rows read where they lie that take no part and hold an infinity or NaN (rare; planes of fp32 hold zeros there) become zeros: every wave
@@ -319,34 +319,41 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
         for (uint32_t m = (uint32_t)__ballot(sign == 0.0f); m; m &= m - 1)
             for (uint32_t c = lane; c < PITCH / 16; c += 64) reinterpret_cast<u32x4 *>(lds + buf * C::BUF + (__ffs(m) - 1) * PITCH)[c] = u32x4{0, 0, 0, 0};
     };
-    // Rare: products are replaced so that the logits made of them come out as they should -- minus infinity for a target (whose logit is
-    // set aside) and for rows behind the last; for a query's own row the logarithm of its weight, whose sign `flip` keeps.
-    uint32_t flip[NX];
-    auto special = [&](const Tile &k, f32x4 (&S)[NX][2]) {
+    // Rare: elements of a tile whose weight is not made of their product: bit 4 h + i of those that take no part (a target, whose logit is set aside;
+    // rows behind the last), or in kRows of a query's own row, which has the logarithm of its weight, and whose sign turns.
+    // (Every instruction here is fetched from memory when it comes to it: as 24 branches a tile it took a workgroup 25 us.)
+    uint32_t off_bits[NX];
+    auto special = [&](const Tile &k, const f32x4 (&S)[NX][2]) {
+        auto bit_of = [&](uint32_t r) { return (r >> 2 & 3) == g ? 1u << (4 * (r >> 4) + (r & 3)) : 0u; };      // of row r < 32, where it lies in this lane
+        if constexpr (MODE == kRows) {
 #pragma unroll
-        for (int j = 0; j < NX; ++j) {
-            flip[j] = 0;
-            const uint32_t x = x0 + j * 16 + n;
+            for (int j = 0; j < NX; ++j) off_bits[j] = 0;
+            const uint32_t at = __float_as_uint(info(k, kTarget, lane & 31)) - x0;
+            for (uint32_t m = (uint32_t)__ballot(at < 16 * NX); m; m &= m - 1) {
+                const uint32_t r = __ffs(m) - 1, x = __builtin_amdgcn_readlane(at, r);
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+                for (int j = 0; j < NX; ++j) off_bits[j] |= x == 16 * j + n ? bit_of(r) : 0;
+            }
+        } else {
+            uint32_t behind = 0;
+            if (k.y0 + 32 > yend)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t r = 16 * h + 4 * g + i;
-                    const float f = INFO ? kx[j] * info(k, kFactor, r) : kx[j];
-                    bool dead = k.y0 + r >= yend;
-                    if (MODE != kRows && k.y0 + r == target[j]) {
-                        if (kq == 0) A.own2[x] = S[j][h][i] * f;
-                        dead = true;
-                    }
-                    if (MODE == kRows && __float_as_uint(info(k, kTarget, r)) == x) {
-                        const float bias = info(k, kBias, r);
-                        if (bias > -INFINITY) S[j][h][i] = (A.ytarget[k.y0 + r] - bias) / f;
-                        flip[j] |= 1u << (4 * h + i);
-                    }
-                    if (dead) S[j][h][i] = copysignf(INFINITY, -f);
-                }
+                for (int h = 0; h < 2; ++h) behind |= (15u << max(min((int)(yend - k.y0) - (int)(16 * h + 4 * g), 4), 0) & 15u) << (4 * h);
+#pragma unroll
+            for (int j = 0; j < NX; ++j) {
+                const uint32_t r = target[j] - k.y0, mine = r < 32 ? bit_of(r) : 0;
+                off_bits[j] = behind | mine;
+                float z = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z = mine >> e & 1 ? S[j][e / 4][e % 4] : z;
+                if (kq == 0 && mine) A.own2[x0 + 16 * j + n] = z * (INFO ? kx[j] * info(k, kFactor, r) : kx[j]);
+            }
         }
     };
+    // the exponent of a row y's own scale, which its weights carry in kRows (kMean: it is the bias).  It is taken from a reference first, which is
+    // exact, so that a bias keeps its digits however large both are.
+    auto exponent = [](float factor) { return (float)((int)(__float_as_uint(factor) >> 23) - 127); };
+    constexpr bool SCALED = F32 && MODE == kRows;
     auto logits = [&](const Tile &k, const f32x4 (&S)[NX][2], bool biased, const float (&ref)[NX], float (&p)[NX][2][4]) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -354,12 +361,28 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
             if (F32) factor = info4(k, kFactor, h);
             if (BIAS) bias = info4(k, kBias, h);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i) {
+                const float e = SCALED ? exponent(factor[i]) : 0.0f;
 #pragma unroll
-                for (int j = 0; j < NX; ++j) p[j][h][i] = fmaf(F32 ? S[j][h][i] * factor[i] : S[j][h][i], kx[j], biased ? bias[i] - ref[j] : -ref[j]);
+                for (int j = 0; j < NX; ++j) p[j][h][i] = fmaf(F32 ? S[j][h][i] * factor[i] : S[j][h][i], kx[j], SCALED ? bias[i] + (e - ref[j]) : biased ? bias[i] - ref[j] : -ref[j]);
+            }
         }
+        if (__builtin_expect(k.rare, 0))
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                f32x4 own{0.0f, 0.0f, 0.0f, 0.0f}, factor = own;
+                if (MODE == kRows) own = *reinterpret_cast<const f32x4 *>(A.ytarget + (k.y0 + 16 * h + 4 * g));
+                if (SCALED) factor = info4(k, kFactor, h);
+#pragma unroll
+                for (int j = 0; j < NX; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float v = MODE == kRows ? own[i] + ((SCALED ? exponent(factor[i]) : 0.0f) - ref[j]) : -INFINITY;
+                        p[j][h][i] = off_bits[j] >> (4 * h + i) & 1 ? v : p[j][h][i];
+                    }
+            }
     };
-    auto over = [&](const float (&p)[NX][2][4]) {
+    auto over = [&](const auto &p) {
         float top = kNothing;
 #pragma unroll
         for (int j = 0; j < NX; ++j)
@@ -369,10 +392,11 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
                 for (int i = 0; i < 4; ++i) top = fmaxf(top, p[j][h][i]);
         return top > kTop;
     };
-    // moves the references of the rows that need it -- p: the logits minus the old ones --, whatever other rows of the wave do (so that results do
-    // not depend on which rows share one); leaves the logits minus the new ones, and what the sums so far are multiplied by
-    auto move = [&](const Tile &k, const f32x4 (&S)[NX][2], bool biased, float (&ref)[NX], float (&p)[NX][2][4], float (&old)[NX]) {
-        float zero[NX], above[NX];
+    // Rare: a logit p passes its reference by kTop.  The references of those rows move -- of those only, so that results do not depend on which rows
+    // share a wave --, the logits are made anew, and `moved` multiplies what was summed under the old references.  (The loop leaves one copy of
+    // the code; a first turn in it, for all tiles, cost 2 %: nothing moves between it and the products.)
+    auto relocate = [&](const Tile &k, const f32x4 (&S)[NX][2], bool biased, float (&ref)[NX], float (&p)[NX][2][4], auto &&moved) {
+        float under[NX], above[NX], old[NX];
         auto largest = [&](int j) {
             float z = kNothing;
 #pragma unroll
@@ -385,19 +409,24 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
 #pragma unroll
         for (int j = 0; j < NX; ++j) {
             above[j] = largest(j);
-            zero[j] = 0.0f;
+            under[j] = 0.0f;
+            old[j] = 1.0f;
         }
-        logits(k, S, biased, zero, p);
+#pragma clang loop unroll(disable)
+        for (int turn = 0; turn < 2; ++turn) {
+            logits(k, S, biased, under, p);
+            if (turn == 0)
 #pragma unroll
-        for (int j = 0; j < NX; ++j) {
-            const float z = largest(j), to = above[j] > kTop ? z - kStart : ref[j];
-            old[j] = exp2_hw(ref[j] - to);
-            ref[j] = to;
+                for (int j = 0; j < NX; ++j) {
+                    under[j] = above[j] > kTop ? largest(j) - kStart : ref[j];
+                    old[j] = exp2_hw(ref[j] - under[j]);
+                    ref[j] = under[j];
+                }
         }
-        logits(k, S, biased, ref, p);
+        moved(old);
     };
     auto sum = [&](const float (&p)[2][4]) { return ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3])); };
-    auto exps = [&](float (&p)[NX][2][4]) {
+    auto exps = [&](auto &p) {
 #pragma unroll
         for (int j = 0; j < NX; ++j)
 #pragma unroll
@@ -426,7 +455,7 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
         for (int e = 0; e < 8; ++e) minus[e / 2] |= (__float_as_uint(info(k, kSign, 16 * (e / 4) + 4 * g + e % 4)) & 0x80000000u) >> (e % 2 ? 0 : 16);
 #pragma unroll
         for (int j = 0; j < NX; ++j) {
-            const uint32_t f = k.rare ? flip[j] : 0;
+            const uint32_t f = k.rare ? off_bits[j] : 0;
 #pragma unroll
             for (int q = 0; q < NP; ++q) {
                 u32x4 v = __builtin_bit_cast(u32x4, W[j][q]);
@@ -436,40 +465,42 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
             }
         }
     };
-    // the weights of a tile, in two halves
-    float pl[TWO ? NX : 1][2][4];
-    auto weigh_first = [&](const Tile &k, const f32x4 (&S)[NX][2], float (&p)[NX][2][4]) {
-        if constexpr (TWO) logits(k, S, false, Ml, pl);
-        logits(k, S, BIAS, M, p);
-        bool o = !NOREF && over(p);
-        if constexpr (TWO) o |= over(pl);
-        return !NOREF && __any(o);
-    };
-    auto move_all = [&](const Tile &k, const f32x4 (&S)[NX][2], float (&p)[NX][2][4]) {
-        float old[NX];
-        if constexpr (TWO) {
-            move(k, S, false, Ml, pl, old);
+    // the weights of a tile, and their sums
+    auto weights = [&](const Tile &k, const f32x4 (&S)[NX][2], float (&p)[NX][2][4]) {
+        auto add = [&](const auto &v) {
+#pragma unroll
+            for (int j = 0; j < NX; ++j) l[j] += sum(v[j]);
+        };
+        auto scale_l = [&](const float (&old)[NX]) {
 #pragma unroll
             for (int j = 0; j < NX; ++j) l[j] *= old[j];
+        };
+        float pl[TWO ? NX : 1][2][4];
+        bool high = false;
+        if constexpr (TWO) {
+            logits(k, S, false, Ml, pl);
+            high = over(pl);
         }
-        move(k, S, BIAS, M, p, old);
+        logits(k, S, BIAS, M, p);
+        if (!NOREF) high |= over(p);
+        if (!NOREF && __builtin_expect(__any(high), 0)) {
+            if constexpr (TWO) relocate(k, S, false, Ml, pl, scale_l);
+            relocate(k, S, BIAS, M, p, [&](const float (&old)[NX]) {
+                if (!TWO) scale_l(old);
+                if (MODE != kStats)
 #pragma unroll
-        for (int j = 0; j < NX; ++j) {
-            if (!TWO) l[j] *= old[j];
-            if (MODE != kStats)
+                    for (int j = 0; j < NX; ++j)
 #pragma unroll
-                for (int ob = 0; ob < OW; ++ob) O[ob][j] *= old[j];
+                        for (int ob = 0; ob < OW; ++ob) O[ob][j] *= old[j];
+            });
         }
-    };
-    auto weigh_second = [&](float (&p)[NX][2][4]) {
         exps(p);
-        if constexpr (TWO) exps(pl);
-        if (MODE != kRows)
-#pragma unroll
-            for (int j = 0; j < NX; ++j) {
-                if constexpr (TWO) l[j] += sum(pl[j]);
-                else l[j] += sum(p[j]);
-            }
+        if constexpr (TWO) {
+            exps(pl);
+            add(pl);
+        } else if (MODE != kRows) {
+            add(p);
+        }
     };
 
     if (ntiles) {
@@ -486,8 +517,7 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
                     const Tile k = look(t);
                     if (__builtin_expect(k.rare, 0)) special(k, S);
                     first_product((t + 1) % NBUF, next);                       // (behind the last tile: of old rows, for nobody)
-                    if (__builtin_expect(weigh_first(k, S, p), 0)) move_all(k, S, p);
-                    weigh_second(p);
+                    weights(k, S, p);
 #pragma unroll
                     for (int j = 0; j < NX; ++j) { S[j][0] = next[j][0]; S[j][1] = next[j][1]; }
                 }
@@ -509,8 +539,7 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
                     if constexpr (KQ > 1) parts_in(S);
                     const Tile k = look(t);
                     if (__builtin_expect(k.rare, 0)) special(k, S);
-                    if (__builtin_expect(weigh_first(k, S, p), 0)) move_all(k, S, p);
-                    weigh_second(p);
+                    weights(k, S, p);
                     if (MODE != kStats) {
                         pack(p, W);
                         if (MODE == kRows && __builtin_expect(k.rare || k.neg, 0)) signs(k, W);

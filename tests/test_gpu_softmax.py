@@ -173,6 +173,22 @@ def test_rows_of_very_different_norms(dtype, spread):
     within(db, e["db"], tb, "db")
 
 
+@pytest.mark.parametrize("scale", [1.0, 0.0, 1e-20])
+@pytest.mark.parametrize("dtype,size", [("f32", 1e-22), ("f32", 1e-30), ("bf16", 1e-25), ("f16", 1e-3)])
+@pytest.mark.parametrize("nq,dim", [(20, 40), (90, 200)])
+def test_products_below_the_normal_range(nq, dim, dtype, size, scale):
+    """every logit is next to zero: losses are log(nb), and targets and rows behind the last still take their own way"""
+    base, q, targets, w, _ = make(nq, 301, dim, "f32", seed=dim)
+    base, q = (base * size).to(DT[dtype]), (q * size).to(DT[dtype])
+    e = exact(base, q, targets, w, scale)
+    tl, tq, tb = tolerances(base, q, targets, w, scale, e, dtype)
+    loss, (dq, db) = step(base, q, targets, w, scale)
+    assert loss.sub(np.log(301.0)).abs().max() < 1e-5
+    within(loss, e["loss"], tl, "loss")
+    within(dq, e["dq"], tq, "dq")
+    within(db, e["db"], tb, "db")
+
+
 def test_small_losses_keep_their_digits():
     """a query that is answered well: loss = log(1 + what the others weigh), to fp32's digits and not to those of its log sums"""
     dim = 64

@@ -35,7 +35,7 @@ def unpack(codes=P, cs=16, scales=P, mins=0, ss=1, nb=100, dim=32, group=32, ids
 
 @pytest.mark.parametrize("call", [
     lambda: shard(base=0), lambda: shard(q=0), lambda: shard(targets=0), lambda: shard(rest=0), lambda: shard(own=0), lambda: shard(work=0), lambda: shard(dim=0), lambda: shard(dim=1025, bstride=1025, qstride=1025),
-    lambda: shard(bstride=31), lambda: shard(qstride=31), lambda: shard(dtype=3), lambda: shard(dtype=-1), lambda: shard(scale=float("nan")), lambda: shard(scale=float("inf")),
+    lambda: shard(bstride=31), lambda: shard(qstride=31), lambda: shard(dtype=3), lambda: shard(dtype=-1), lambda: shard(scale=float("nan")), lambda: shard(scale=float("inf")), lambda: shard(scale=3e38),
     lambda: shard(base=P + 2), lambda: shard(q=P + 1, dtype=1), lambda: shard(work=P + 128), lambda: shard(bytes_=64), lambda: shard(nb=1 << 31), lambda: shard(nq=1 << 31),
     lambda: shard(id_base=0xffffffff - 50),
     lambda: grad(lse=0), lambda: grad(loss=0), lambda: grad(w=0), lambda: grad(mean=0), lambda: grad(rest=0), lambda: grad(targets=0), lambda: grad(dqs=31), lambda: grad(dbs=31), lambda: grad(db=P + 2),
