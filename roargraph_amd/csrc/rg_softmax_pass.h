@@ -1,6 +1,6 @@
 // rg_softmax_pass.h -- the pass of the softmax operators (rg_softmax.hip): stationary rows x against streamed rows y.
 //
-// A workgroup of four waves owns NX blocks of 16 rows x per wave, held in registers as MFMA operands for the whole pass, and streams rows y
+// A wave owns NX blocks of 16 rows x (or a part of their dimensions), held in registers as MFMA operands for the whole pass; its workgroup streams rows y
 // through LDS, 32 at a time.  Per tile and wave:
 //
 //   S^T[y][x] = Y X^T       v_mfma_f32_16x16x32: A = 16 rows y (ds_read_b128), B = 16 rows x (registers)
