@@ -339,21 +339,24 @@ struct Plan {
     }
 };
 
-// The kernel of a mode.  Few rows x: the pass is bound by reading y, and the thin kernel, which reads fp32 rows and rows of any alignment once
-// and where they lie, beats planes made first (1M x 256 fp32, 8 to 64 queries: 280 - 331 us against 649 us).  It holds a row in a wave's
-// registers: of wide rows the sums no longer fit, and the wide kernel is faster even with planes (fp32 x 768: 994 against 669 us; x 512: 519
-// against 649 us).  16-bit rows it can read where they lie are a draw up to 256 elements, and the wide kernel's beyond (x 512: 238 - 333
-// against 150 - 160 us); their statistics alone are the thin kernel's up to 512 (111 against 121 us; x 1024: 131 against 122 us).
-bool thin_of(int mode, int ks, uint32_t nx, bool direct) {
-    if (mode == kRows || nx > 64) return false;
-    return mode == kStats ? ks <= 16 || !direct : ks <= (direct ? 8 : 16);
+// The kernel of a mode.  Few rows x: the pass is bound by reading y, and the thin kernel, which reads fp32 rows and rows of any alignment where
+// they lie, once for 64 rows x, beats planes made first, read and read again (1.25M x 200 fp32: 64 queries 391 us against 721 us, 128 queries
+// 633 / 818 us, 256 1167 / 1152 us; 16-bit rows that need planes gain more: 830k x 301 bf16, 256 queries 455 / 556 us) -- and of short 16-bit rows
+// that need none it still does up to 128 (2M x 64 bf16 180 / 221 us; x 200, where the wide kernel reads in place what fills its tiles, 247 / 190 us).
+// It holds a row in a wave's registers: of wide rows the sums no longer fit, and the wide kernel is faster even with planes (fp32 x 768, 64
+// queries: 994 against 669 us; x 512 519 / 649 us, with 128 queries 1078 / 838 us; fp16 x 512 in place 238 - 333 / 150 - 160 us).  Statistics alone
+// are the thin kernel's up to 512 elements in place (111 / 121 us; x 1024 131 / 122 us) and at all widths with planes.
+bool thin_of(int dtype, int mode, int ks, uint32_t nx, bool direct) {
+    const bool f32 = dtype == RG_DTYPE_F32;
+    if (mode == kRows || nx > (direct ? (ks <= 2 ? 128 : 64) : f32 ? 128 : 256)) return false;
+    return mode == kStats ? ks <= 16 || !direct : ks <= (direct || (f32 && nx > 64) ? 8 : 16);
 }
 
 // direct: the streamed rows can be read where they lie (16-bit rows of whole 16-byte chunks, 16-byte aligned)
 Plan plan_of(int dtype, int mode, uint32_t dim, uint32_t nx, uint32_t ny, bool direct) {
     Plan p;
     p.ks = steps_of(dim);
-    p.thin = thin_of(mode, p.ks, nx, direct);
+    p.thin = thin_of(dtype, mode, p.ks, nx, direct);
     p.k = kernel_of(dtype, mode, p.thin, p.ks);
     p.planes = !p.thin && !direct;
     p.nx = nx;
@@ -363,13 +366,13 @@ Plan plan_of(int dtype, int mode, uint32_t dim, uint32_t nx, uint32_t ny, bool d
     p.nuse = 0;
     bool any_planes = false;
     for (int m = mode == kRows ? kRows : kStats; m <= (mode == kRows ? kRows : kMean); ++m) {
-        const bool thin = thin_of(m, p.ks, nx, direct);
+        const bool thin = thin_of(dtype, m, p.ks, nx, direct);
         const SoftmaxKernel k = kernel_of(dtype, m, thin, p.ks);
         Use &u = p.use[p.nuse++];
         u.nt = std::max<uint64_t>(1, ((uint64_t)nx + k.xt - 1) / k.xt);
         u.places = 256ull * std::min<uint32_t>(k.wps * 256 / k.threads, 160 * 1024 / k.lds);     // (256 CUs)
         const double ops = 2.0 * (dtype == RG_DTYPE_F32 ? 3 : 1) * (double)(u.nt * k.xt) * (32.0 * p.ks + (m == kStats ? 0.0 : 16.0 * k.ob));     // of a row y
-        u.row_cost = std::max(thin || direct ? (double)dim * elem_bytes(dtype) : 0.0, thin ? 0.0 : ops / kOpsPerByte);
+        u.row_cost = std::max(thin || direct ? (double)dim * elem_bytes(dtype) * (thin ? (double)u.nt : 1.0) : 0.0, thin ? 0.0 : ops / kOpsPerByte);
         any_planes |= !thin && !direct;
     }
     p.slot_cost = 8.0 * opitch_of(dim) * std::max(nx, 1u);

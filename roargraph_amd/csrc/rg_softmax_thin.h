@@ -1,5 +1,5 @@
-// rg_softmax_thin.h -- the pass of the softmax operators for few stationary rows (at most 64): bound by memory, so the streamed rows are
-// read once in the caller's type and layout, through registers (where fp32 rows are split), and every wave holds one block of 16 rows x.
+// rg_softmax_thin.h -- the pass of the softmax operators for few stationary rows: bound by memory, so the streamed rows are
+// read once for 64 of them, in the caller's type and layout, through registers (where fp32 rows are split), and every wave holds one block of 16 rows x.
 // rg_softmax_pass.h has the mathematics, the operand layouts and the LDS swizzle.
 #pragma once
 #include "rg_softmax_pass.h"
@@ -35,9 +35,9 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
     constexpr float kTop = 15.0f, kStart = DT == RG_DTYPE_BF16 ? 0.0f : 7.0f;   // a weight is at most 2^15; the first largest one 2^0 / 2^7
     extern __shared__ char lds[];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = lane & 15, g = lane >> 4;
-    const uint32_t split = xcd_block(blockIdx.x, gridDim.x);
+    const uint32_t ntx = (A.nx + C::XT - 1) / C::XT, b = xcd_block(blockIdx.x, gridDim.x), split = b / ntx;
     const uint32_t ybeg = min(A.ny, split * A.rows_per_split), yend = min(A.ny, ybeg + A.rows_per_split);
-    const uint32_t x0 = wave * 16;
+    const uint32_t x0 = b % ntx * C::XT + wave * 16;
     const bool live = x0 < A.nx;                                // waves behind the last row only help to load
     const uint32_t dim = A.dim;
     const size_t esz = sizeof(T);

@@ -92,7 +92,8 @@ def within(got, want, tol, what):
 SHAPES = [(1, 1, 1), (1, 17, 8), (3, 1000, 24), (64, 1000, 24), (65, 333, 33), (16, 16, 64), (17, 129, 7), (33, 31, 65), (130, 4097, 200), (64, 2048, 208), (40, 700, 209),
           (5, 513, 93), (100, 300, 128), (31, 900, 256), (70, 257, 257), (66, 1025, 384), (129, 515, 512), (20, 260, 513), (9, 400, 768), (19, 130, 1000), (35, 97, 1024),
           (1, 30000, 200), (2000, 40, 96), (300, 20000, 16),
-          (70, 2000, 768), (200, 700, 700), (130, 3000, 1024), (64, 6000, 1000), (65, 500, 515), (90, 600, 385)]
+          (70, 2000, 768), (200, 700, 700), (130, 3000, 1024), (64, 6000, 1000), (65, 500, 515), (90, 600, 385),
+          (100, 3000, 40), (128, 2000, 64), (129, 2000, 64), (128, 900, 201), (256, 1500, 301), (257, 1500, 301), (200, 5000, 7), (110, 40000, 130)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
@@ -328,7 +329,7 @@ def test_targets_beyond_32_bits():
     assert (loss[:3] == np.inf).all() and loss[3] == 0 and torch.equal(loss[4:], softmax.softmax_loss(q.cuda(), base.cuda(), targets.cuda(), scale).cpu()[4:])
 
 
-@pytest.mark.parametrize("dtype,nq,nb,dim", [("f32", 70, 4_300_000, 8), ("bf16", 70, 8_500_000, 5), ("f32", 5, 270_000, 1000)])
+@pytest.mark.parametrize("dtype,nq,nb,dim", [("f32", 70, 4_300_000, 8), ("bf16", 70, 8_500_000, 5), ("f32", 5, 270_000, 1000), ("f32", 300, 4_300_000, 8), ("bf16", 300, 8_500_000, 5)])
 def test_a_base_of_more_than_one_piece(dtype, nq, nb, dim):
     """planes of fp32 and unaligned rows are made a gigabyte at a time; the sums go on from piece to piece"""
     gen = torch.Generator(device="cuda").manual_seed(dim)
