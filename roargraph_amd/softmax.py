@@ -9,17 +9,24 @@ The nq x nb logits are never stored.  Thin host layer over the C ABI (rg_softmax
 the base per rank, like the ground truth.
 """
 import ctypes as C
+import functools
 
 from ._lib import check, lib
 
 STATS, MEAN, GRAD = 0, 1, 2
 
 
+_codes = {}
+
+
 def _dtype_code(t):
-    import torch
-    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}.get(t.dtype)
+    code = _codes.get(t.dtype)
     if code is None:
-        raise TypeError("rows are fp32, fp16 or bf16, got %s" % t.dtype)
+        import torch
+        _codes.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+        code = _codes.get(t.dtype)
+        if code is None:
+            raise TypeError("rows are fp32, fp16 or bf16, got %s" % t.dtype)
     return code
 
 
@@ -42,7 +49,7 @@ def _ptr(t):
 
 def _stream(t):
     import torch
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(t.device.index)     # (current_stream(...).cuda_stream without the objects: 2 us of a call)
 
 
 def _device(t):
@@ -72,6 +79,7 @@ def _targets(targets, n, like):
     return _check_vector(targets, n, torch.int32, like, "targets")
 
 
+@functools.lru_cache(maxsize=1024)
 def workspace(what, nb, nq, dim, dtype_code):
     """rg_softmax_workspace: bytes of scratch of one call"""
     n = C.c_uint64()
@@ -82,7 +90,7 @@ def workspace(what, nb, nq, dim, dtype_code):
 def _scratch(what, nb, nq, dim, like):
     import torch
     n = workspace(what, nb, nq, dim, _dtype_code(like))
-    return torch.empty(max(n, 256), dtype=torch.uint8, device=like.device), n
+    return like.new_empty(max(n, 256), dtype=torch.uint8), n
 
 
 def softmax_shard_dev(base_t, queries_t, targets_t, scale, id_base=0, want_mean=False):
@@ -155,8 +163,8 @@ def _softmax_function():
                 _check_pair(q, b)
                 (nq, dim), nb, code = q.shape, b.shape[0], _dtype_code(b)
                 want_mean = ctx.needs_input_grad[0]
-                loss = torch.empty(nq, dtype=torch.float32, device=b.device)
-                kept = torch.empty((3 + dim if want_mean else 3) * nq, dtype=torch.float32, device=b.device)
+                loss = b.new_empty(nq, dtype=torch.float32)
+                kept = b.new_empty((3 + dim if want_mean else 3) * nq, dtype=torch.float32)
                 work, n = _scratch(MEAN if want_mean else STATS, nb, nq, dim, b)
                 at = kept.data_ptr()
                 check(lib().rg_softmax_shard_dev(b.data_ptr(), nb, _stride(b), q.data_ptr(), nq, _stride(q), dim, code, scale, targets.data_ptr(), 0, at, at + 4 * nq, at + 8 * nq,
@@ -172,8 +180,8 @@ def _softmax_function():
                 q, b = _rows(queries, "queries"), _rows(base, "base")
                 (nq, dim), nb, code = q.shape, b.shape[0], _dtype_code(b)
                 weights = weights.contiguous()
-                dq = torch.empty((nq, dim), dtype=b.dtype, device=b.device) if ctx.needs_input_grad[0] else None
-                db = torch.empty((nb, dim), dtype=b.dtype, device=b.device) if ctx.needs_input_grad[1] else None
+                dq = b.new_empty((nq, dim)) if ctx.needs_input_grad[0] else None
+                db = b.new_empty((nb, dim)) if ctx.needs_input_grad[1] else None
                 work, n = _scratch(GRAD, nb if db is not None else 0, nq, dim, b)
                 at = kept.data_ptr()
                 check(lib().rg_softmax_grad_dev(b.data_ptr(), nb, _stride(b), q.data_ptr(), nq, _stride(q), dim, code, ctx.scale, targets.data_ptr(), 0, at + 8 * nq, loss.data_ptr(),
