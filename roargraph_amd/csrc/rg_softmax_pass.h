@@ -9,7 +9,7 @@
 //                           lie: slot (g, e) of the 32-deep product is row y = 16 (e / 4) + 4 g + e % 4, for both operands
 //
 // so a tile is read from memory once for both products and no weight crosses lanes.  fp32 rows are split into two fp16 halves, each row
-// scaled by its own power of two to [1, 2): x = 2^e (hi + lo), 22 bits; a product is hi hi + hi lo + lo hi (what is left out is 2^-22 of it).
+// scaled by its own power of two to the top of fp16's range: x = 2^e (hi + lo), 22 bits; a product is hi hi + hi lo + lo hi (what is left out is 2^-22 of it).
 // Weights are rounded to the 16-bit type they are multiplied in -- bf16 as such, fp16 with 2^7 .. 2^15 at the top of its range, fp32 rows
 // as two halves again; sums of weights are taken before that rounding, and every accumulation is fp32.
 //

@@ -190,6 +190,22 @@ def test_products_below_the_normal_range(nq, dim, dtype, size, scale):
     within(db, e["db"], tb, "db")
 
 
+@pytest.mark.parametrize("scale", [1.0, 8.0])
+@pytest.mark.parametrize("nq,nb,dim", [(1, 300, 40), (2, 1630, 177), (5, 200, 512), (70, 150, 200)])
+def test_small_elements_of_fp32_rows_keep_their_digits(nq, nb, dim, scale):
+    """elements of five decades in a row: each gradient is compared with the size of its own terms"""
+    base, q, targets, w, _ = make(nq, nb, dim, "f32", seed=nq + dim)
+    g = torch.Generator().manual_seed(dim)
+    shrink = 10.0 ** (-5 * torch.rand(dim, generator=g))
+    base, q = base * shrink, q * shrink
+    e = exact(base, q, targets, w, scale)
+    tl, tq, tb = tolerances(base, q, targets, w, scale, e, "f32")
+    loss, (dq, db) = step(base, q, targets, w, scale)
+    within(loss, e["loss"], tl, "loss")
+    within(dq, e["dq"], tq, "dq")
+    within(db, e["db"], tb, "db")
+
+
 def test_small_losses_keep_their_digits():
     """a query that is answered well: loss = log(1 + what the others weigh), to fp32's digits and not to those of its log sums"""
     dim = 64
