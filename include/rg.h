@@ -315,8 +315,8 @@ rg_status rg_groundtruth(const char *base_fbin, const char *query_fbin, const ch
  *
  * Rows are `dtype` (RG_DTYPE_*; base, queries and their gradients alike), row strides in elements (any stride >= dim, any alignment of
  * the element; 16-bit rows of a multiple of 8 elements, 16-byte aligned, are read in place by every kernel), dim 1 .. 1024, sums in fp32, at
- * most 2^24 - 1 queries a call.  fp32 rows are multiplied as pairs of 16-bit halves: 22 bits of every element down to 2^-28 of the
- * largest of its row.  Targets are global ids (row + id_base);
+ * most 2^24 - 1 queries a call.  fp32 rows are multiplied as pairs of 16-bit halves: 22 bits of every element, or 2^-39 of
+ * the largest of its row.  Targets are global ids (row + id_base);
  * 0xffffffff = the query has no row: loss 0, no gradient, whatever it holds.  A target no shard holds: own = -inf, loss = +inf.
  *
  * Shard form, like rg_gt_shard_dev: a rank holds rows [id_base, id_base + nb).  rg_softmax_shard_dev gives rest and own over the shard

@@ -25,8 +25,9 @@ inline bool known_dtype(int dtype) { return dtype == RG_DTYPE_F32 || dtype == RG
 inline uint32_t elem_bytes(int dtype) { return dtype == RG_DTYPE_F32 ? 4 : 2; }
 
 // ---- fp32 rows as two fp16 halves, scaled by a power of two of their own
-// exponent e of a row: 2^-e brings its largest value to [2^14, 2^15), the top of fp16's range, so that elements down to 2^-28 of it keep their
-// 22 bits (brought to [1, 2), the second halves of elements below 2^-3 of it were subnormal: 2 queries on 1630 x 177, a gradient off by 3e-5).
+// exponent e of a row: 2^-e brings its largest value to [2^14, 2^15), the top of fp16's range, so that elements down to 2^-17 of it keep their
+// 22 bits and none is off by more than 2^-39 of it (brought to [1, 2), the second halves of elements below 2^-3 of it were subnormal, off by 2^-25
+// of it: two queries on 1630 x 177, elements of a gradient by 3e-5 of themselves).
 // Rows below 2^-112 are brought as far as 2^126 does.
 __device__ __forceinline__ int row_exponent(float top) {
     const uint32_t u = __float_as_uint(top) >> 23;

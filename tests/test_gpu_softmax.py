@@ -193,13 +193,17 @@ def test_products_below_the_normal_range(nq, dim, dtype, size, scale):
 @pytest.mark.parametrize("scale", [1.0, 8.0])
 @pytest.mark.parametrize("nq,nb,dim", [(1, 300, 40), (2, 1630, 177), (5, 200, 512), (70, 150, 200)])
 def test_small_elements_of_fp32_rows_keep_their_digits(nq, nb, dim, scale):
-    """elements of five decades in a row: each gradient is compared with the size of its own terms"""
+    """Elements of five decades in a row: each gradient is compared with the size of its own terms.  An element x of a row whose largest is t is
+    brought to x 2^-e with t 2^-e >= 2^14 and held as two fp16 halves: the second is rounded to 2^-11 of itself, 2^-22 |x|, or, where it is
+    subnormal, to half of fp16's smallest step, 2^-25 2^e <= 2^-39 t."""
     base, q, targets, w, _ = make(nq, nb, dim, "f32", seed=nq + dim)
     g = torch.Generator().manual_seed(dim)
     shrink = 10.0 ** (-5 * torch.rand(dim, generator=g))
     base, q = base * shrink, q * shrink
     e = exact(base, q, targets, w, scale)
     tl, tq, tb = tolerances(base, q, targets, w, scale, e, "f32")
+    tq = tq + scale * e["g"].abs() @ base.double().abs().amax(1, keepdim=True) * 2.0 ** -39
+    tb = tb + scale * e["g"].abs().T @ q.double().abs().amax(1, keepdim=True) * 2.0 ** -39
     loss, (dq, db) = step(base, q, targets, w, scale)
     within(loss, e["loss"], tl, "loss")
     within(dq, e["dq"], tq, "dq")
