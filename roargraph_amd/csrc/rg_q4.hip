@@ -87,6 +87,7 @@ __global__ void __launch_bounds__(256) rg_q4_pack_kernel(const void *rows, uint3
             for (int i = 0; i < 8; ++i) {
                 const double r = fma(-(double)c[i], (double)s, (double)v[i] - (double)m), half = 0.5 * (double)s;
                 const bool odd = ((int)c[i] & 1) != 0;
+                if (s == 0.0f) continue;             // (one level)
                 if (r > half || (r == half && odd)) c[i] += 1.0f;
                 else if (r < -half || (r == -half && odd)) c[i] -= 1.0f;
             }

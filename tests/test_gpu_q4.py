@@ -182,6 +182,19 @@ def test_empty_and_refused():
             bad()
 
 
+@pytest.mark.parametrize("mins", [False, True])
+def test_a_scale_of_zero_has_one_level(mins):
+    """groups whose values are all alike, beside values between two levels: codes of the first level, whatever the neighbours"""
+    x = torch.zeros(40, 65)
+    x[:, :32] = torch.tensor([0.0, 15.0, 0.5, 1.5, 2.5, 3.5, 7.0, 4.0] * 4)      # (with minima: a scale of 1)
+    x[:, 32:64] = torch.linspace(0.1, 3.0, 40)[:, None]
+    x[:, 64] = torch.linspace(-1.0, 1.0, 40) + 1e-5
+    for rows in (x, x * 1e-9):
+        codes, scales, low, values = plain_pack(rows, 32, mins)
+        p = q4.q4_pack(rows.cuda(), group=32, mins=mins)
+        assert (nibbles(p.codes, 65)[:, :65] == codes).all() and (p.scales.cpu().numpy() == scales).all() and (q4.q4_unpack(p).cpu().numpy() == values).all()
+
+
 def test_rows_that_overlap_are_refused():
     """(an expanded matrix has no row stride: reading it as rows would leave the tensor)"""
     p = q4.q4_pack(torch.randn(100, 24, device="cuda"), mins=True)
