@@ -547,9 +547,11 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
                     part_out(S);
                     __syncthreads();
                 }
-                const Tile k = look(t);
+                Tile k;
+                if (TWICE) k = look(t);              // (all waves: they turn together)
                 if (live) {
                     if constexpr (KQ > 1) parts_in(S);
+                    if (!TWICE) k = look(t);
                     if (__builtin_expect(k.rare, 0)) special(k, S);
                     weights(k, S, p);
                     if (MODE != kStats) {
@@ -566,8 +568,10 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
                         second_product(t % NBUF, W);
                     }
                 }
-                again = TWICE && !again && k.twice;
-                if (again) continue;
+                if constexpr (TWICE) {
+                    again = !again && k.twice;
+                    if (again) continue;
+                }
                 if (NBUF == 1 && t + 1 < ntiles) {
                     __syncthreads();
                     load(t + 1);
