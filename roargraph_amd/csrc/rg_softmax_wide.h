@@ -66,7 +66,6 @@ __device__ __forceinline__ void load_lds16(const void *base, uint32_t off, uint3
 template <int DT, int KS, int MODE>
 __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, MODE>::WPS)) rg_softmax_wide_kernel(PassArgs A) {
     typedef WideCfg<DT, KS, MODE> C;
-    typedef typename Elem<DT>::T T;
     typedef typename Frag<DT>::V V;
     constexpr int NP = C::NP, NX = C::NX, KQ = C::KQ, KW = C::KW, OW = C::OW, PITCH = C::PITCH, NBUF = C::NBUF;
     constexpr bool F32 = C::F32, INFO = C::INFO;
