@@ -2,8 +2,8 @@
 //
 // With z_ij = scale <q_i, b_j> (kept in units of log 2: z2 = z log2 e, so that every exponential is one v_exp_f32):
 //
-//   statistics + mean   for each query i one pass over the rows j != target with a running reference M, sum l and sum O:
-//                         P = 2^(z2 - M),  l += P,  O += P b_j          rest = ln 2 (M + log2 l),  mean = O / l
+//   statistics + mean   for each query i one pass over the rows j != target with a running reference M, sums l, R and sum O:
+//                         P = 2^(z2 - M),  l += P,  W = P in the rows' type,  R += W,  O += W b_j      rest = ln 2 (M + log2 l),  mean = O / R
 //                       the target's own logit is set aside, so that loss = log(1 + e^(rest - own)) keeps its digits where it is small
 //   gradient of rows    for each row j one pass over the queries i -- the same pass with the roles exchanged:
 //                         G = w_i 2^(z2 - lse2_i) = +-2^(z2 + bias_i),   bias_i = log2|w_i| - lse2_i
@@ -58,16 +58,22 @@ __global__ void __launch_bounds__(256) rg_softmax_join_kernel(const float4 *ml, 
     M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     Mo = fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
     const bool none = M == kNothing;       // no other row than the target
-    float l = 0.0f;
+    float l = 0.0f, div = 0.0f;            // sum of the weights; what the mean is divided by (the weights as they were multiplied)
     for (uint32_t s = tid; s < nslots; s += 256) {
         const float4 v = ml[(size_t)s * nq + i];
-        l += v.y * exp2f(v.x - M);
+        const float f = exp2f(v.x - M);
+        l += v.y * f;
+        div += v.w * f;
     }
-    for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
+    for (int d = 1; d < 64; d <<= 1) {
+        l += __shfl_xor(l, d);
+        div += __shfl_xor(div, d);
+    }
     __syncthreads();
-    if (lane == 0) red[wave] = l;
+    if (lane == 0) { red[wave] = l; red[4 + wave] = div; }
     __syncthreads();
     l = red[0] + red[1] + red[2] + red[3];
+    div = red[4] + red[5] + red[6] + red[7];
     if (tid == 0 && blockIdx.y == 0) {
         const uint32_t t = targets[i];
         const bool here = target_here(t, id_base, nb);
@@ -81,7 +87,7 @@ __global__ void __launch_bounds__(256) rg_softmax_join_kernel(const float4 *ml, 
         if (loss) loss[i] = v;
     }
     if (mean) {
-        const float f = none ? 0.0f : exp2f(Mo - M) / l;
+        const float f = none ? 0.0f : exp2f(Mo - M) / div;
         const bool many = nslots >= kJoinSlots;
         const uint32_t width = many ? kJoinDims : 256, group = tid / 16;
         for (uint32_t k0 = blockIdx.y * width; k0 < dim; k0 += gridDim.y * width) {

@@ -11,7 +11,9 @@
 // so a tile is read from memory once for both products and no weight crosses lanes.  fp32 rows are split into two fp16 halves, each row
 // scaled by its own power of two to the top of fp16's range: x = 2^e (hi + lo), 22 bits; a product is hi hi + hi lo + lo hi (what is left out is 2^-22 of it).
 // Weights are rounded to the 16-bit type they are multiplied in -- bf16 as such, fp16 with 2^7 .. 2^15 at the top of its range, fp32 rows
-// as two halves again; sums of weights are taken before that rounding, and every accumulation is fp32.
+// as two halves again; sums of weights are taken before that rounding, and every accumulation is fp32.  What O is divided by is the sum of the
+// weights as they were multiplied: divided by the others' sum, the mean is off by up to half a step of itself, which shows where a query's
+// gradient is the small difference of mean and target (bf16, rows 0.1 beside the target: 0.012 of the gradient's norm, now 0.0017).
 //
 // M is a reference, not the running maximum: it moves only when a weight would pass 2^15 (a branch no wave takes on most tiles), so sums
 // are rescaled a few times per pass instead of once per tile.
@@ -38,7 +40,7 @@ struct PassArgs {
     uint32_t nsplit, rows_per_split;   // of y
     uint32_t opitch;                   // floats of a row of o
     uint32_t resume;                   // the slots hold what earlier pieces of y left
-    float4 *ml;                        // [slot][nx] reference and sum of the weights, reference of O, -- (kMean, kStats; kRows in pieces: the third)
+    float4 *ml;                        // [slot][nx] reference and sum of the weights, reference of O, what O is divided by under the first (kMean, kStats; kRows in pieces: the third)
     float *o;                          // [slot][nx][opitch] (kMean, kRows in pieces)
     const uint32_t *targets;           // kStats, kMean: per x (global ids)
     uint32_t id_base;
@@ -233,9 +235,29 @@ __device__ __forceinline__ float load_stationary(const PassArgs &A, uint32_t x, 
     }
 }
 
+// the sum of a lane's weights as they are multiplied (16-bit subnormals count)
+__device__ __forceinline__ float sum_of(half8 w) {
+    typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+    const half2 one{(_Float16)1.0f, (_Float16)1.0f};
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_fdot2(half2{w[2 * e], w[2 * e + 1]}, one, s, false);
+    return s;
+}
+__device__ __forceinline__ float sum_of(bf8 w) {
+    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+    const bf2 one{(__bf16)1.0f, (__bf16)1.0f};
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_fdot2_f32_bf16(bf2{w[2 * e], w[2 * e + 1]}, one, s, false);
+    return s;
+}
+// kMean, 16-bit rows: such a sum is kept beside l (fp32 rows' weights are 22 bits of themselves, and l serves)
+constexpr bool softmax_sums_rounded(int dt, int mode) { return mode == kMean && dt != RG_DTYPE_F32; }
+
 // what an earlier piece left in a wave's slot
-template <int MODE, int OB, int NX, int NO>
-__device__ __forceinline__ void take_up(const PassArgs &A, uint32_t x0, uint32_t n, uint32_t g, uint32_t kq, uint32_t split, float (&M)[NX], float (&Ml)[NX], float (&l)[NX], f32x4 (&O)[NO][NX]) {
+template <int DT, int MODE, int OB, int NX, int NO>
+__device__ __forceinline__ void take_up(const PassArgs &A, uint32_t x0, uint32_t n, uint32_t g, uint32_t kq, uint32_t split, float (&M)[NX], float (&Ml)[NX], float (&l)[NX], float (&R)[NX], f32x4 (&O)[NO][NX]) {
 #pragma unroll
     for (int j = 0; j < NX; ++j) {
         const uint32_t x = x0 + j * 16 + n;
@@ -245,6 +267,7 @@ __device__ __forceinline__ void take_up(const PassArgs &A, uint32_t x0, uint32_t
         Ml[j] = v.x;
         M[j] = v.z;
         l[j] = g == 0 ? v.y : 0.0f;                  // (finish adds the four up)
+        if (softmax_sums_rounded(DT, MODE)) R[j] = g == 0 ? v.w : 0.0f;
         if constexpr (MODE != kStats)
 #pragma unroll
             for (int ob = 0; ob < OB; ++ob) {
@@ -257,7 +280,7 @@ __device__ __forceinline__ void take_up(const PassArgs &A, uint32_t x0, uint32_t
 // what a wave (with part kq of the output blocks) leaves behind: references and sums, and the sums of rows (partial results, or the gradient itself)
 template <int DT, int MODE, int OB, int NX, int NO>
 __device__ __forceinline__ void finish(const PassArgs &A, uint32_t x0, uint32_t n, uint32_t g, uint32_t kq, uint32_t split, const float (&M)[NX], const float (&Ml)[NX], const float (&l)[NX],
-                                       const f32x4 (&O)[NO][NX]) {
+                                       const float (&R)[NX], const f32x4 (&O)[NO][NX]) {
     typedef typename Elem<DT>::T T;
 #pragma unroll
     for (int j = 0; j < NX; ++j) {
@@ -265,10 +288,16 @@ __device__ __forceinline__ void finish(const PassArgs &A, uint32_t x0, uint32_t 
         float s = l[j];
         s += __shfl_xor(s, 16);
         s += __shfl_xor(s, 32);
+        float r = s;
+        if (softmax_sums_rounded(DT, MODE)) {
+            r = R[j];
+            r += __shfl_xor(r, 16);
+            r += __shfl_xor(r, 32);
+        }
         if (x >= A.nx) continue;
         const size_t at = (size_t)split * A.nx + x;
         const bool direct = MODE == kRows && A.nsplit == 1;
-        if (!direct && g == 0 && kq == 0) A.ml[at] = make_float4(Ml[j], s, M[j], 0.0f);
+        if (!direct && g == 0 && kq == 0) A.ml[at] = make_float4(Ml[j], s, M[j], r);
         if constexpr (MODE != kStats) {
             const float f = direct ? exp2_hw(0.5f * M[j]) : 1.0f;      // 2^M in two steps: it may lie below the normal range
 #pragma unroll

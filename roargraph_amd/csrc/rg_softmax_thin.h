@@ -59,17 +59,18 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
     f32x4 O[MODE == kStats ? 1 : OB][NX];
     // M: reference of the weights of O; with fp32 rows those carry the rows' scales, so that the sum l has a reference Ml of its own
     constexpr bool TWO = F32 && MODE == kMean;
-    float M[NX], l[NX], Ml[NX];
+    constexpr bool SUM = softmax_sums_rounded(DT, MODE);
+    float M[NX], l[NX], Ml[NX], R[NX];
 #pragma unroll
     for (int j = 0; j < NX; ++j) {
         M[j] = Ml[j] = kNothing;
-        l[j] = 0.0f;
+        l[j] = R[j] = 0.0f;
         if (MODE != kStats)
 #pragma unroll
             for (int ob = 0; ob < OB; ++ob) O[ob][j] = f32x4{0, 0, 0, 0};
     }
 
-    if (A.resume) take_up<MODE, OB, NX>(A, x0, n, g, 0, split, M, Ml, l, O);
+    if (A.resume) take_up<DT, MODE, OB, NX>(A, x0, n, g, 0, split, M, Ml, l, R, O);
 
     // streaming: LPR lanes per row, rows lr, lr + ROWS, .. per thread
     const uint32_t lr = tid / C::LPR, lc = tid % C::LPR;
@@ -126,6 +127,9 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
         }
     };
 
+    // Where registers are few, a lane's LDS addresses are made of one, by its bits 5 - 7, for every read, not kept over the tiles (mean of 20 fp16
+    // queries on 500k x 509 304 us, so 236 us; statistics, which have registers to spare, 177 us, so 181 us).
+    constexpr bool MADE = KS > 12 && MODE == kMean;
     auto compute = [&](uint32_t t, uint32_t y0) {
         const char *tile = lds + t * C::BUF;
         const float *yv = reinterpret_cast<const float *>(lds + C::NBUF * C::TURN * C::BUF) + t * C::TY * 2;
@@ -137,6 +141,8 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
         {
             const uint32_t sw = swizzle(n);                     // (row + 16: the same swizzle)
             const char *row = tile + n * PITCH;
+            uint32_t first = t * C::BUF + n * PITCH + ((g ^ sw) << 4);
+            if (MADE) asm("" : "+v"(first));
             constexpr int PART = KS / softmax_parts(DT, KS);
             f32x4 sum[2][NX];
 #pragma unroll
@@ -151,7 +157,7 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
                         }
                 }
                 const uint32_t c = 4 * ks + g;
-                const char *at = row + (c & ~15u) * 16 + (((c & 15) ^ sw) << 4);
+                const char *at = MADE ? lds + (first ^ (uint32_t)(ks % 4 << 6)) + ks / 4 * 256 : row + (c & ~15u) * 16 + (((c & 15) ^ sw) << 4);
                 V a[2][NP];
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -257,6 +263,7 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
             }
             if (weigh(TWO, M[j], old, p)) {
                 if (!TWO) l[j] *= old;
+                if (SUM) R[j] *= old;
                 if (MODE != kStats)
 #pragma unroll
                     for (int ob = 0; ob < OB; ++ob) O[ob][j] *= old;
@@ -275,6 +282,7 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
                             if (F32) wl[4 * h + i] = (_Float16)(p[h][i] - (float)w[4 * h + i]);
                         }
                     }
+                if constexpr (SUM) R[j] += sum_of(w);
                 S[0][j] = __builtin_bit_cast(f32x4, w);
                 if (F32) S[1][j] = __builtin_bit_cast(f32x4, wl);
             }
@@ -284,10 +292,12 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
             typedef __attribute__((address_space(3))) s16x4 *tr_ptr;
             const uint32_t r = 4 * g + (n >> 2), sw = swizzle(r);     // (row + 16: the same swizzle)
             const char *row = tile + r * PITCH + (n & 1) * 8;
+            uint32_t second = t * C::BUF + r * PITCH + (((n >> 1 & 1) ^ sw) << 4) + (n & 1) * 8;
+            if (MADE) asm("" : "+v"(second));
 #pragma unroll
             for (int ob = 0; ob < OB; ++ob) {
                 const uint32_t c = 2 * ob + ((n >> 1) & 1);
-                const char *at = row + (c & ~15u) * 16 + (((c & 15) ^ sw) << 4);
+                const char *at = MADE ? lds + (second ^ (uint32_t)(ob % 8 << 5)) + ob / 8 * 256 : row + (c & ~15u) * 16 + (((c & 15) ^ sw) << 4);
                 V a[NP];
 #pragma unroll
                 for (int p = 0; p < NP; ++p) {
@@ -337,7 +347,7 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
         }
     }
 
-    finish<DT, MODE, OB, NX>(A, x0, n, g, 0, split, M, TWO ? Ml : M, l, O);
+    finish<DT, MODE, OB, NX>(A, x0, n, g, 0, split, M, TWO ? Ml : M, l, R, O);
 }
 
 }  // namespace rg

@@ -150,19 +150,20 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);             // the compiler's own loads (vmcnt(0)): none of its waits is left for the loop
     f32x4 O[MODE == kStats ? 1 : OW][NX];
-    float M[NX], l[NX], Ml[NX];
+    constexpr bool SUM = softmax_sums_rounded(DT, MODE);
+    float M[NX], l[NX], Ml[NX], R[NX];
 #pragma unroll
     for (int j = 0; j < NX; ++j) {
         M[j] = NOREF ? -60.0f : kNothing;
         Ml[j] = kNothing;
-        l[j] = 0.0f;
+        l[j] = R[j] = 0.0f;
         if (MODE != kStats)
 #pragma unroll
             for (int ob = 0; ob < OW; ++ob) O[ob][j] = f32x4{0, 0, 0, 0};
     }
 
     if (MODE != kRows && A.resume) {
-        take_up<MODE, OW, NX>(A, x0, n, g, kq, split, M, Ml, l, O);
+        take_up<DT, MODE, OW, NX>(A, x0, n, g, kq, split, M, Ml, l, R, O);
         __builtin_amdgcn_s_waitcnt(0x0f70);         // (as above)
     }
 
@@ -176,23 +177,28 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
         return a;
     };
     // what a lane reads of a tile: chunks 4 ks + g of row n, and dims 4 (n % 4) of each block of rows 4 g + n / 4 (they repeat every 256 bytes)
-    uint32_t first_at[4], second_at[8];
+    // -- where registers are few, all of them are made of the first, by its bits 5 - 7, for every read (a wave's part of a row starts with 256 bytes there):
+    // mean of 2048 bf16 queries on 400k x 256 923 us, so 743 us; 2000 fp16 on 30k x 1024 492 us, so 414 us; but 4096 bf16 on 250k x 512, which fit, 1.74 ms, so 1.78
+    constexpr bool MADE = softmax_sums_rounded(DT, MODE) && (KS == 8 || KS == 32);
+    static_assert(!MADE || KQ == 1 || (KW % 4 == 0 && OW % 8 == 0), "parts start with 256 bytes");
+    uint32_t first_at[MADE ? 1 : 4], second_at[MADE ? 1 : 8];
     auto chunk_at = [&](uint32_t row, uint32_t c) { return ring + row * PITCH + (c >> 4 << 8) + (((c & 15) ^ swizzle(row)) << 4); };
 #pragma unroll
-    for (int i = 0; i < 4; ++i) first_at[i] = chunk_at(n, 4 * (kq * KW + i) + g);
+    for (int i = 0; i < (MADE ? 1 : 4); ++i) first_at[i] = chunk_at(n, 4 * (kq * KW + i) + g);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) second_at[i] = chunk_at(4 * g + (n >> 2), 2 * (kq * OW + i) + (n >> 1 & 1)) + (n & 1) * 8;
+    for (int i = 0; i < (MADE ? 1 : 8); ++i) second_at[i] = chunk_at(4 * g + (n >> 2), 2 * (kq * OW + i) + (n >> 1 & 1)) + (n & 1) * 8;
     auto first_product = [&](uint32_t buf, f32x4 (&S)[NX][2]) {
         constexpr int AHEAD = 1;
-        uint32_t at[4];
+        uint32_t at[MADE ? 1 : 4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) at[i] = lds_at(first_at[i] + buf * C::BUF);
+        for (int i = 0; i < (MADE ? 1 : 4); ++i) at[i] = lds_at(first_at[i] + buf * C::BUF);
         V a[AHEAD + 1][2][NP];
         auto read = [&](int ks) {
+            const uint32_t from = MADE ? lds_at(at[0] ^ (uint32_t)(ks % 4 << 6)) : at[MADE ? 0 : ks % 4];
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int p = 0; p < NP; ++p) a[ks % (AHEAD + 1)][h][p] = *(LdsV *)(at[ks % 4] + (uint32_t)(ks / 4 * 256 + h * 16 * PITCH + p * C::PLANE));
+                for (int p = 0; p < NP; ++p) a[ks % (AHEAD + 1)][h][p] = *(LdsV *)(from + (uint32_t)(ks / 4 * 256 + h * 16 * PITCH + p * C::PLANE));
         };
 #pragma unroll
         for (int j = 0; j < NX; ++j) S[j][0] = S[j][1] = f32x4{0, 0, 0, 0};
@@ -258,15 +264,16 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
         if constexpr (MODE != kStats) {
             typedef __attribute__((address_space(3))) s16x4 *tr_ptr;
             constexpr int AHEAD = 2;
-            uint32_t at[8];
+            uint32_t at[MADE ? 1 : 8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) at[i] = lds_at(second_at[i] + buf * C::BUF);
+            for (int i = 0; i < (MADE ? 1 : 8); ++i) at[i] = lds_at(second_at[i] + buf * C::BUF);
             s16x4 a[AHEAD + 1][NP][2];
             auto read = [&](int ob) {
+                const uint32_t from = MADE ? lds_at(at[0] ^ (uint32_t)(ob % 8 << 5)) : at[MADE ? 0 : ob % 8];
 #pragma unroll
                 for (int p = 0; p < NP; ++p)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) a[ob % (AHEAD + 1)][p][h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(at[ob % 8] + (uint32_t)(ob / 8 * 256 + p * C::PLANE + h * 16 * PITCH)));
+                    for (int h = 0; h < 2; ++h) a[ob % (AHEAD + 1)][p][h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(from + (uint32_t)(ob / 8 * 256 + p * C::PLANE + h * 16 * PITCH)));
             };
 #pragma unroll
             for (int ob = 0; ob < AHEAD && ob < OW; ++ob) read(ob);
@@ -493,6 +500,9 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
             if constexpr (TWO) relocate(k, S, false, Ml, pl, scale_l);
             relocate(k, S, BIAS, M, p, [&](const float (&old)[NX]) {
                 if (!TWO) scale_l(old);
+                if (SUM)
+#pragma unroll
+                    for (int j = 0; j < NX; ++j) R[j] *= old[j];
                 if (MODE != kStats)
 #pragma unroll
                     for (int j = 0; j < NX; ++j)
@@ -563,6 +573,9 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
 #pragma unroll
                                         for (int i = 0; i < 4; ++i) p[j][h][i] -= (float)(__bf16)p[j][h][i];
                         pack(p, W);
+                        if constexpr (SUM)
+#pragma unroll
+                            for (int j = 0; j < NX; ++j) R[j] += sum_of(W[j][0]);
                         if (MODE == kRows && __builtin_expect(k.rare || k.neg, 0)) signs(k, W);
                         second_product(t % NBUF, W);
                     }
@@ -579,7 +592,7 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
             }
         }
     }
-    finish<DT, MODE, OW, NX>(A, x0, n, g, kq, split, M, TWO ? Ml : M, l, O);
+    finish<DT, MODE, OW, NX>(A, x0, n, g, kq, split, M, TWO ? Ml : M, l, R, O);
 }
 
 }  // namespace rg

@@ -1,0 +1,57 @@
+"""-m gpu: softmax cross entropy over a base where its digits cancel, and where values are not finite (rg_softmax_*), against the definition in 64 bits.
+
+The formats' roundings are those of test_gpu_softmax: half a step of bf16 is 2^-8 of a value, of fp16 2^-11, of fp32 2^-24 (U)."""
+import numpy as np
+import pytest
+import torch
+
+from roargraph_amd import softmax
+from test_gpu_softmax import DT, U, exact, make, step, tolerances, within
+
+pytestmark = pytest.mark.gpu
+
+HALF = {"f32": U, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+
+
+def rounded(x, dtype):
+    return x.to(DT[dtype]).double()
+
+
+# ---- digits of the gradients
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("nq,nb,dim", [(3, 20000, 200), (20, 20000, 64), (300, 20000, 200), (40, 6000, 1024), (150, 9000, 93)])
+@pytest.mark.parametrize("dist", [0.1, 0.03])
+def test_a_hard_negative_next_to_the_target(nq, nb, dim, dist, dtype):
+    """A query is answered by rows that lie `dist` beside its target t: dq = w scale (part mean - miss b_t) is small beside mean and b_t.  What a rounding
+    of the weights may do to it: with W_j = P_j (1 + d_j), |d_j| <= h, and the mean taken over the W,
+      mean' - mean = sum p_j d_j (b_j - mean) / (1 + sum p_j d_j),  at most h / (1 - h) sum p_j |b_j - mean|
+    -- small where the rows that have it all are alike, whatever their weights are rounded to.  (Divided by the sum of the P, the mean is off by up to h of itself.)"""
+    g = torch.Generator().manual_seed(nq + dim)
+    base = torch.randn(nb, dim, generator=g)
+    base /= base.norm(dim=1, keepdim=True)
+    at = torch.randperm(nb // 10, generator=g)[:nq] * 10
+    t = at + 9
+    off = torch.randn(nq, dim, generator=g)
+    n = base[t] + dist * off / off.norm(dim=1, keepdim=True)
+    for k in range(8):                                             # (eight of them, a little shorter each: their weights are no powers of two)
+        base[at + k] = n * (1 - 0.013 * k)
+    q = n + 0.3 * torch.randn(nq, dim, generator=g) / dim ** 0.5
+    base, q, w, scale, targets = base.to(DT[dtype]), q.to(DT[dtype]), torch.ones(nq), 16.0, t.int()
+    e = exact(base, q, targets, w, scale)
+    got = step(base, q, targets, w, scale, grads="q")[1][0].double().cpu()
+    b, half = base.double(), HALF[dtype]
+    z = e["z"].clone()
+    z[torch.arange(nq), t] = -np.inf
+    p = torch.exp(z - e["rest"][:, None])
+    mean = p @ b
+    spread = (p * torch.cdist(mean, b)).sum(1)
+    size = (p * b.norm(dim=1)[None]).sum(1)
+    miss, bt = -torch.expm1(-e["loss"]), b[t].norm(dim=1)
+    dz = float(b.norm(dim=1).max() * q.double().norm(dim=1).max()) * scale * (dim + 8) * U
+    # the weights' rounding and the logits'; sums of 32 products each in fp32, in tiles and slots; part and miss are made apart, of rest, lse and loss
+    delta = scale * miss * ((half / (1 - half) + 2 * dz) * spread + (nb / 32 + 256 + 64) * U * size + 2 * dz * (mean - b[t]).norm(dim=1)
+                            + (2 * (e["rest"].abs() + e["lse"].abs()) + 16) * U * bt)
+    last = (rounded(e["dq"], dtype) - e["dq"]).norm(dim=1)
+    worst = ((got - e["dq"]).norm(dim=1) / (last + 2 * delta)).max().item()        # (rounded from delta beside: |got - x| <= |round(x) - x| + 2 delta)
+    assert worst <= 1.0, worst
