@@ -71,7 +71,8 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
     constexpr bool F32 = C::F32, INFO = C::INFO;
     constexpr bool TWO = F32 && MODE == kMean;      // weights of O carry the rows' scales: the sum l has a reference of its own
     constexpr bool BIAS = TWO || MODE == kRows;
-    // (weights of kRows are at most |w| and bf16 has the range of fp32: a constant serves, which keeps small ones normal)
+    // (weights of kRows are at most |w| and bf16 has the range of fp32: a constant serves.  2^-16 keeps weights down to 2^-142 normal, and sums of weight times
+    // query up to 2^111 finite; with 2^-60 those from 2^67 on were infinite.)
     constexpr bool NOREF = DT == RG_DTYPE_BF16 && MODE == kRows;
     constexpr float kTop = 15.0f, kStart = DT == RG_DTYPE_BF16 ? 0.0f : 7.0f;
     extern __shared__ char lds[];
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__((WideCfg<DT, KS, MODE>::NT), (WideCfg<DT, KS, 
     float M[NX], l[NX], Ml[NX], R[NX];
 #pragma unroll
     for (int j = 0; j < NX; ++j) {
-        M[j] = NOREF ? -60.0f : kNothing;
+        M[j] = NOREF ? -16.0f : kNothing;
         Ml[j] = kNothing;
         l[j] = R[j] = 0.0f;
         if (MODE != kStats)

@@ -55,3 +55,18 @@ def test_a_hard_negative_next_to_the_target(nq, nb, dim, dist, dtype):
     last = (rounded(e["dq"], dtype) - e["dq"]).norm(dim=1)
     worst = ((got - e["dq"]).norm(dim=1) / (last + 2 * delta)).max().item()        # (rounded from delta beside: |got - x| <= |round(x) - x| + 2 delta)
     assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("nq,nb,dim", [(33, 300, 40), (200, 500, 200), (20, 90, 520)])
+@pytest.mark.parametrize("size", [1e24, 1e-24, 1e28])
+def test_rows_and_queries_of_opposite_sizes(nq, nb, dim, size, dtype):
+    """logits of ordinary size made of large queries and small rows, or the other way round: both gradients are far from 1"""
+    base, q, targets, w, scale = make(nq, nb, dim, "f32", seed=dim)
+    base, q = (base / size).to(DT[dtype]), (q * size).to(DT[dtype])
+    e = exact(base, q, targets, w, scale)
+    tl, tq, tb = tolerances(base, q, targets, w, scale, e, dtype)
+    loss, (dq, db) = step(base, q, targets, w, scale)
+    within(loss, e["loss"], tl, "loss")
+    within(dq, e["dq"], tq, "dq")
+    within(db, e["db"], tb, "db")
