@@ -57,7 +57,6 @@ __global__ void __launch_bounds__(256) rg_softmax_join_kernel(const float4 *ml, 
     __syncthreads();
     M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     Mo = fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
-    const bool none = M == kNothing;       // no other row than the target
     float l = 0.0f, div = 0.0f;            // sum of the weights; what the mean is divided by (the weights as they were multiplied)
     for (uint32_t s = tid; s < nslots; s += 256) {
         const float4 v = ml[(size_t)s * nq + i];
@@ -74,13 +73,14 @@ __global__ void __launch_bounds__(256) rg_softmax_join_kernel(const float4 *ml, 
     __syncthreads();
     l = red[0] + red[1] + red[2] + red[3];
     div = red[4] + red[5] + red[6] + red[7];
+    const bool none = M == kNothing && l == 0.0f;       // no other row than the target (where all logits are NaN the reference has not moved either, but l is NaN)
     if (tid == 0 && blockIdx.y == 0) {
         const uint32_t t = targets[i];
         const bool here = target_here(t, id_base, nb);
         // (in 64 bits: the instruction behind log2f rounds down, which a small loss shows)
         const double r2 = none ? -INFINITY : (double)M + log2((double)l), z2 = here ? own2[i] : -INFINITY;
         const float r = (float)(r2 * kLn2), z = (float)(z2 * kLn2);
-        const float v = here ? softplus((float)((r2 - z2) * kLn2)) : t == kNoTarget ? 0.0f : INFINITY;
+        const float v = t == kNoTarget ? 0.0f : here ? softplus((float)((r2 - z2) * kLn2)) : r != r ? r : INFINITY;
         rest[i] = r;
         own[i] = z;
         if (lse) lse[i] = here ? z + v : r;
@@ -127,13 +127,14 @@ __global__ void __launch_bounds__(256) rg_softmax_merge_kernel(const float *rest
     float m = -INFINITY, own = -INFINITY;
     for (uint32_t s = 0; s < nlists; ++s) {
         m = fmaxf(m, rest_in[(size_t)s * nq + i]);
-        own = fmaxf(own, own_in[(size_t)s * nq + i]);
+        const float z = own_in[(size_t)s * nq + i];
+        own = z != z || z > own ? z : own;             // (once NaN, it stays)
     }
     float l = 0.0f;
     const float ref = m == -INFINITY ? 0.0f : m;
-    for (uint32_t s = 0; s < nlists; ++s) l += expf(rest_in[(size_t)s * nq + i] - ref);
-    const float r = m == -INFINITY ? -INFINITY : m + logf(l);
-    const float v = targets[i] == kNoTarget ? 0.0f : own == -INFINITY ? INFINITY : softplus(r - own);
+    for (uint32_t s = 0; s < nlists; ++s) l += expf(rest_in[(size_t)s * nq + i] - ref);       // (NaN where a shard's rest is)
+    const float r = l == 0.0f ? -INFINITY : ref + logf(l);
+    const float v = targets[i] == kNoTarget ? 0.0f : r != r ? r : own == -INFINITY ? INFINITY : softplus(r - own);
     lse[i] = targets[i] == kNoTarget || own == -INFINITY ? r : own + v;
     loss[i] = v;
 }

@@ -70,3 +70,44 @@ def test_rows_and_queries_of_opposite_sizes(nq, nb, dim, size, dtype):
     within(loss, e["loss"], tl, "loss")
     within(dq, e["dq"], tq, "dq")
     within(db, e["db"], tb, "db")
+
+
+# ---- values that are not finite
+
+def sharded(base, q, t, w, scale, cuts):
+    b, x, tt, ww = base.cuda(), q.cuda(), t.cuda(), w.cuda()
+    parts = [softmax.softmax_shard_dev(b[lo:hi], x, tt, scale, id_base=lo, want_mean=True) for lo, hi in zip(cuts, cuts[1:])]
+    lse, loss = softmax.softmax_merge_dev(torch.stack([p[0] for p in parts]), torch.stack([p[1] for p in parts]), tt)
+    grads = [softmax.softmax_grad_dev(b[lo:hi], x, tt, scale, lse, loss, ww, rest=p[0], mean=p[4], id_base=lo) for (lo, hi), p in zip(zip(cuts, cuts[1:]), parts)]
+    return lse.cpu(), loss.cpu(), sum(g[0].double().cpu() for g in grads), torch.cat([g[1] for g in grads]).cpu()
+
+
+CUTS = [(0, 300), (0, 150, 300), (0, 70, 70, 299, 300)]
+
+
+@pytest.mark.parametrize("cuts", CUTS)
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_a_query_of_nan_shows_over_shards(dtype, cuts):
+    """wherever its target lies, and where it has none: not like a query whose target no shard holds"""
+    base, q, targets, w, scale = make(20, 300, 40, dtype, seed=30)
+    targets[0], targets[6], targets[7], targets[8], targets[9] = -1, 20, 299, 300, -1
+    want = sharded(base, q, targets, w, scale, cuts)
+    assert want[1][8] == np.inf and want[1][9] == 0
+    bad = q.clone()
+    bad[6:10, 3] = float("nan")
+    lse, loss, dq, db = sharded(base, bad, targets, w, scale, cuts)
+    ok = torch.tensor([i for i in range(20) if not 6 <= i <= 9])
+    assert torch.equal(loss[ok], want[1][ok]) and torch.equal(lse[ok], want[0][ok]) and torch.equal(dq[ok], want[2][ok])
+    assert loss[6:9].isnan().all() and loss[9] == 0 and lse[6:10].isnan().all()
+    assert dq[6:9].isnan().all() and not dq[9].any() and db.isnan().all()
+
+
+@pytest.mark.parametrize("cuts", CUTS[:2])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nq", [20, 300])
+def test_a_row_of_nan_shows_over_shards(nq, dtype, cuts):
+    base, q, targets, w, scale = make(nq, 300, 40, dtype, seed=31)
+    targets[0] = -1
+    base[200, 1] = float("nan")
+    lse, loss, dq, db = sharded(base, q, targets, w, scale, cuts)
+    assert loss[1:].isnan().all() and loss[0] == 0 and lse.isnan().all() and dq[1:].isnan().all(1).all() and not dq[0].any()
