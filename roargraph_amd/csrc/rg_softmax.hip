@@ -34,6 +34,11 @@ __device__ __forceinline__ bool target_here(uint32_t t, uint32_t id_base, uint32
 // log(1 + e^d) without overflow: loss of a target d below the others' log sum
 __device__ __forceinline__ float softplus(float d) { return d > 15.0f ? d + log1pf(expf(-d)) : log1pf(expf(d)); }
 
+// the loss of a target whose logit is `own`, d below the others' log sum, and the log sum r with it: a logit of +inf is infinity less infinity, no
+// perfect answer; one of -inf takes no part in the sum
+__device__ __forceinline__ float loss_of(float own, float d) { return own == INFINITY ? NAN : own == -INFINITY ? INFINITY : softplus(d); }
+__device__ __forceinline__ float lse_of(float own, float loss, float r) { return own == -INFINITY ? r : own + loss; }
+
 // joins the slots of a query: rest, target logit, lse, loss, mean of the others.  One workgroup per query, or, where queries are few, per query
 // and kJoinDims of the mean's elements; with many slots, sixteen groups of lanes share them
 // (244 slots of 333 queries x 93: four groups of single elements 25 us, now 12 us).
@@ -80,10 +85,10 @@ __global__ void __launch_bounds__(256) rg_softmax_join_kernel(const float4 *ml, 
         // (in 64 bits: the instruction behind log2f rounds down, which a small loss shows)
         const double r2 = none ? -INFINITY : (double)M + log2((double)l), z2 = here ? own2[i] : -INFINITY;
         const float r = (float)(r2 * kLn2), z = (float)(z2 * kLn2);
-        const float v = t == kNoTarget ? 0.0f : here ? softplus((float)((r2 - z2) * kLn2)) : r != r ? r : INFINITY;
+        const float v = t == kNoTarget ? 0.0f : r != r ? r : here ? loss_of(z, (float)((r2 - z2) * kLn2)) : INFINITY;
         rest[i] = r;
         own[i] = z;
-        if (lse) lse[i] = here ? z + v : r;
+        if (lse) lse[i] = here ? lse_of(z, v, r) : r;
         if (loss) loss[i] = v;
     }
     if (mean) {
@@ -134,8 +139,8 @@ __global__ void __launch_bounds__(256) rg_softmax_merge_kernel(const float *rest
     const float ref = m == -INFINITY ? 0.0f : m;
     for (uint32_t s = 0; s < nlists; ++s) l += expf(rest_in[(size_t)s * nq + i] - ref);       // (NaN where a shard's rest is)
     const float r = l == 0.0f ? -INFINITY : ref + logf(l);
-    const float v = targets[i] == kNoTarget ? 0.0f : r != r ? r : own == -INFINITY ? INFINITY : softplus(r - own);
-    lse[i] = targets[i] == kNoTarget || own == -INFINITY ? r : own + v;
+    const float v = targets[i] == kNoTarget ? 0.0f : r != r ? r : loss_of(own, r - own);
+    lse[i] = targets[i] == kNoTarget ? r : lse_of(own, v, r);
     loss[i] = v;
 }
 

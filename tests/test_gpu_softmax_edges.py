@@ -111,3 +111,50 @@ def test_a_row_of_nan_shows_over_shards(nq, dtype, cuts):
     base[200, 1] = float("nan")
     lse, loss, dq, db = sharded(base, q, targets, w, scale, cuts)
     assert loss[1:].isnan().all() and loss[0] == 0 and lse.isnan().all() and dq[1:].isnan().all(1).all() and not dq[0].any()
+
+
+@pytest.mark.parametrize("cuts", CUTS)
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nq", [20, 300])
+def test_a_target_of_infinity(nq, dtype, cuts):
+    """z_target = +inf: inf - inf, no perfect answer (loss and lse NaN).  z_target = -inf: loss +inf, lse without it, and the other rows' gradients as they are."""
+    base, q, targets, w, scale = make(nq, 300, 40, dtype, seed=32)
+    targets[targets == 100] = 101
+    base[100, 5] = float("inf")
+    q[:, 5] = -q[:, 5].abs().clamp(min=0.01)                      # every query gives row 100 a logit of -inf ...
+    targets[3] = 100
+    q[4, 5], targets[4] = 0.25, 100                               # ... and this one +inf
+    lse, loss, dq, db = sharded(base, q, targets, w, scale, cuts)
+    one = step(base, q, targets, w, scale)[0].cpu()
+    assert torch.equal(one.isnan(), loss.isnan()) and torch.equal(one == np.inf, loss == np.inf)
+    assert loss[4].isnan() and lse[4].isnan() and dq[4].isnan().all()
+    keep = torch.tensor([i for i in range(nq) if i != 4])
+    without = torch.cat((base[:100], base[101:]))
+    t = torch.where(targets > 100, targets - 1, targets)
+    t[3], t[4] = -1, -1
+    e = exact(without, q, t, w, scale)
+    tl, _, _ = tolerances(without, q, t, w, scale, e, dtype)
+    rest = [i for i in keep.tolist() if i != 3]
+    assert ((one.double() - e["loss"]).abs() <= tl)[rest].all()
+    tl = tl * len(cuts)
+    assert ((loss.double() - e["loss"]).abs() <= tl)[rest].all() and ((lse.double() - e["lse"]).abs() <= tl + 4 * U * e["lse"].abs())[keep].all()
+    assert loss[3] == np.inf
+    # db of the other rows where the query of NaN takes no part
+    targets[4] = -1
+    lse, loss, dq, db = sharded(base, q, targets, w, scale, cuts)
+    x, ww = q.double(), w.double().clone()
+    ww[4] = 0
+    p = torch.exp(e["z"] - e["lse"][:, None]) * ww[:, None]
+    for i in rest:
+        if t[i] >= 0:
+            p[i, t[i]] -= ww[i]
+    size = p.abs()
+    want = scale * p.T @ x
+    # (t = -1 for query 3 in the oracle's tolerances, so they are made here: weights off by the rounding and by 2 |dz|, sums, the last rounding)
+    top = float(without.double().norm(dim=1).max() * x.norm(dim=1).max()) * scale
+    dz = top * 48 * U + (3 * 2.0 ** -22 * 40 ** 0.5 * top if dtype == "f32" else 0)
+    half = {"f32": 2.0 ** -22, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[dtype]
+    tol = scale * (half + 4 * dz + (nq + 8) * U) * size.T @ x.abs() + HALF[dtype] * want.abs() + {"f32": 1e-30, "f16": 2.0 ** -24, "bf16": 1e-30}[dtype]
+    tol = tol + scale * 2.0 ** -32 * size.amax(0)[:, None] * x.abs().sum(0)[None]
+    others = torch.cat((db[:100], db[101:])).double()
+    assert torch.isfinite(others).all() and ((others - want).abs() <= tol).all()
