@@ -138,8 +138,9 @@ __global__ void __launch_bounds__(256) rg_softmax_merge_kernel(const float *rest
     float l = 0.0f;
     const float ref = m == -INFINITY ? 0.0f : m;
     for (uint32_t s = 0; s < nlists; ++s) l += expf(rest_in[(size_t)s * nq + i] - ref);       // (NaN where a shard's rest is)
-    const float r = l == 0.0f ? -INFINITY : ref + logf(l);
-    const float v = targets[i] == kNoTarget ? 0.0f : r != r ? r : loss_of(own, r - own);
+    const double r2 = l == 0.0f ? -INFINITY : (double)ref + log((double)l);        // (in 64 bits, as in the join: a sum near the target's logit keeps its digits)
+    const float r = (float)r2;
+    const float v = targets[i] == kNoTarget ? 0.0f : r != r ? r : loss_of(own, (float)(r2 - own));
     lse[i] = targets[i] == kNoTarget ? r : lse_of(own, v, r);
     loss[i] = v;
 }

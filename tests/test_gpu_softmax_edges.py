@@ -158,3 +158,32 @@ def test_a_target_of_infinity(nq, dtype, cuts):
     tol = tol + scale * 2.0 ** -32 * size.amax(0)[:, None] * x.abs().sum(0)[None]
     others = torch.cat((db[:100], db[101:])).double()
     assert torch.isfinite(others).all() and ((others - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("scale", [20.0, 40.0, 80.0])
+def test_small_losses_keep_their_digits_over_shards(scale):
+    """loss = log(1 + e^(rest - own)) of two shards: rest and own are fp32 values, off by U of themselves, and by 2 U scale as in the one-shard form"""
+    base, q = torch.eye(64), torch.eye(64)[:32]
+    t = torch.arange(32, dtype=torch.int32)
+    lse, loss, dq, db = sharded(base, q, t, torch.ones(32), scale, (0, 20, 64))
+    want = torch.log1p(63 * torch.exp(torch.tensor(-scale, dtype=torch.float64)))
+    # (the shards' rests are logs of at most 63; the last two terms: 4 of them, and a few roundings of the loss)
+    assert ((loss.double() - want).abs() <= want * (3 * scale + 4 * 4.2 + 16) * U).all()
+
+
+def test_a_merge_is_as_good_as_its_lists():
+    """loss = log(1 + e^d), d = rest - own of the lists' fp32 values: d is off by U of itself and by 4 U of its sum's logarithm (fp32 sum of 3 terms, each to 2 ulp), however
+    large rest and own are; exponential and logarithm of the loss to 2 ulp each"""
+    g = torch.Generator().manual_seed(50)
+    nq = 2000
+    base = torch.rand(nq, generator=g) * 400 - 200
+    rest = base[None] + torch.randn(3, nq, generator=g) * 2
+    own = torch.full((3, nq), -np.inf)
+    own[torch.arange(nq) % 3, torch.arange(nq)] = base + torch.randn(nq, generator=g) * 4
+    t = torch.zeros(nq, dtype=torch.int32)
+    lse, loss = softmax.softmax_merge_dev(rest.cuda(), own.cuda(), t.cuda())
+    r, o = torch.logsumexp(rest.double(), 0), own.double().amax(0)
+    d = r - o
+    want = torch.nn.functional.softplus(d, threshold=1e9)
+    assert ((loss.cpu().double() - want).abs() <= torch.sigmoid(d) * (d.abs() + 12) * U + 8 * U * want).all()
+    assert ((lse.cpu().double() - (o + want)).abs() <= U * (o + want).abs() + 2 * U * o.abs() + 20 * U * (1 + want)).all()
