@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(256) rg_softmax_planes_kernel(const void *rows
                 *reinterpret_cast<half8 *>(out + 8 * (lc + 16 * i)) = hi;
                 *reinterpret_cast<half8 *>(out + ks * 32 + 8 * (lc + 16 * i)) = lo;
             }
-            if (lc == 0) put_info(info, r, row_factor(top, e), (float)e, 1.0f, kNoTarget);
+            if (lc == 0) put_info(info, r, row_factor(top, e), row_bias(top, e), 1.0f, kNoTarget);
         } else {
 #pragma unroll
             for (int i = 0; i < CI; ++i)

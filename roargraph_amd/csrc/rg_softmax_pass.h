@@ -185,6 +185,10 @@ __device__ __forceinline__ void split8(Chunk<RG_DTYPE_F32> c, float top, float s
     }
 }
 
+// the bias of a streamed fp32 row's logits in kMean, its scale.  Of a row that is not finite the second product would take the signs: with logits of -inf,
+// which leave the loss alone, its weight is 0, and 0 times infinity is no number.
+__device__ __forceinline__ float row_bias(float top, int e) { return top < INFINITY ? (float)e : NAN; }
+
 // stationary operands of row x: lane (n, g) holds elements 32 ks + 8 g .. + 7 of part kq of KQ of the row; returns what its logits are
 // multiplied by
 template <int DT, int KS, int KQ, int NP>

@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(256, (ThinCfg<DT, KS>::WPS)) rg_softmax_thin_k
             }
             if (F32 && lc == 0) {
                 yv[r] = row_factor(top, e);
-                yv[32 + r] = MODE == kMean ? (float)e : 0.0f;
+                yv[32 + r] = MODE == kMean ? row_bias(top, e) : 0.0f;
             }
         }
     };

@@ -160,6 +160,19 @@ def test_a_target_of_infinity(nq, dtype, cuts):
     assert torch.isfinite(others).all() and ((others - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nq,dim", [(20, 40), (300, 40), (9, 520), (200, 700)])
+def test_a_row_of_minus_infinity_shows_in_the_queries_gradients(nq, dim, dtype):
+    """a row with an infinity whose logits are all -inf takes no part in the losses; 0 times infinity is no number, so the gradients of the queries show it"""
+    base, q, targets, w, scale = make(nq, 300, dim, dtype, seed=33)
+    targets[targets == 100] = 101
+    targets[0] = -1
+    base[100, 5] = float("inf")
+    q[:, 5] = -q[:, 5].abs().clamp(min=0.01)
+    loss, (dq,) = step(base, q, targets, w, scale, grads="q")
+    assert torch.isfinite(loss).all() and dq[1:, 5].isnan().all() and not dq[0].any()
+
+
 @pytest.mark.parametrize("scale", [20.0, 40.0, 80.0])
 def test_small_losses_keep_their_digits_over_shards(scale):
     """loss = log(1 + e^(rest - own)) of two shards: rest and own are fp32 values, off by U of themselves, and by 2 U scale as in the one-shard form"""
