@@ -158,11 +158,10 @@ def _softmax_function():
         # the calls of softmax_shard_dev and softmax_grad_dev with fewer tensors between them: rest, own, lse and the mean rows in one
         class SoftmaxLoss(torch.autograd.Function):
             @staticmethod
-            def forward(ctx, queries, base, targets, scale):
+            def forward(ctx, queries, base, targets, scale, want_mean):
                 q, b = _rows(queries, "queries"), _rows(base, "base")
                 _check_pair(q, b)
                 (nq, dim), nb, code = q.shape, b.shape[0], _dtype_code(b)
-                want_mean = ctx.needs_input_grad[0]
                 loss = b.new_empty(nq, dtype=torch.float32)
                 kept = b.new_empty((3 + dim if want_mean else 3) * nq, dtype=torch.float32)
                 work, n = _scratch(MEAN if want_mean else STATS, nb, nq, dim, b)
@@ -186,7 +185,7 @@ def _softmax_function():
                 at = kept.data_ptr()
                 check(lib().rg_softmax_grad_dev(b.data_ptr(), nb, _stride(b), q.data_ptr(), nq, _stride(q), dim, code, ctx.scale, targets.data_ptr(), 0, at + 8 * nq, loss.data_ptr(),
                                                 at, at + 12 * nq if dq is not None else None, weights.data_ptr(), _ptr(dq), dim, _ptr(db), dim, work.data_ptr(), n, _device(b), _stream(b)))
-                return dq, db, None, None
+                return dq, db, None, None, None
 
         _function = SoftmaxLoss
     return _function
@@ -194,5 +193,7 @@ def _softmax_function():
 
 def softmax_loss(queries, base, targets, scale=1.0):
     """Cross entropy of softmax(scale * queries @ base.T) against `targets`, per query [nq] fp32; differentiable (once) in queries and base."""
+    import torch
     targets = _targets(targets, queries.shape[0], base)
-    return _softmax_function().apply(queries, base, targets, float(scale))
+    # (the mean rows are for the queries' gradient only; inside forward a leaf wants one even under no_grad)
+    return _softmax_function().apply(queries, base, targets, float(scale), queries.requires_grad and torch.is_grad_enabled())

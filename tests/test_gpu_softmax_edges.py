@@ -200,3 +200,25 @@ def test_a_merge_is_as_good_as_its_lists():
     want = torch.nn.functional.softplus(d, threshold=1e9)
     assert ((loss.cpu().double() - want).abs() <= torch.sigmoid(d) * (d.abs() + 12) * U + 8 * U * want).all()
     assert ((lse.cpu().double() - (o + want)).abs() <= U * (o + want).abs() + 2 * U * o.abs() + 20 * U * (1 + want)).all()
+
+
+# ---- calls
+
+def asked(monkeypatch):
+    """which kinds of scratch calls ask for"""
+    kinds, scratch = [], softmax._scratch
+    monkeypatch.setattr(softmax, "_scratch", lambda what, *a: kinds.append(what) or scratch(what, *a))
+    return kinds
+
+
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_without_gradients_no_mean_is_made(monkeypatch, mode):
+    base, q, targets, w, scale = make(30, 500, 40, "bf16", seed=34)
+    kinds = asked(monkeypatch)
+    b, x, t = base.cuda().requires_grad_(), q.cuda().requires_grad_(), targets.cuda()
+    want = softmax.softmax_loss(x, b, t, scale)
+    with mode():
+        loss = softmax.softmax_loss(x, b, t, scale)
+    assert torch.equal(loss, want) and not loss.requires_grad
+    softmax.softmax_loss(x.detach(), b, t, scale)
+    assert kinds == [softmax.MEAN, softmax.STATS, softmax.STATS]
