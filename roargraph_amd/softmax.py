@@ -192,8 +192,13 @@ def _softmax_function():
 
 
 def softmax_loss(queries, base, targets, scale=1.0):
-    """Cross entropy of softmax(scale * queries @ base.T) against `targets`, per query [nq] fp32; differentiable (once) in queries and base."""
+    """Cross entropy of softmax(scale * queries @ base.T) against `targets`, per query [nq] fp32; differentiable (once) in queries and base.
+
+    scale is a number (one held in a GPU tensor is read back, which waits for the GPU).  A learned one goes into the queries, softmax_loss(queries * s, base,
+    targets), which gives it its gradient; a scale that requires grad is refused."""
     import torch
+    if isinstance(scale, torch.Tensor) and scale.requires_grad and torch.is_grad_enabled():
+        raise TypeError("softmax_loss: the scale gets no gradient here; multiply the queries by it instead: softmax_loss(queries * scale, base, targets)")
     targets = _targets(targets, queries.shape[0], base)
     # (the mean rows are for the queries' gradient only; inside forward a leaf wants one even under no_grad)
     return _softmax_function().apply(queries, base, targets, float(scale), queries.requires_grad and torch.is_grad_enabled())

@@ -222,3 +222,25 @@ def test_without_gradients_no_mean_is_made(monkeypatch, mode):
     assert torch.equal(loss, want) and not loss.requires_grad
     softmax.softmax_loss(x.detach(), b, t, scale)
     assert kinds == [softmax.MEAN, softmax.STATS, softmax.STATS]
+
+
+def test_a_learned_scale_goes_into_the_queries():
+    """scale is a number; queries * s gives a learned one its gradient: dL/ds = sum_i q_i . dL/d(s q_i)"""
+    base, q, targets, w, scale = make(30, 500, 40, "f32", seed=35)
+    b, x, t = base.cuda(), q.cuda(), targets.cuda()
+    s = torch.tensor(8.0, device="cuda", requires_grad=True)
+    with pytest.raises(TypeError, match="queries"):
+        softmax.softmax_loss(x, b, t, s)
+    with pytest.raises(TypeError, match="queries"):
+        softmax.softmax_loss(x, b, t, scale=s.log().exp())
+    want = softmax.softmax_loss(x, b, t, 8.0)
+    with torch.no_grad():
+        assert torch.equal(softmax.softmax_loss(x, b, t, s), want)
+    assert torch.equal(softmax.softmax_loss(x, b, t, s.detach()), want)
+    loss = softmax.softmax_loss(x * s, b, t)
+    (ds,) = torch.autograd.grad(loss, s, w.cuda())
+    e = exact(base, q * 8.0, targets, w, 1.0)
+    tl, tq, _ = tolerances(base, q * 8.0, targets, w, 1.0, e, "f32")
+    within(loss.detach(), e["loss"], tl, "loss")
+    x64 = q.double()
+    assert abs(ds.item() - (e["dq"] * x64).sum().item()) <= ((tq + (30 * 40) * U * e["dq"].abs()) * x64.abs()).sum().item()

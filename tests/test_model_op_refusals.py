@@ -85,3 +85,12 @@ def test_scratch_sizes():
     with pytest.raises(RgError):
         softmax.workspace(0, 10, 10, 0, 0)
     assert lib().rg_softmax_workspace(C.c_int(0), u32(1), u32(1), u32(8), C.c_int(0), None) == RG_ERR_ARG
+
+
+def test_a_scale_that_requires_grad():
+    import torch
+    s = torch.tensor(2.0, requires_grad=True)
+    x, t = torch.zeros(2, 8), torch.zeros(2, dtype=torch.int32)
+    for scale in (s, s.exp()):
+        with pytest.raises(TypeError, match="queries"):
+            softmax.softmax_loss(x, x, t, scale)
