@@ -9,7 +9,7 @@ Thin host layer over the C ABI (rg_q4_*, include/rg.h); everything is torch CUDA
 from collections import namedtuple
 
 from ._lib import check, lib
-from .softmax import _device, _dtype_code, _ptr, _rows, _stream, _stride
+from .softmax import _counts, _device, _dtype_code, _ptr, _rows, _stream, _stride
 
 # codes uint8 [nb, >= ceil(dim / 8) * 4], scales fp16 [nb, ceil(dim / group)], mins alike or None (rg.h: "a base in 4 bits")
 Q4Base = namedtuple("Q4Base", "codes scales mins dim group")
@@ -21,6 +21,7 @@ def _check_form(p):
     nb = p.codes.shape[0]
     if p.codes.dtype != torch.uint8 or p.codes.dim() != 2 or p.codes.stride(1) != 1 or not p.codes.is_cuda:
         raise ValueError("codes: rows of uint8 on a GPU are wanted")
+    _counts(p.codes, "codes")
     if p.codes.shape[1] < -(-p.dim // 8) * 4:
         raise ValueError("codes: %d bytes a row, dim %d needs %d" % (p.codes.shape[1], p.dim, -(-p.dim // 8) * 4))
     if nb > 1 and p.codes.stride(0) < p.codes.shape[1]:
@@ -61,6 +62,7 @@ def q4_unpack(packed, ids=None):
     if ids is not None:
         if ids.dim() != 1 or ids.device != packed.codes.device or ids.dtype not in (torch.int32, torch.int64):
             raise ValueError("ids: a vector of int32 or int64 on %s is wanted" % packed.codes.device)
+        _counts(ids, "ids")
         if ids.dtype == torch.int64:
             ids = ids.clamp(-1, 0xffffffff).to(torch.int32)      # (what 32 bits cannot say becomes an id that is no row)
         ids = ids.contiguous()

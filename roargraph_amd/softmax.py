@@ -30,10 +30,23 @@ def _dtype_code(t):
     return code
 
 
+def _counts(t, name):
+    """sizes reach the C ABI in 32 bits, of which ctypes takes the lowest without a word"""
+    if max(t.shape) > 0x7fffffff:
+        raise ValueError("%s: at most 2^31 - 1 rows and columns, got shape %s" % (name, tuple(t.shape)))
+
+
+def _id_base(n):
+    if not 0 <= n <= 0xffffffff:
+        raise ValueError("id_base: a row id of 32 bits is wanted, got %d" % n)
+    return n
+
+
 def _rows(t, name):
     """t itself where its rows can be read in place, else a contiguous copy (transposed or broadcast tensors)."""
     if t.dim() != 2:
         raise ValueError("%s: a matrix of rows is wanted, got shape %s" % (name, tuple(t.shape)))
+    _counts(t, name)
     if t.stride(1) == 1 and t.stride(0) >= t.shape[1] or t.is_contiguous():
         return t
     return t.contiguous()
@@ -82,6 +95,8 @@ def _targets(targets, n, like):
 @functools.lru_cache(maxsize=1024)
 def workspace(what, nb, nq, dim, dtype_code):
     """rg_softmax_workspace: bytes of scratch of one call"""
+    if not 0 <= min(nb, nq, dim) <= max(nb, nq, dim) <= 0xffffffff:
+        raise ValueError("sizes of 32 bits are wanted, got %d, %d, %d" % (nb, nq, dim))
     n = C.c_uint64()
     check(lib().rg_softmax_workspace(what, nb, nq, dim, dtype_code, C.byref(n)))
     return n.value
@@ -97,7 +112,7 @@ def softmax_shard_dev(base_t, queries_t, targets_t, scale, id_base=0, want_mean=
     """rg_softmax_shard_dev on the current stream: (rest, own, lse, loss, mean) of one row shard, fp32; lse and loss as if the shard were the
     whole base; mean is None unless asked for."""
     import torch
-    queries_t, base_t = _rows(queries_t, "queries"), _rows(base_t, "base")
+    queries_t, base_t, id_base = _rows(queries_t, "queries"), _rows(base_t, "base"), _id_base(id_base)
     _check_pair(queries_t, base_t)
     nq, nb, dim = queries_t.shape[0], base_t.shape[0], base_t.shape[1]
     targets_t = _targets(targets_t, nq, base_t)
@@ -116,6 +131,7 @@ def softmax_merge_dev(rest_in, own_in, targets_t):
     import torch
     if rest_in.dim() != 2 or rest_in.shape != own_in.shape or rest_in.dtype != torch.float32 or own_in.dtype != torch.float32 or rest_in.device != own_in.device:
         raise ValueError("rest and own: two fp32 matrices [nlists, nq] on one GPU are wanted")
+    _counts(rest_in, "rest and own")
     rest_in, own_in = rest_in.contiguous(), own_in.contiguous()
     targets_t = _targets(targets_t, rest_in.shape[1], rest_in)
     lse, loss = torch.empty((2, rest_in.shape[1]), dtype=torch.float32, device=rest_in.device).unbind(0)
@@ -128,7 +144,7 @@ def softmax_grad_dev(base_t, queries_t, targets_t, scale, lse, loss, weights, re
     """rg_softmax_grad_dev: (this shard's part of dq, the shard's rows of db).  lse, loss: over the whole base; rest, mean: this shard's
     (for dq only); weights = dL/dloss [nq]."""
     import torch
-    queries_t, base_t = _rows(queries_t, "queries"), _rows(base_t, "base")
+    queries_t, base_t, id_base = _rows(queries_t, "queries"), _rows(base_t, "base"), _id_base(id_base)
     _check_pair(queries_t, base_t)
     nq, nb, dim = queries_t.shape[0], base_t.shape[0], base_t.shape[1]
     targets_t = _targets(targets_t, nq, base_t)

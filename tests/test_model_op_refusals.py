@@ -94,3 +94,23 @@ def test_a_scale_that_requires_grad():
     for scale in (s, s.exp()):
         with pytest.raises(TypeError, match="queries"):
             softmax.softmax_loss(x, x, t, scale)
+
+
+def test_sizes_beyond_32_bits():
+    """(ctypes takes the lowest 32 bits of a number: 2^32 + 5 rows would be 5)"""
+    import torch
+    from roargraph_amd import q4
+    t = torch.zeros(3, dtype=torch.int32)
+    x = torch.zeros(3, 32)
+    for shape in ((2 ** 31, 1), (2 ** 32 + 5, 1), (1, 2 ** 32 + 8)):
+        far = torch.empty(shape, device="meta")
+        for call in (lambda: softmax.softmax_shard_dev(far, x, t, 1.0), lambda: softmax.softmax_grad_dev(x, far, t, 1.0, x, x, x), lambda: q4.q4_pack(far)):
+            with pytest.raises(ValueError, match="2\\^31"):
+                call()
+    for id_base in (-1, 2 ** 32):
+        for call in (lambda: softmax.softmax_shard_dev(x, x, t, 1.0, id_base=id_base), lambda: softmax.softmax_grad_dev(x, x, t, 1.0, x, x, x, id_base=id_base)):
+            with pytest.raises(ValueError, match="id_base"):
+                call()
+    for sizes in ((2 ** 32, 1, 8), (1, 2 ** 32 + 1, 8), (1, 1, 2 ** 32 + 8), (-1, 1, 8)):
+        with pytest.raises(ValueError, match="32 bits"):
+            softmax.workspace(softmax.STATS, *sizes, 0)
