@@ -15,8 +15,14 @@ from .softmax import _counts, _device, _dtype_code, _ptr, _rows, _stream, _strid
 Q4Base = namedtuple("Q4Base", "codes scales mins dim group")
 
 
+def _check_group(group):
+    if group not in (32, 64, 128):
+        raise ValueError("groups of 32, 64 or 128 elements")
+
+
 def _check_form(p):
     import torch
+    _check_group(p.group)
     groups = -(-p.dim // p.group)
     nb = p.codes.shape[0]
     if p.codes.dtype != torch.uint8 or p.codes.dim() != 2 or p.codes.stride(1) != 1 or not p.codes.is_cuda:
@@ -43,8 +49,9 @@ def q4_pack(base_t, group=32, mins=False):
     base_t = _rows(base_t, "base")
     code = _dtype_code(base_t)
     nb, dim = base_t.shape
-    if group not in (32, 64, 128):
-        raise ValueError("groups of 32, 64 or 128 elements")
+    if not base_t.is_cuda:
+        raise ValueError("base: a tensor on a GPU is wanted, got one on %s" % base_t.device)
+    _check_group(group)
     groups = -(-dim // group)
     codes = torch.empty((nb, -(-dim // 8) * 4), dtype=torch.uint8, device=base_t.device)
     both = torch.empty((2 if mins else 1, nb, groups), dtype=torch.float16, device=base_t.device)

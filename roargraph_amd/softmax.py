@@ -129,7 +129,7 @@ def softmax_shard_dev(base_t, queries_t, targets_t, scale, id_base=0, want_mean=
 def softmax_merge_dev(rest_in, own_in, targets_t):
     """rg_softmax_merge_dev: statistics [nlists, nq] of the row shards -> (lse, loss) over the whole base."""
     import torch
-    if rest_in.dim() != 2 or rest_in.shape != own_in.shape or rest_in.dtype != torch.float32 or own_in.dtype != torch.float32 or rest_in.device != own_in.device:
+    if rest_in.dim() != 2 or rest_in.shape != own_in.shape or rest_in.dtype != torch.float32 or own_in.dtype != torch.float32 or rest_in.device != own_in.device or not rest_in.is_cuda:
         raise ValueError("rest and own: two fp32 matrices [nlists, nq] on one GPU are wanted")
     _counts(rest_in, "rest and own")
     rest_in, own_in = rest_in.contiguous(), own_in.contiguous()

@@ -114,3 +114,15 @@ def test_sizes_beyond_32_bits():
     for sizes in ((2 ** 32, 1, 8), (1, 2 ** 32 + 1, 8), (1, 1, 2 ** 32 + 8), (-1, 1, 8)):
         with pytest.raises(ValueError, match="32 bits"):
             softmax.workspace(softmax.STATS, *sizes, 0)
+
+
+def test_tensors_of_the_host_and_unknown_groups():
+    import torch
+    from roargraph_amd import q4
+    x, t = torch.zeros(3, 32), torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="GPU"):
+        q4.q4_pack(x)
+    with pytest.raises(ValueError, match="GPU"):
+        softmax.softmax_merge_dev(torch.zeros(1, 3), torch.zeros(1, 3), t)
+    with pytest.raises(ValueError, match="groups"):
+        q4.q4_score(x, q4.Q4Base(torch.zeros(4, 16, dtype=torch.uint8), torch.zeros(4, 1).half(), None, 32, 0))
