@@ -57,6 +57,29 @@ def test_a_hard_negative_next_to_the_target(nq, nb, dim, dist, dtype):
     assert worst <= 1.0, worst
 
 
+@pytest.mark.parametrize("nq,nb,dim", [(100, 20000, 200), (700, 20000, 64), (100, 6000, 1024), (60, 9000, 512), (33, 5000, 93)])
+def test_the_weight_of_a_target_keeps_16_bits(nq, nb, dim):
+    """bf16, gradient of the rows that are a target: nearly all of it is -w (1 - p) q of one query, which is multiplied to 16 bits, so that its error is that of
+    the last rounding (0.0017 of the norm; with 8 bits of that weight 0.0024); the other queries' weights, rounded to 8 bits, are few"""
+    base, q, _, _, _ = make(nq, nb, dim, "bf16", seed=nq)
+    targets = torch.randperm(nb, generator=torch.Generator().manual_seed(1))[:nq].int()
+    g = torch.Generator().manual_seed(2)
+    w, scale = 0.5 + torch.rand(nq, generator=g), 1.0
+    e = exact(base, q, targets, w, scale)
+    got = step(base, q, targets, w, scale, grads="b")[1][0].double().cpu()
+    t = targets.long()
+    x = q.double().abs()
+    own = e["g"][torch.arange(nq), t].abs()
+    others = e["g"].abs()[:, t]
+    others[torch.arange(nq), torch.arange(nq)] = 0
+    dz = float(base.double().norm(dim=1).max() * x.norm(dim=1).max()) * scale * (dim + 8) * U
+    delta = scale * ((2.0 ** -8 + 2 * dz) * others.T @ x + (2.0 ** -16 + 2 * dz) * own[:, None] * x + (nq + 8) * U * (others.T @ x + own[:, None] * x))
+    want = e["db"][t]
+    last = (rounded(want, "bf16") - want).norm()
+    assert (got[t] - want).norm() <= last + 2 * delta.norm(), ((got[t] - want).norm() / want.norm(), last / want.norm(), delta.norm() / want.norm())
+    assert last + 2 * delta.norm() < 0.0021 * want.norm()          # (the bound tells the two apart)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("nq,nb,dim", [(33, 300, 40), (200, 500, 200), (20, 90, 520)])
 @pytest.mark.parametrize("size", [1e24, 1e-24, 1e28])
@@ -244,3 +267,35 @@ def test_a_learned_scale_goes_into_the_queries():
     within(loss.detach(), e["loss"], tl, "loss")
     x64 = q.double()
     assert abs(ds.item() - (e["dq"] * x64).sum().item()) <= ((tq + (30 * 40) * U * e["dq"].abs()) * x64.abs()).sum().item()
+
+
+def test_a_whole_step_is_captured():
+    """forward and backward of leaves that no eager graph holds, replayed on new inputs between eager steps"""
+    sets = [[a.cuda() for a in make(50, 3000, 200, "bf16", seed=40 + k)[:4]] for k in range(3)]
+
+    def run(b, x, t, w):
+        loss = softmax.softmax_loss(x, b, t, 8.0)
+        return (loss.detach(),) + torch.autograd.grad(loss, (x, b), w)
+
+    def leaves(s):
+        return s[0].clone().requires_grad_(), s[1].clone().requires_grad_(), s[2].clone(), s[3].clone()
+
+    want = [run(*leaves(s)) for s in sets]
+    held, side, graph = leaves(sets[0]), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        run(*held)
+        side.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            out = run(*held)
+    torch.cuda.synchronize()
+    for k in (1, 2, 0, 1):
+        with torch.no_grad():
+            for h, s in zip(held, sets[k]):
+                h.copy_(s)
+        torch.cuda.synchronize()
+        graph.replay()
+        eager = run(*leaves(sets[k]))
+        torch.cuda.synchronize()
+        for a, b, c in zip(out, eager, want[k]):
+            assert torch.equal(a, c) and torch.equal(b, c), k
