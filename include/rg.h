@@ -316,8 +316,13 @@ rg_status rg_groundtruth(const char *base_fbin, const char *query_fbin, const ch
  * Rows are `dtype` (RG_DTYPE_*; base, queries and their gradients alike), row strides in elements (any stride >= dim, any alignment of
  * the element; 16-bit rows of a multiple of 8 elements, 16-byte aligned, are read in place by every kernel), dim 1 .. 1024, sums in fp32, at
  * most 2^24 - 1 queries a call.  fp32 rows are multiplied as pairs of 16-bit halves: 22 bits of every element, or 2^-39 of
- * the largest of its row.  Targets are global ids (row + id_base);
+ * the largest of its row.  The weights exp(z) of a gradient's sums are multiplied in the rows' type (8 bits of bf16, 11 of fp16 down to 2^-32 of the
+ * largest, fp32 rows 22 alike; a target's weight in the gradient of bf16 rows 16), the mean is divided by their sum as multiplied; bf16 elements up to 2^80, and
+ * queries times loss weights up to 2^100, keep the sums in fp32's range.  Targets are global ids (row + id_base);
  * 0xffffffff = the query has no row: loss 0, no gradient, whatever it holds.  A target no shard holds: own = -inf, loss = +inf.
+ * What is not finite shows: loss and lse of a query that holds a NaN, or has a logit that is NaN or +inf (its target's too), are NaN, over shards as
+ * over one.  A row whose logit is -inf takes no part in the sums (as the target: loss = +inf), but the gradients of the queries, where 0 meets its infinity,
+ * are NaN (fp32 rows: in all elements).
  *
  * Shard form, like rg_gt_shard_dev: a rank holds rows [id_base, id_base + nb).  rg_softmax_shard_dev gives rest and own over the shard
  * (-inf where the shard has no such row, mean 0 where it has none at all), rg_softmax_merge_dev joins nlists of them ([list][nq]) into
@@ -356,7 +361,8 @@ rg_status rg_softmax_grad_dev(const void *d_base, uint32_t nb, uint64_t bstride,
  * the nearest level (ties to the even code), padding codes 0.  Rows must be finite; values whose scale leaves fp16's range (6e-8 .. 65504)
  * are scaled by the caller first.
  * rg_q4_unpack_dev: the fp32 values of the rows `d_ids` lists (NULL: rows 0 .. n-1) -- for an exact re-score or further training.
- * rg_q4_score_dev: out[i][j] = <q_i, value of row j>, fp32 sums, dim 1 .. 4096; queries fp32 / fp16 / bf16.
+ * rg_q4_score_dev: out[i][j] = <q_i, value of row j>, fp32 sums, dim 1 .. 4096; queries fp32 / fp16 / bf16, of which 22 bits of every element, or
+ * 2^-39 of the query's largest, are multiplied.
  * Enqueued on `stream`, no scratch, capturable. */
 rg_status rg_q4_pack_dev(const void *d_rows, uint32_t nb, uint64_t stride, uint32_t dim, int dtype, uint32_t group, uint8_t *d_codes,
                          uint64_t cstride, uint16_t *d_scales, uint16_t *d_mins, uint64_t sstride, int device, void *stream);

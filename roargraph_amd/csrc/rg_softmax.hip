@@ -353,11 +353,11 @@ struct Plan {
 };
 
 // The kernel of a mode.  Few rows x: the pass is bound by reading y, and the thin kernel, which reads fp32 rows and rows of any alignment where
-// they lie, once for 64 rows x, beats planes made first, read and read again (1.25M x 200 fp32: 64 queries 391 us against 721 us, 128 queries
-// 633 / 818 us, 256 1167 / 1152 us; 16-bit rows that need planes gain more: 830k x 301 bf16, 256 queries 455 / 556 us) -- and of short 16-bit rows
-// that need none it still does up to 128 (2M x 64 bf16 180 / 221 us; x 200, where the wide kernel reads in place what fills its tiles, 247 / 190 us).
+// they lie, once for 64 rows x, beats planes made first, read and read again (1.25M x 200 fp32: 64 queries 349 us against 660 us, 128 queries
+// 613 / 772 us, 256 1138 / 1124 us; 16-bit rows that need planes gain more: 830k x 301 bf16, 256 queries 488 / 570 us) -- and of short 16-bit rows
+// that need none it still does up to 128 (2M x 64 bf16 179 / 226 us; 1.25M x 200, where the wide kernel reads in place what fills its tiles, 250 / 197 us).
 // It holds a row in a wave's registers: of wide rows the sums no longer fit, and the wide kernel is faster even with planes (fp32 x 768, 64
-// queries: 994 against 669 us; x 512 519 / 649 us, with 128 queries 1078 / 838 us; fp16 x 512 in place 238 - 333 / 150 - 160 us).  Statistics alone
+// queries: 994 against 669 us; 488k x 512 559 / 622 us, with 128 queries 1042 / 802 us; fp16 500k x 512 in place, 8 - 64 queries 209 - 241 / 113 - 127 us).  Statistics alone
 // are the thin kernel's up to 512 elements in place (111 / 121 us; x 1024 131 / 122 us) and at all widths with planes.
 bool thin_of(int dtype, int mode, int ks, uint32_t nx, bool direct) {
     const bool f32 = dtype == RG_DTYPE_F32;

@@ -22,7 +22,7 @@ struct WideChoice {
 };
 // Measured (2000 queries, 30M elements of base, training step; with spills: the form whose registers were not enough): fp32 x 512 one wave a row
 // 1.82 ms, two 1.57 ms; x 768 four waves, 16 rows each 2.31 ms, 32 rows (spills) 2.80 ms, one wave (spills) 6.07 ms; fp16 x 512 one wave, 16 rows
-// 0.62 ms, two waves, 32 rows (spills) 1.10 ms; x 1024 four waves 1.10 ms, one (spills) 5.59 ms.  Statistics alone: fp16 x 768 one wave 0.14 ms,
+// 0.62 ms, two waves, 32 rows (spills) 1.10 ms; x 1024 four waves 0.93 ms, one (spills) 5.59 ms.  Statistics alone: fp16 x 768 one wave 0.14 ms,
 // four 0.26 ms; fp32 x 768 four waves, 32 rows 0.56 ms, one 0.93 ms.
 constexpr WideChoice softmax_wide_cfg(int dt, int ks, int mode) {
     const bool f32 = dt == RG_DTYPE_F32;
