@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 import torch
 
+import test_gpu_softmax
 from roargraph_amd import softmax
 from test_gpu_softmax import DT, U, exact, make, step, tolerances, within
 
@@ -299,3 +300,12 @@ def test_a_whole_step_is_captured():
         torch.cuda.synchronize()
         for a, b, c in zip(out, eager, want[k]):
             assert torch.equal(a, c) and torch.equal(b, c), k
+
+
+# ---- the kernels that the shapes of test_gpu_softmax leave out: widths, types and numbers of queries in other pairs
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nq,nb,dim", [(300, 900, 37), (300, 900, 93), (40, 900, 96), (260, 700, 201), (270, 700, 243), (80, 900, 256), (200, 700, 256), (20, 600, 320), (30, 600, 350), (300, 500, 509),
+                                       (20, 500, 512), (300, 400, 701), (300, 300, 1001), (20, 400, 1001)])
+def test_loss_and_gradients_of_other_pairs(nq, nb, dim, dtype):
+    test_gpu_softmax.test_loss_and_gradients(nq, nb, dim, dtype)
